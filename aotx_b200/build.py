@@ -18,8 +18,11 @@ LIB = os.path.join(HERE, "libaotx_q8_b200.so")
 CALLS = os.path.join(HERE, "_host_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
 SOURCES = ["q8_api.cu", "q8_simt.cu", "q8_dispatch.cu", "q8_stream.cu", "q8_decode.cu", "q8_decode_warp.cu", "q8_decode_rows.cu", "q8_mid.cu", "q8_pair.cu", "q8_wide.cu", "q8_static.cu", "q8_moe.cu", "q8_route.cu", "q8_peers.cu",
            "q_generic.cu", "q_warp.cu", "gguf_table.cpp", "gguf_upload.cu"]
+# The MX4 tensors (include/aotx_mx4_b200.h), in the same library.
+MX4_SOURCES = ["mx4_api.cu", "mx4_quant.cu", "mx4_product.cu", "mx4_order.cu"]
 HEADERS = ["q8_common.cuh", "q8_ptx.cuh", "q8_warp_ptx.cuh", "q8_rows.cuh", "q8_schedule.cuh", "q8_decode_operands.cuh", "q8_store.cuh", "q8_simt_gemv.cuh", "q8_route.cuh", "q8_launch.h", "q8_tile.cuh", "q_blocks.cuh", os.path.join("..", "..", "include", "aotx_q8_b200.h"),
-           os.path.join("..", "..", "include", "aotx_gguf_b200.h")]
+           os.path.join("..", "..", "include", "aotx_gguf_b200.h"), "q8_context.h"]
+MX4_HEADERS = ["mx4.h", "mx4_ptx.cuh", os.path.join("..", "..", "include", "aotx_mx4_b200.h")]
 NVCC_FLAGS = ["-std=c++17", "-O3", "-lineinfo", "-gencode", "arch=compute_100a,code=sm_100a",
               "-Xcompiler", "-fPIC", "-Xptxas", "-v"]
 
@@ -33,7 +36,7 @@ def _stale(target, deps):
 
 def _compile(src):
     obj = os.path.join(OBJ, os.path.splitext(src)[0] + ".o")
-    deps = [os.path.join(CSRC, src)] + [os.path.join(CSRC, h) for h in HEADERS]
+    deps = [os.path.join(CSRC, src)] + [os.path.join(CSRC, h) for h in HEADERS + (MX4_HEADERS if src in MX4_SOURCES else [])]
     log = obj + ".ptxas.log"   # what ptxas -v said for this object: registers, spills, shared memory
     if not _stale(obj, deps) and os.path.exists(log):
         return obj, ""
@@ -46,12 +49,12 @@ def _compile(src):
     return obj, done.stderr
 
 
-def resource_usage():
+def resource_usage(sources=tuple(SOURCES)):
     """{kernel or out-of-line function (mangled): {"registers": r (kernels only), "spill_stores": s,
     "spill_loads": l, "stack": b}} from the ptxas reports kept beside the objects (build() first)."""
     import re
     usage = {}
-    for src in SOURCES:
+    for src in sources:
         log = os.path.join(OBJ, os.path.splitext(src)[0] + ".o.ptxas.log")
         if not os.path.exists(log):
             continue
@@ -90,8 +93,8 @@ def _build_calls(include=sysconfig.get_paths()["include"]):
 
 def build(verbose=False):
     os.makedirs(OBJ, exist_ok=True)
-    with ThreadPoolExecutor(max_workers=len(SOURCES)) as pool:
-        results = list(pool.map(_compile, SOURCES))
+    with ThreadPoolExecutor(max_workers=len(SOURCES + MX4_SOURCES)) as pool:
+        results = list(pool.map(_compile, SOURCES + MX4_SOURCES))
     objs = [r[0] for r in results]
     log = "".join(r[1] for r in results)
     if log:

@@ -1,0 +1,49 @@
+// Internal launch interface of the MX4 kernels (mx4_api.cu calls them; the format is described in include/aotx_mx4_b200.h).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace q8 {
+
+constexpr uint32_t kMx4MaxExperts = 256u;
+
+__host__ __device__ inline uint32_t mx4_chunks(uint32_t k)
+{
+    return (k + 127u) / 128u;   // words of four scales in a row
+}
+
+cudaError_t launch_mx4_quantize(cudaStream_t stream, bool overlap, const void *x, int x_dtype, uint32_t x_rows,
+                                unsigned long long ldx, uint32_t k, const uint32_t *rows_of, uint32_t rows,
+                                const uint32_t *rows_dev, uint32_t *codes, uint32_t *scales);
+cudaError_t launch_mx4_dequant(cudaStream_t stream, bool overlap, const uint32_t *codes, const uint8_t *scales,
+                               uint32_t total_rows, uint32_t k, uint32_t first_row, uint32_t rows, void *out, int out_dtype);
+
+// A product, or (offsets not null) products grouped by expert.
+struct Mx4Product {
+    const void *w_codes;
+    const uint32_t *w_scales;
+    uint32_t experts;          // 1 for a plain product
+    uint32_t n, k;
+    const void *x_codes;
+    const uint32_t *x_scales;
+    uint32_t m;                // rows of x
+    const uint32_t *m_dev;
+    const uint32_t *offsets;
+    const uint32_t *y_rows_of;
+    uint32_t y_rows;
+    void *y;
+    int y_dtype;
+    unsigned int epilogue;
+    unsigned int *status;
+    bool overlap;
+    bool weights_late;         // the operation before this one writes them
+};
+cudaError_t launch_mx4_product(cudaStream_t stream, unsigned int sm_count, const Mx4Product &p);
+
+cudaError_t launch_mx4_order(cudaStream_t stream, bool overlap, const uint32_t *ids, uint32_t tokens,
+                             const uint32_t *tokens_dev, uint32_t used, uint32_t experts, uint32_t *order, uint32_t *token_of,
+                             uint32_t *offsets);
+
+} // namespace q8

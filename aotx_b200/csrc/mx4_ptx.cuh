@@ -1,0 +1,62 @@
+// The instructions of the MX4 kernels that the Q8_0 kernels do not use, one small function each.
+#pragma once
+
+#include <stdint.h>
+
+namespace q8 {
+
+// Eight floats to eight E2M1 codes in a word, v[0] in the lowest four bits: nearest, ties to even, saturating at 6.
+__device__ __forceinline__ uint32_t cvt_e2m1x8(const float (&v)[8])
+{
+    uint32_t out;
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+        "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+        : "=r"(out)
+        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+    return out;
+}
+
+// The eight values of a word of codes as pairs of binary16, out[0] the two lowest.
+__device__ __forceinline__ void cvt_f16x2_e2m1(uint32_t codes, uint32_t (&out)[4])
+{
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+        : "=r"(out[0]), "=r"(out[1]), "=r"(out[2]), "=r"(out[3])
+        : "r"(codes));
+}
+
+// A thread's own copy of four bytes, global to shared; zeros where `bytes` is 0 (the source is not read then).
+__device__ __forceinline__ void copy_async_4(uint32_t dst, const void *src, uint32_t bytes)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+// 32 rows of 16 bytes from shared memory (a descriptor without swizzle) to four columns of tensor memory, the same in each
+// quarter of the lanes: the way a block of scales is laid down for the MMA.
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc)
+{
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+// D[tmem] (+)= A[smem] * B[smem], one 128 x N x 64 step of E2M1 codes with a scale (a power of two) per 32 values of
+// either, scales in tensor memory, float sums.
+__device__ __forceinline__ void umma_mx4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scales,
+                                         uint32_t b_scales, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate)
+        : "memory");
+}
+
+} // namespace q8

@@ -7,17 +7,8 @@
 #include <new>
 
 #include "q8_common.cuh"
+#include "q8_context.h"
 #include "q8_launch.h"
-
-struct aotx_q8_ctx {
-    int device;
-    unsigned int sm_count;
-    int path;
-    int last_cuda;
-    int overlap;
-    unsigned int launches;
-    q8::UmmaScratch scratch;
-};
 
 namespace {
 

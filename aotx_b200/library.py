@@ -31,6 +31,12 @@ GGUF_SYMBOLS = (
     "aotx_gguf_upload", "aotx_gguf_upload_rows",
 )
 
+# every symbol include/aotx_mx4_b200.h declares
+MX4_SYMBOLS = (
+    "aotx_mx4_quantize", "aotx_mx4_dequant", "aotx_mx4_matmul", "aotx_mx4_linear_workspace_bytes", "aotx_mx4_linear",
+    "aotx_mx4_moe_order", "aotx_mx4_matmul_grouped",
+)
+
 
 class TensorInfo(C.Structure):
     """aotx_gguf_tensor_info of include/aotx_gguf_b200.h."""
@@ -61,6 +67,7 @@ def load_library():
     lib = C.CDLL(LIB_PATH)
     declare_q8(lib)
     declare_gguf(lib)
+    declare_mx4(lib)
     _lib = lib
     return lib
 
@@ -71,6 +78,8 @@ def native_call(lib, name):
     try:
         from . import _host_calls
     except ImportError:
+        return getattr(lib, name)
+    if not hasattr(_host_calls, name):      # a module of an earlier build
         return getattr(lib, name)
     return functools.partial(getattr(_host_calls, name), C.cast(getattr(lib, name), C.c_void_p).value)
 
@@ -110,6 +119,21 @@ def declare_q8(lib):
         fn = getattr(lib, name)
         if name not in ("aotx_q8_moe_workspace_bytes", "aotx_q8_moe_ep_workspace_bytes"):
             fn.restype = i32
+
+
+def declare_mx4(lib):
+    """Argument and result types of every entry point of include/aotx_mx4_b200.h."""
+    vp, u32, i32, u64 = C.c_void_p, C.c_uint32, C.c_int, C.c_uint64
+    lib.aotx_mx4_quantize.argtypes = [vp, vp, vp, i32, u32, u64, u32, vp, u32, vp, vp, vp]
+    lib.aotx_mx4_dequant.argtypes = [vp, vp, vp, vp, u32, u32, u32, u32, vp, i32]
+    lib.aotx_mx4_matmul.argtypes = [vp, vp, vp, vp, u32, u32, vp, vp, u32, vp, vp, i32, i32]
+    lib.aotx_mx4_linear_workspace_bytes.argtypes = [u32, u32]
+    lib.aotx_mx4_linear.argtypes = [vp, vp, vp, vp, u32, u32, vp, i32, u64, u32, vp, vp, i32, i32, vp, C.c_size_t]
+    lib.aotx_mx4_moe_order.argtypes = [vp, vp, vp, u32, vp, u32, u32, vp, vp, vp]
+    lib.aotx_mx4_matmul_grouped.argtypes = [vp, vp, vp, vp, u32, u32, u32, vp, vp, u32, vp, vp, u32, vp, i32, i32]
+    for name in MX4_SYMBOLS:
+        getattr(lib, name).restype = i32
+    lib.aotx_mx4_linear_workspace_bytes.restype = C.c_size_t
 
 
 def declare_gguf(lib):

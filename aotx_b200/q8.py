@@ -9,6 +9,7 @@ import ctypes as C
 import numpy as np
 
 from .library import load_library, native_call
+from .mx4 import Mx4Calls
 
 Q8_0 = 8  # cuda/model/model.cuh:31
 F32, F16, BF16 = 0, 1, 2
@@ -111,7 +112,7 @@ def _dtype_code(dtype):
     return code
 
 
-class Q8Context:
+class Q8Context(Mx4Calls):
     """One per device: owns the scratch of the streaming kernel (aotx_q8_init)."""
 
     def __init__(self, device=0):
@@ -130,6 +131,12 @@ class Q8Context:
         self._matmul = native_call(self.lib, "aotx_q8_matmul")
         self._matmul_fused = native_call(self.lib, "aotx_q8_matmul_fused")
         self._dequant = native_call(self.lib, "aotx_q8_dequant")
+        self._mx4_quantize_call = native_call(self.lib, "aotx_mx4_quantize")
+        self._mx4_dequant_call = native_call(self.lib, "aotx_mx4_dequant")
+        self._mx4_matmul_call = native_call(self.lib, "aotx_mx4_matmul")
+        self._mx4_linear_call = native_call(self.lib, "aotx_mx4_linear")
+        self._mx4_order_call = native_call(self.lib, "aotx_mx4_moe_order")
+        self._mx4_grouped_call = native_call(self.lib, "aotx_mx4_matmul_grouped")
         # The current stream as a number.  (Through the Stream object it took 2.4 us of the 8.2 us
         # that the smallest product keeps the host; this takes 0.1.)
         self._device_index = self.device.index

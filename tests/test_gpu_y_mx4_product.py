@@ -1,0 +1,324 @@
+"""Products of MX4 tensors against the sums in 64 bits (tests/_mx4.py), plain and grouped by expert."""
+import numpy as np
+import pytest
+
+import _mx4
+from _util import GUARD, torch_mod
+
+pytestmark = pytest.mark.gpu
+STORE, ADD, SWIGLU = 0, 1, 2
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    import aotx_b200
+    made = aotx_b200.Q8Context(0)
+    yield made
+    assert made.device_status() == 0
+    made.close()
+
+
+def dtype(name):
+    torch = torch_mod()
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[name]
+
+
+def tensor(codes, scales):
+    import aotx_b200
+    torch = torch_mod()
+    return aotx_b200.Mx4Tensor(torch.from_numpy(codes).cuda(), torch.from_numpy(scales).cuda())
+
+
+def random_codes(rows, k, seed, low, high):
+    """Codes of every kind and scales 2^low .. 2^high."""
+    rng = np.random.Generator(np.random.PCG64(seed))
+    codes = rng.integers(0, 256, (rows, k // 2), dtype=np.uint8)
+    chunks = (k + 127) // 128
+    flat = np.zeros((rows, chunks * 4), np.uint8)
+    flat[:, :k // 32] = rng.integers(127 + low, 128 + high, (rows, k // 32))
+    return codes, np.ascontiguousarray(flat.reshape(rows, chunks, 4).transpose(1, 0, 2))
+
+
+# one block; one tile; tiles cut by every edge; a depth that ends inside a stage, inside a word of scales
+SHAPES = [(128, 64, 16), (16, 32, 1), (1, 32, 3), (130, 96, 5), (127, 256, 17), (300, 416, 33), (129, 1056, 100), (512, 512, 128),
+          (260, 320, 129), (257, 288, 200), (200, 1024, 256), (140, 192, 257), (388, 544, 513), (64, 4096, 2)]
+
+
+@pytest.mark.parametrize("n,k,m", SHAPES)
+def test_exact_sums(ctx, n, k, m):
+    """Scales 2^-2 .. 2^2: products are multiples of 2^-6, and where the magnitudes of a sum add up to less than 2^18 floats hold
+    every partial sum: the result is the sum itself."""
+    w, x = random_codes(n, k, n + k, -2, 2), random_codes(m, k, m + k + 1, -2, 2)
+    want = _mx4.values(*x) @ _mx4.values(*w).T
+    assert (np.abs(_mx4.values(*x)) @ np.abs(_mx4.values(*w)).T).max() < 2.0 ** 18
+    torch = torch_mod()
+    y = torch.full((m + 1, n), GUARD, device="cuda")
+    got = ctx.mx4_matmul(tensor(*w), tensor(*x), y=y[:m]).cpu().numpy()
+    assert np.array_equal(got, want.astype(np.float32))
+    assert (y[m:] == GUARD).all()
+
+
+@pytest.mark.parametrize("out", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,k,m", [(130, 96, 5), (300, 416, 33), (388, 544, 140), (256, 1024, 300), (1000, 512, 8)])
+def test_types_and_epilogues(ctx, n, k, m, out):
+    torch = torch_mod()
+    w, x = random_codes(n, k, n, -9, -3), random_codes(m, k, m, -4, 3)
+    w64, x64 = _mx4.values(*w), _mx4.values(*x)
+    want, error = x64 @ w64.T, _mx4.sum_bound(w64, x64)
+    dw, dx = tensor(*w), tensor(*x)
+    got = ctx.mx4_matmul(dw, dx, y_dtype=dtype(out)).double().cpu().numpy()
+    assert _mx4.close(got, want, error, out).all()
+    got = ctx.mx4_matmul(dw, dx, y_dtype=dtype(out), epilogue=SWIGLU).double().cpu().numpy()
+    assert got.shape == (m, n // 2)
+    assert _mx4.close(got, _mx4.gated(want), _mx4.gated_bound(want, error), out).all()
+    if out == "f32":
+        before = torch.randn((m, n), device="cuda")
+        y = before.clone()
+        ctx.mx4_matmul(dw, dx, y=y, epilogue=ADD)
+        plain = ctx.mx4_matmul(dw, dx)
+        assert torch.equal(y, before + plain)
+
+
+@pytest.mark.parametrize("m,live", [(1, 0), (1, 1), (40, 17), (40, 99), (300, 0), (300, 5), (300, 256), (300, 290)])
+def test_live_batch(ctx, m, live):
+    torch = torch_mod()
+    n, k = 200, 320
+    w, x = random_codes(n, k, 1, -2, 2), random_codes(m, k, 2, -2, 2)
+    want = _mx4.values(*x) @ _mx4.values(*w).T
+    y = torch.full((m, n), GUARD, device="cuda")
+    word = torch.tensor([live], dtype=torch.int32, device="cuda")
+    ctx.mx4_matmul(tensor(*w), tensor(*x), y=y, m_dev=word)
+    got = y.cpu().numpy()
+    rows = min(live, m)
+    assert np.array_equal(got[:rows], want[:rows].astype(np.float32)) and (got[rows:] == GUARD).all()
+
+
+def test_y_off_a_boundary_and_scale_nan(ctx):
+    torch = torch_mod()
+    n, k, m = 66, 128, 9
+    w, x = random_codes(n, k, 1, -2, 2), random_codes(m, k, 2, -2, 2)
+    x[1][0, 3, 2] = 255      # a block of row 3 is not a number, and with it the row
+    want = _mx4.values(*x) @ _mx4.values(*w).T
+    flat = torch.full((m * n + 3,), GUARD, device="cuda")
+    for name in ("f32", "f16", "bf16"):
+        flat = torch.full((m * n + 3,), GUARD, device="cuda", dtype=dtype(name))
+        y = flat[1:1 + m * n].view(m, n)
+        ctx.mx4_matmul(tensor(*w), tensor(*x), y=y)
+        got = y.double().cpu().numpy()
+        rows = np.arange(m) != 3
+        assert np.isnan(got[3]).all()
+        assert _mx4.close(got[rows], want[rows], 0.0, name).all()
+        assert flat[0] == flat[m * n + 1] == flat[m * n + 2] == torch.tensor(GUARD, dtype=flat.dtype)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,k,m", [(130, 96, 1), (300, 416, 5), (200, 2080, 16), (4096, 512, 8), (140, 1056, 17), (200, 96, 33),
+                                   (260, 320, 100), (130, 64, 300)])
+def test_linear_is_quantisation_and_product(ctx, n, k, m, kind):
+    torch = torch_mod()
+    w = tensor(*random_codes(n, k, n, -9, -3))
+    gen = torch.Generator().manual_seed(m)
+    x = torch.randn((m, k + 8), generator=gen)
+    x[m // 2, :32] = 0
+    x = x.to(dtype(kind)).cuda()
+    for view in (x[:, :k].contiguous(), x[:, 8:], x[:, 1:k + 1]):
+        q = ctx.mx4_quantize(view)
+        assert torch.equal(ctx.mx4_linear(w, view), ctx.mx4_matmul(w, q))
+        for out in ("f16", "bf16"):
+            assert torch.equal(ctx.mx4_linear(w, view, y_dtype=dtype(out), epilogue=SWIGLU),
+                               ctx.mx4_matmul(w, q, y_dtype=dtype(out), epilogue=SWIGLU))
+        y = torch.ones((m, n), device="cuda")
+        ctx.mx4_linear(w, view, y=y, epilogue=ADD)
+        assert torch.equal(y, 1 + ctx.mx4_matmul(w, q))
+        live = torch.tensor([m // 2], dtype=torch.int32, device="cuda")
+        y = torch.full((m, n), GUARD, device="cuda")
+        ctx.mx4_linear(w, view, y=y, m_dev=live)
+        assert torch.equal(y[:m // 2], ctx.mx4_matmul(w, q)[:m // 2]) and (y[m // 2:] == GUARD).all()
+
+
+def test_linear_takes_not_a_number_into_its_row_only(ctx):
+    torch = torch_mod()
+    w = tensor(*random_codes(256, 512, 3, -9, -3))
+    for m in (4, 40):
+        x = torch.randn((m, 512), device="cuda").half()
+        clean = ctx.mx4_linear(w, x)
+        x[1, 100] = float("inf")
+        y = ctx.mx4_linear(w, x)
+        assert torch.isnan(y[1]).all()
+        rows = torch.arange(m, device="cuda") != 1
+        assert torch.equal(y[rows], clean[rows])
+
+
+def order_of(ids, experts, live):
+    flat = ids[:live].reshape(-1)
+    lists = [np.nonzero(flat == e)[0] for e in range(experts)]
+    return np.concatenate(lists), np.cumsum([0] + [len(part) for part in lists])
+
+
+@pytest.mark.parametrize("tokens,used,experts", [(1, 1, 1), (1, 8, 128), (8, 8, 128), (7, 3, 5), (77, 4, 20), (512, 8, 128),
+                                                 (300, 2, 256), (2048, 8, 64), (33, 1, 3)])
+def test_order(ctx, tokens, used, experts):
+    torch = torch_mod()
+    rng = np.random.Generator(np.random.PCG64(tokens))
+    ids = np.argsort(rng.standard_normal((tokens, experts)) + rng.standard_normal(experts), axis=1)[:, :used].astype(np.int32)
+    strange = ids.copy()
+    strange[rng.random(ids.shape) < 0.2] = -1
+    strange[rng.random(ids.shape) < 0.1] = experts
+    one = np.zeros_like(ids)
+    for chosen in (ids, strange, one, np.full_like(ids, -1)):
+        for live in (None, 0, tokens // 2, tokens, tokens + 9):
+            word = None if live is None else torch.tensor([live], dtype=torch.int32, device="cuda")
+            got = [t.cpu().numpy() for t in ctx.moe_order(torch.from_numpy(chosen).cuda(), experts, tokens_dev=word)]
+            want, offsets = order_of(chosen, experts, tokens if live is None else min(live, tokens))
+            assert np.array_equal(got[2], offsets)
+            assert np.array_equal(got[0][:len(want)], want) and (got[0][len(want):] == -1).all()
+            assert np.array_equal(got[1][:len(want)], want // used) and (got[1][len(want):] == -1).all()
+
+
+@pytest.mark.parametrize("counts", [[5], [0, 3, 0, 0, 129, 1, 0], [0] * 7, [16] * 20, [0] * 255 + [40], [1] * 256, [600, 0, 2],
+                                    [300, 20, 257, 31]])
+@pytest.mark.parametrize("n,k", [(96, 160), (260, 512)])
+def test_grouped(ctx, counts, n, k):
+    """Every expert's rows by its own matrix; rows behind the last expert's stay as they are."""
+    torch = torch_mod()
+    experts, spare = len(counts), 3
+    rows = sum(counts) + spare
+    edges = np.cumsum([0] + counts)
+    w, x = random_codes(experts * n, k, n, -2, 2), random_codes(rows, k, rows, -2, 2)
+    w64, x64 = _mx4.values(*w), _mx4.values(*x)
+    want = np.full((rows, n), GUARD)
+    for e in range(experts):
+        want[edges[e]:edges[e + 1]] = x64[edges[e]:edges[e + 1]] @ w64[e * n:e * n + n].T
+    offsets = torch.from_numpy(edges.astype(np.int32)).cuda()
+    dw, dx = tensor(*w), tensor(*x)
+    y = torch.full((rows, n), GUARD, device="cuda")
+    ctx.mx4_matmul_grouped(dw, experts, dx, offsets, y=y)
+    assert np.array_equal(y.cpu().numpy(), want.astype(np.float32))
+    # rows to places of their own, some outside y
+    rng = np.random.Generator(np.random.PCG64(3))
+    places = rng.permutation(rows + 4)[:rows].astype(np.int32)
+    places[rng.random(rows) < 0.1] = -1
+    scattered = np.full((rows, n), GUARD)
+    for i in range(edges[-1]):
+        if 0 <= places[i] < rows:
+            scattered[places[i]] = want[i]
+    y = torch.full((rows, n), GUARD, device="cuda")
+    ctx.mx4_matmul_grouped(dw, experts, dx, offsets, y_rows=torch.from_numpy(places).cuda(), y=y)
+    assert np.array_equal(y.cpu().numpy(), scattered.astype(np.float32))
+    for out in ("f16", "bf16"):
+        act = torch.full((rows, n // 2), GUARD, device="cuda", dtype=dtype(out))
+        ctx.mx4_matmul_grouped(dw, experts, dx, offsets, y=act, epilogue=SWIGLU)
+        got = act.double().cpu().numpy()
+        assert (act[edges[-1]:] == torch.tensor(GUARD, dtype=act.dtype)).all()
+        if edges[-1]:
+            placed = want[:edges[-1]]
+            bound = _mx4.gated_bound(placed, np.zeros_like(placed))
+            assert _mx4.close(got[:edges[-1]], _mx4.gated(placed), bound, out).all()
+
+
+def test_offsets_that_make_no_sense_reach_nothing_outside(ctx):
+    torch = torch_mod()
+    experts, n, k, rows = 4, 64, 64, 50
+    w, x = tensor(*random_codes(experts * n, k, 1, -2, 2)), tensor(*random_codes(rows, k, 2, -2, 2))
+    guard = torch.full((rows + 2, n), GUARD, device="cuda")
+    for offsets in ([0, 10, 5, 60, 70], [-5, 20, 20, 30, 2 ** 31 - 1], [50, 40, 30, 20, 10], [60, 61, 62, 63, 64]):
+        ctx.mx4_matmul_grouped(w, experts, x, torch.tensor(offsets, dtype=torch.int32, device="cuda"), y=guard[1:-1])
+        torch.cuda.synchronize()
+        assert (guard[0] == GUARD).all() and (guard[-1] == GUARD).all()
+
+
+@pytest.mark.parametrize("tokens,used,experts,hidden,ffn", [(1, 2, 8, 256, 160), (8, 8, 128, 512, 256), (77, 4, 20, 544, 96),
+                                                            (300, 2, 4, 256, 256)])
+def test_routed_step(ctx, tokens, used, experts, hidden, ffn):
+    """The calls of a routed layer as they are used together.  The activations between the two products are rounded to four bits, so
+    the second product is held to what the first one gave: each step is checked on the step before it."""
+    torch = torch_mod()
+    w_gate_up = random_codes(experts * 2 * ffn, hidden, 1, -9, -5)
+    w_down = random_codes(experts * hidden, ffn, 2, -9, -5)
+    gen = torch.Generator().manual_seed(tokens)
+    x = torch.randn((tokens, hidden), generator=gen).half().cuda()
+    router = torch.randn((experts, hidden), generator=gen).cuda()
+    prob, ids = ctx.moe_route(x, router, used)
+    out = ctx.mx4_moe_ffn(tensor(*w_gate_up), tensor(*w_down), experts, x, prob, ids)
+    order, token_of, offsets = ctx.moe_order(ids, experts)
+    feed = ctx.mx4_quantize(x, rows=token_of)
+    act = ctx.mx4_matmul_grouped(tensor(*w_gate_up), experts, feed, offsets, y_dtype=torch.float16, epilogue=SWIGLU)
+    ids_host, edges = ids.cpu().numpy(), offsets.cpu().numpy()
+    want_order, want_edges = order_of(ids_host, experts, tokens)
+    assert np.array_equal(order.cpu().numpy(), want_order) and np.array_equal(edges, want_edges)
+    x64 = _mx4.values(*_mx4.quantize(x.cpu().double().numpy()[want_order // used]))
+    gate_up64, down64 = _mx4.values(*w_gate_up), _mx4.values(*w_down)
+    act64 = _mx4.values(*_mx4.quantize(act.cpu().double().numpy()))
+    proj64, proj_error = np.zeros((tokens * used, hidden)), np.zeros((tokens * used, hidden))
+    for e in range(experts):
+        a, b = edges[e], edges[e + 1]
+        w64 = gate_up64[e * 2 * ffn:(e + 1) * 2 * ffn]
+        y64, error = x64[a:b] @ w64.T, _mx4.sum_bound(w64, x64[a:b])
+        assert _mx4.close(act.cpu().double().numpy()[a:b], _mx4.gated(y64), _mx4.gated_bound(y64, error), "f16").all()
+        w64 = down64[e * hidden:(e + 1) * hidden]
+        proj64[want_order[a:b]] = act64[a:b] @ w64.T
+        proj_error[want_order[a:b]] = _mx4.sum_bound(w64, act64[a:b])
+    chosen = np.take_along_axis(prob.cpu().double().numpy(), ids_host.astype(np.int64), axis=1)[:, :, None]
+    want = (proj64.reshape(tokens, used, hidden) * chosen).sum(axis=1)
+    parts = (np.abs(proj64).reshape(tokens, used, hidden) * chosen).sum(axis=1)
+    error = (proj_error.reshape(tokens, used, hidden) * chosen).sum(axis=1)
+    # each rank: a rounded product and a rounded sum
+    assert (np.abs(out.cpu().double().numpy() - want) <= error + parts * (2 * used) * 2.0 ** -24).all()
+    # selections that name no expert, and tokens past the live ones
+    ids[0, 0] = experts + 3
+    live = torch.tensor([max(tokens - 1, 1)], dtype=torch.int32, device="cuda")
+    got = torch.full((tokens, hidden), GUARD, device="cuda")
+    ctx.mx4_moe_ffn(tensor(*w_gate_up), tensor(*w_down), experts, x, prob, ids, tokens_dev=live, out=got)
+    rows = int(live)
+    assert torch.equal(got[1:rows], out[1:rows])
+    assert (got[rows:] == GUARD).all()
+    part = (proj64.reshape(tokens, used, hidden) * chosen)[0, 1:].sum(axis=0)
+    assert (np.abs(got[0].cpu().double().numpy() - part) <= error[0] + parts[0] * (2 * used) * 2.0 ** -24).all()
+
+
+def test_weights_quantised_just_before(ctx):
+    """A product right behind the quantisation of its weights, and behind one of other rows, reads what they wrote."""
+    torch = torch_mod()
+    n, k = 4096, 2048
+    for m in (3, 300):
+        x = ctx.mx4_quantize(torch.randn((m, k), device="cuda"))
+        out = ctx.mx4_quantize(torch.zeros((n, k), device="cuda"))
+        for turn in range(8):
+            w = torch.randn((n, k), device="cuda").half()
+            ctx.mx4_quantize(w, out=out)
+            if turn % 2:
+                x = ctx.mx4_quantize(torch.randn((m, k), device="cuda"))
+            y = ctx.mx4_matmul(out, x)
+            torch.cuda.synchronize()
+            assert torch.equal(ctx.mx4_matmul(out, x), y)
+
+
+@pytest.mark.parametrize("m", [1, 8, 40, 300])
+def test_captured_twice_and_on_another_stream(ctx, m):
+    """Two graphs of the same calls, replayed in turn with new inputs, and the calls on a second stream."""
+    torch = torch_mod()
+    n, k = 520, 544
+    w = tensor(*random_codes(n, k, 3, -9, -3))
+    x = torch.randn((m, k), device="cuda").half()
+    ys = [torch.empty((m, n), device="cuda") for _ in range(2)]
+    ctx.mx4_linear(w, x, y=ys[0])
+    torch.cuda.synchronize()
+    graphs = []
+    for y in ys:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ctx.mx4_linear(w, x, y=y)
+            ctx.mx4_linear(w, x, y=y, epilogue=ADD)
+        graphs.append(graph)
+    for turn in range(4):
+        x.copy_(torch.randn((m, k), device="cuda").half())
+        graphs[turn % 2].replay()
+        torch.cuda.synchronize()
+        once = ctx.mx4_matmul(w, ctx.mx4_quantize(x))
+        assert torch.equal(ys[turn % 2], once + once)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = ctx.mx4_linear(w, x)
+    side.synchronize()
+    assert torch.equal(other, ctx.mx4_linear(w, x))
