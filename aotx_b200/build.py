@@ -87,7 +87,8 @@ def _build_calls(include=sysconfig.get_paths()["include"]):
     if not os.path.exists(os.path.join(include, "Python.h")) or shutil.which("gcc") is None:
         print("no Python headers or no gcc: " + os.path.basename(CALLS) + " is not built", file=sys.stderr)
         return
-    if _stale(CALLS, [calls, os.path.join(CSRC, "..", "..", "include", "aotx_q8_b200.h")]):
+    headers = [os.path.join(CSRC, "..", "..", "include", name) for name in ("aotx_q8_b200.h", "aotx_mx4_b200.h")]
+    if _stale(CALLS, [calls, *headers]):
         subprocess.run(["gcc", "-O2", "-Wall", "-Werror", "-shared", "-fPIC", "-I" + include, "-o", CALLS, calls], check=True)
 
 

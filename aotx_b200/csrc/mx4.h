@@ -5,6 +5,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "q8_launch.h"
+
 namespace q8 {
 
 constexpr uint32_t kMx4MaxExperts = 256u;
@@ -36,11 +38,17 @@ struct Mx4Product {
     void *y;
     int y_dtype;
     unsigned int epilogue;
-    unsigned int *status;
     bool overlap;
     bool weights_late;         // the operation before this one writes them
+    // x in 16 or 32 bits instead of MX4 (null: x_codes and x_scales), where mx4_linear_quantizes
+    const void *x;
+    int x_dtype;
+    unsigned long long ldx;
 };
-cudaError_t launch_mx4_product(cudaStream_t stream, unsigned int sm_count, const Mx4Product &p);
+cudaError_t launch_mx4_product(cudaStream_t stream, const UmmaScratch &scratch, unsigned int sm_count, unsigned int set,
+                               const Mx4Product &p);
+// Does the product's kernel quantise x itself?
+bool mx4_linear_quantizes(uint32_t n, uint32_t k, uint32_t m, unsigned int sm_count);
 
 cudaError_t launch_mx4_order(cudaStream_t stream, bool overlap, const uint32_t *ids, uint32_t tokens,
                              const uint32_t *tokens_dev, uint32_t used, uint32_t experts, uint32_t *order, uint32_t *token_of,

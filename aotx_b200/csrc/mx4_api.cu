@@ -172,14 +172,16 @@ extern "C" int aotx_mx4_matmul(aotx_q8_ctx *ctx, void *stream, const void *w_cod
     p.y = y;
     p.y_dtype = y_dtype;
     p.epilogue = (unsigned int)epilogue;
-    p.status = ctx->scratch.status;
     p.overlap = ctx->overlap != 0;
     p.weights_late = fresh(ctx, w_codes, code_bytes(n, k)) || fresh(ctx, w_scales, scale_bytes(n, k));
-    return code_of(ctx, q8::launch_mx4_product((cudaStream_t)stream, ctx->sm_count, p));
+    return code_of(ctx, q8::launch_mx4_product((cudaStream_t)stream, ctx->scratch, ctx->sm_count, ctx->launches++, p));
 }
 
-extern "C" size_t aotx_mx4_linear_workspace_bytes(uint32_t m, uint32_t k)
+extern "C" size_t aotx_mx4_linear_workspace_bytes(const aotx_q8_ctx *ctx, uint32_t n, uint32_t k, uint32_t m)
 {
+    if (ctx == nullptr || !depth(k) || n == 0u || m == 0u || q8::mx4_linear_quantizes(n, k, m, ctx->sm_count)) {
+        return 0u;
+    }
     return (code_bytes(m, k) + 255u) / 256u * 256u + scale_bytes(m, k);
 }
 
@@ -198,15 +200,36 @@ extern "C" int aotx_mx4_linear(aotx_q8_ctx *ctx, void *stream, const void *w_cod
         || !aligned(y, size_of(y_dtype)) || !aligned(m_dev, 4u)) {
         return AOTX_Q8_ERR_ARGUMENT;
     }
-    const size_t need = aotx_mx4_linear_workspace_bytes(m, k);
-    if (need != 0u && (workspace == nullptr || !aligned(workspace, 16u) || workspace_bytes < need)) {
-        return AOTX_Q8_ERR_WORKSPACE;
+    const size_t need = aotx_mx4_linear_workspace_bytes(ctx, n, k, m);
+    if (need != 0u) {
+        if (workspace == nullptr || !aligned(workspace, 16u) || workspace_bytes < need) {
+            return AOTX_Q8_ERR_WORKSPACE;
+        }
+        unsigned char *codes = static_cast<unsigned char *>(workspace);
+        unsigned char *scales = codes + (code_bytes(m, k) + 255u) / 256u * 256u;
+        const int code = aotx_mx4_quantize(ctx, stream, x, x_dtype, m, ldx, k, nullptr, m, m_dev, codes, scales);
+        return code != AOTX_Q8_OK ? code
+             : aotx_mx4_matmul(ctx, stream, w_codes, w_scales, n, k, codes, scales, m, m_dev, y, y_dtype, epilogue);
     }
-    unsigned char *codes = static_cast<unsigned char *>(workspace);
-    unsigned char *scales = codes + (code_bytes(m, k) + 255u) / 256u * 256u;
-    const int code = aotx_mx4_quantize(ctx, stream, x, x_dtype, m, ldx, k, nullptr, m, m_dev, codes, scales);
-    return code != AOTX_Q8_OK ? code
-         : aotx_mx4_matmul(ctx, stream, w_codes, w_scales, n, k, codes, scales, m, m_dev, y, y_dtype, epilogue);
+    const OnDevice on(ctx);
+    q8::Mx4Product p = {};
+    p.w_codes = w_codes;
+    p.w_scales = static_cast<const uint32_t *>(w_scales);
+    p.experts = 1u;
+    p.n = n;
+    p.k = k;
+    p.m = m;
+    p.m_dev = m_dev;
+    p.y_rows = m;
+    p.y = y;
+    p.y_dtype = y_dtype;
+    p.epilogue = (unsigned int)epilogue;
+    p.overlap = ctx->overlap != 0;
+    p.weights_late = fresh(ctx, w_codes, code_bytes(n, k)) || fresh(ctx, w_scales, scale_bytes(n, k));
+    p.x = x;
+    p.x_dtype = x_dtype;
+    p.ldx = ldx;
+    return code_of(ctx, q8::launch_mx4_product((cudaStream_t)stream, ctx->scratch, ctx->sm_count, ctx->launches++, p));
 }
 
 extern "C" int aotx_mx4_moe_order(aotx_q8_ctx *ctx, void *stream, const uint32_t *ids, uint32_t tokens,
@@ -257,9 +280,8 @@ extern "C" int aotx_mx4_matmul_grouped(aotx_q8_ctx *ctx, void *stream, const voi
     p.y = y;
     p.y_dtype = y_dtype;
     p.epilogue = (unsigned int)epilogue;
-    p.status = ctx->scratch.status;
     p.overlap = ctx->overlap != 0;
     const uint64_t w_rows = (uint64_t)experts * n;
     p.weights_late = fresh(ctx, w_codes, code_bytes(w_rows, k)) || fresh(ctx, w_scales, scale_bytes(w_rows, k));
-    return code_of(ctx, q8::launch_mx4_product((cudaStream_t)stream, ctx->sm_count, p));
+    return code_of(ctx, q8::launch_mx4_product((cudaStream_t)stream, ctx->scratch, ctx->sm_count, ctx->launches++, p));
 }

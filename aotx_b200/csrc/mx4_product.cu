@@ -11,9 +11,16 @@
 //   * One thread issues the copies of the scales and the MMAs behind them (they run in that order).  Each stage has its own
 //     columns of tensor memory for scales, so that nothing is overwritten before its MMAs are done.
 //   * Four warps store: the sums of 16 rows of x are turned round in shared memory, 16 bytes a lane.
+//   * The grid is at most one block per SM, and the steps of all tiles (a tile by one stage) are dealt to it in equal runs, so
+//     copies go on from tile to tile and every SM streams to the end.  A tile that is cut between blocks belongs to the one
+//     with its first step: the others leave their sums in the context's scratch and raise a flag per warp (a block does so
+//     once, with its first tile, before it waits for anyone), and the owner adds them in the order of the blocks.
+//   * Few rows of x in 16 or 32 bits (mx4_linear) are quantised by the storing warps, which have nothing else to do at first,
+//     straight into the shared memory that the MMA reads, every stage that the block needs once.
 #include <cuda.h>
 
 #include "mx4.h"
+#include "mx4_block.cuh"
 #include "mx4_ptx.cuh"
 #include "q8_rows.cuh"
 
@@ -27,13 +34,16 @@ constexpr uint32_t kMxRows = 128;           // rows of w per tile
 constexpr uint32_t kMxMaxTok = 256;         // rows of x per tile, at most
 constexpr uint32_t kMxStageK = 256;         // values of a row per stage
 constexpr uint32_t kMxStageBytes = kMxStageK / 2;
-constexpr uint32_t kMxMaxStages = 8;
+constexpr uint32_t kMxMaxStages = 12;
+constexpr uint32_t kMxMaxSlots = 64;        // stages of x that stay
 constexpr uint32_t kMxScaleBlock = 512;     // scales of 128 rows and 128 values
-constexpr uint32_t kMxAhead = 3;            // stages whose scales are on their way, at most
 constexpr uint32_t kMxEpilogueStage = 16u * 32u * 4u;  // per storing warp
-constexpr uint32_t kMxBars = 3 * kMxMaxStages + 1;
-constexpr uint32_t kMxTail = 4u * kMxEpilogueStage + kMxBars * 8u + 16u;
-constexpr uint32_t kMxSmem = 226u * 1024u;
+constexpr uint32_t kMxFewSteps = 2;         // steps of a block, at least
+constexpr uint32_t kMxFusedRows = 32;       // rows of x that the kernel quantises itself, at most
+constexpr uint32_t kMxBars = 2 * kMxMaxStages + 4 + kMxMaxSlots;
+constexpr uint32_t kMxTail = 4u * kMxEpilogueStage + kMxBars * 8u;
+constexpr uint32_t kMxSmem = 223u * 1024u;
+constexpr uint32_t kMxRings = (kMxSmem - 1024u - kMxTail) / 1024u * 1024u;
 
 struct MxArgs {
     const uint32_t *w_scales;
@@ -52,9 +62,18 @@ struct MxArgs {
     unsigned int *status;
     uint32_t ntok;                 // rows of x per tile, a multiple of 16
     uint32_t stages, stage_bytes;
-    uint32_t tmem_columns;
+    uint32_t tmem_columns, accumulators;
     uint32_t weights_late;
     uint32_t wide;                 // rows of y lie on 16-byte boundaries
+    // x in 16 or 32 bits, quantised here: its stages stay in `slots` places behind the ring
+    const void *x;
+    uint32_t x_type;
+    uint32_t x_aligned;
+    unsigned long long ldx;
+    uint32_t slots;                // 0: x is in MX4 and goes through the ring
+    float *partial;                // per block: [row of x][row of w], and its flags
+    unsigned int *flags;
+    unsigned long long tile_floats;
 };
 
 __host__ __device__ inline uint32_t mx_scale_blocks(uint32_t ntok)
@@ -87,56 +106,221 @@ __device__ __forceinline__ uint64_t mx_scale_desc(uint32_t smem_addr)
     return desc;
 }
 
-// The rows of x of a tile and the expert they belong to; no rows: no tile.
+// The groups of a grouped product, in shared memory: expert e's rows of x from first[e], rows[e] of them, and the tiles up
+// to and with it.
+struct MxGroups {
+    uint32_t first[kMx4MaxExperts];
+    uint32_t rows[kMx4MaxExperts];
+    uint32_t through[kMx4MaxExperts];
+    uint32_t warps[8];
+};
+
+// Every thread calls it, once the offsets are there.  Returns the number of tiles.
+__device__ __forceinline__ uint32_t mx_groups(const MxArgs &args, MxGroups &groups, uint32_t row_tiles)
+{
+    const uint32_t e = threadIdx.x;
+    uint32_t through = 0u;
+    if (e < kMx4MaxExperts) {
+        uint32_t first = 0u, rows = 0u;
+        if (e < args.experts) {
+            first = args.offsets[e];
+            uint32_t end = args.offsets[e + 1u];
+            first = first < args.x_rows ? first : args.x_rows;
+            end = end < args.x_rows ? end : args.x_rows;
+            rows = end > first ? end - first : 0u;
+        }
+        through = (rows + args.ntok - 1u) / args.ntok * row_tiles;
+#pragma unroll
+        for (uint32_t step = 1u; step < 32u; step <<= 1) {
+            const uint32_t below = __shfl_up_sync(0xFFFFFFFFu, through, step);
+            if ((threadIdx.x & 31u) >= step) {
+                through += below;
+            }
+        }
+        groups.first[e] = first;
+        groups.rows[e] = rows;
+        if ((threadIdx.x & 31u) == 31u) {
+            groups.warps[e / 32u] = through;
+        }
+    }
+    __syncthreads();
+    if (e < kMx4MaxExperts) {
+        for (uint32_t w = 0; w < e / 32u; ++w) {
+            through += groups.warps[w];
+        }
+        groups.through[e] = through;
+    }
+    __syncthreads();
+    return groups.through[kMx4MaxExperts - 1u];
+}
+
+// A tile: 128 rows of w from w_row (row `row0` of n), and rows of x.
 struct MxTile {
-    uint32_t expert;
+    uint32_t w_row, row0;
     uint32_t first, rows;
 };
 
-// Token tile `index` of the groups in order (all threads call it; `scratch` is shared memory of 33 words).
-__device__ __forceinline__ MxTile mx_group_tile(const MxArgs &args, uint32_t index, uint32_t *scratch)
+// Tile `index`; the tiles of one run of rows of w follow each other, so that the second finds it in L2.
+__device__ __forceinline__ MxTile mx_tile(const MxArgs &args, const MxGroups &groups, uint32_t index, uint32_t tok_tiles,
+                                          uint32_t live)
 {
-    // thread e holds expert e
-    const uint32_t e = threadIdx.x;
-    uint32_t first = 0u, rows = 0u;
-    if (e < args.experts) {
-        first = args.offsets[e];
-        uint32_t end = args.offsets[e + 1u];
-        first = first < args.x_rows ? first : args.x_rows;
-        end = end < args.x_rows ? end : args.x_rows;
-        rows = end > first ? end - first : 0u;
+    MxTile tile;
+    uint32_t expert = 0u, first = 0u, rows = live;
+    if (args.offsets != nullptr) {
+        // the expert is the first whose tiles go past the index
+        uint32_t low = 0u, high = args.experts - 1u;
+        while (low < high) {
+            const uint32_t middle = (low + high) / 2u;
+            if (groups.through[middle] > index) {
+                high = middle;
+            } else {
+                low = middle + 1u;
+            }
+        }
+        expert = low;
+        index -= expert != 0u ? groups.through[expert - 1u] : 0u;
+        first = groups.first[expert];
+        rows = groups.rows[expert];
+        tok_tiles = (rows + args.ntok - 1u) / args.ntok;
     }
-    const uint32_t tiles = (rows + args.ntok - 1u) / args.ntok;
-    uint32_t through = tiles;          // of the experts up to and with this one
-#pragma unroll
-    for (uint32_t step = 1u; step < 32u; step <<= 1) {
-        const uint32_t below = __shfl_up_sync(0xFFFFFFFFu, through, step);
-        if ((threadIdx.x & 31u) >= step) {
-            through += below;
+    const uint32_t row_tile = index / tok_tiles;
+    const uint32_t skip = (index - row_tile * tok_tiles) * args.ntok;
+    tile.row0 = row_tile * kMxRows;
+    tile.w_row = expert * args.n + tile.row0;
+    tile.first = first + skip;
+    tile.rows = rows > skip ? (rows - skip < args.ntok ? rows - skip : args.ntok) : 0u;
+    return tile;
+}
+
+// The run of steps of block b: of `units` in all, the first units % blocks blocks take one more.
+__host__ __device__ __forceinline__ unsigned long long mx_run_begin(uint32_t b, uint32_t blocks, unsigned long long units)
+{
+    const unsigned long long share = units / blocks;
+    const unsigned long long more = units - share * blocks;
+    return b * share + (b < more ? b : more);
+}
+
+// The pieces of a run: a tile and the steps [from, to) of its depth.
+struct MxPieces {
+    unsigned long long unit, end;
+    uint32_t steps;
+    uint32_t tile, from, to;
+
+    __device__ __forceinline__ bool next()
+    {
+        if (unit >= end) {
+            return false;
+        }
+        tile = (uint32_t)(unit / steps);
+        from = (uint32_t)(unit - (unsigned long long)tile * steps);
+        const unsigned long long left = end - unit;
+        to = left < steps - from ? from + (uint32_t)left : steps;
+        unit += to - from;
+        return true;
+    }
+};
+
+// A place in a ring of stages, and how often the ring has come round, as the parity that its barriers are waited for with.
+struct MxRing {
+    uint32_t at = 0, parity = 0;
+
+    __device__ __forceinline__ void next(uint32_t size)
+    {
+        if (++at == size) {
+            at = 0;
+            parity ^= 1u;
         }
     }
-    if ((threadIdx.x & 31u) == 31u) {
-        scratch[threadIdx.x >> 5] = through;
+};
+
+// Has the block that this flag belongs to left its sums?  Bounded like every wait.
+__device__ __forceinline__ bool mx_wait_flag(const unsigned int *flag, volatile uint32_t *abort_flag, unsigned int *status)
+{
+    const long long begin = clock64();
+    while (ld_acquire_gpu(flag) == 0u) {
+        if (*abort_flag != 0u || clock64() - begin > Q8_WAIT_CYCLES) {
+            *abort_flag = 1u;
+            atomicOr(status, Q8_DEV_FLAG_TIMEOUT);
+            return false;
+        }
     }
-    if (threadIdx.x == 0u) {
-        scratch[17] = 0u;              // rows: none
+    return true;
+}
+
+// One block of 32 values of x for the MMA: 16 bytes of codes at `cell`, its scale's byte at `scale_at`.
+template <typename T>
+__device__ __forceinline__ void mx_quantize_block(const T *x, bool aligned, uint32_t cell, uint32_t scale_at)
+{
+    Eight<T> raw[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        raw[i].load(x + 8 * i, aligned);
     }
-    __syncthreads();
-    for (uint32_t w = 0; w < threadIdx.x >> 5; ++w) {
-        through += scratch[w];
+    float v[8];
+    uint32_t largest = 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        raw[i].floats(v);
+        largest = mx4_largest(v, largest);
     }
-    if (index < through && index >= through - tiles) {
-        const uint32_t skip = (index - (through - tiles)) * args.ntok;
-        scratch[16] = first + skip;
-        scratch[17] = rows - skip < args.ntok ? rows - skip : args.ntok;
-        scratch[18] = e;
+    const uint32_t scale = mx4_scale(largest);
+    const float inverse = mx4_inverse(scale);
+    uint32_t word[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        raw[i].floats(v);
+        word[i] = mx4_codes(v, scale, inverse);
     }
-    __syncthreads();
-    MxTile tile;
-    tile.first = scratch[16];
-    tile.rows = scratch[17];
-    tile.expert = scratch[18];
-    return tile;
+    st_shared_v4(cell, word[0], word[1], word[2], word[3]);
+    st_shared_b8(scale_at, scale);
+}
+
+// The stages of x that this block needs, in the order in which it needs them, by the 128 threads of four warps.  Each warp
+// arrives on a stage's barrier when its part of it is there.
+template <typename T>
+__device__ __forceinline__ void mx_quantize_x(const MxArgs &args, const T *x, uint32_t place, uint32_t slot_bytes,
+                                              uint32_t bars, uint32_t first_step, uint32_t slots, uint32_t steps, uint32_t live)
+{
+    const uint32_t t = threadIdx.x;
+    // rows past the last and values past k stay zero
+    for (uint32_t at = t * 16u; at < slots * slot_bytes; at += 128u * 16u) {
+        st_shared_v4(place + at, 0u, 0u, 0u, 0u);
+    }
+    named_bar_sync(1u, 128u);
+    const uint32_t items = live * 8u;      // blocks of 32 in a stage
+    uint32_t told = 0u;                    // stages whose barrier this warp has arrived on
+    for (uint32_t base = 0; base < slots * items; base += 128u) {
+        const uint32_t item = base + t;
+        if (item < slots * items) {
+            const uint32_t slot = item / items;
+            const uint32_t row = (item - slot * items) / 8u;
+            const uint32_t b = item & 7u;
+            const uint32_t step = first_step + slot < steps ? first_step + slot : first_step + slot - steps;
+            const uint32_t at = step * kMxStageK + b * 32u;
+            if (at < args.k) {
+                const uint32_t stage = place + slot * slot_bytes;
+                mx_quantize_block<T>(x + (unsigned long long)row * args.ldx + at, args.x_aligned != 0u,
+                                     stage + row * kMxStageBytes + ((b ^ (row & 7u)) * 16u),
+                                     stage + args.ntok * kMxStageBytes + (b / 4u) * kMxScaleBlock + (row % 32u) * 16u
+                                         + (row / 32u) * 4u + b % 4u);
+            }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        const uint32_t whole = base + 128u < slots * items ? (base + 128u) / items : slots;
+        for (; told < whole; ++told) {
+            if ((t & 31u) == 0u) {
+                mbar_arrive(bars + told * 8u);
+            }
+        }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    for (; told < slots; ++told) {         // (no live row: zeros all over)
+        if ((t & 31u) == 0u) {
+            mbar_arrive(bars + told * 8u);
+        }
+    }
 }
 
 // 16 rows of x (v: this lane's row of w for each) to y, rows `first` and up below `end`.
@@ -226,7 +410,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                    const __grid_constant__ MxArgs args)
 {
     extern __shared__ unsigned char smem_raw[];
-    __shared__ uint32_t scratch[20];
+    __shared__ MxGroups groups;
     __shared__ uint32_t abort_flag;
     __shared__ uint32_t tmem_base;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -234,17 +418,20 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const uint32_t lane = threadIdx.x & 31u;
     const uint32_t stages = args.stages;
     const uint32_t x_blocks = mx_scale_blocks(args.ntok);
-    // a stage: codes of w, codes of x, scales of w, scales of x
-    const uint32_t x_codes_at = kMxRows * kMxStageBytes;
-    const uint32_t w_scales_at = x_codes_at + args.ntok * kMxStageBytes;
-    const uint32_t x_scales_at = w_scales_at + 2u * kMxScaleBlock;
-    const uint32_t tail = base + stages * args.stage_bytes;
+    const bool stays = args.slots != 0u;
+    // a stage: codes of w, scales of w, codes of x, scales of x; x that stays has places of its own behind the ring
+    const uint32_t w_scales_at = kMxRows * kMxStageBytes;
+    const uint32_t x_codes_at = w_scales_at + 2u * kMxScaleBlock;
+    const uint32_t x_scales_at = x_codes_at + args.ntok * kMxStageBytes;
+    const uint32_t place = base + stages * args.stage_bytes;
+    const uint32_t slot_bytes = args.ntok * kMxStageBytes + 2u * x_blocks * kMxScaleBlock;
+    const uint32_t tail = base + kMxRings;
     const uint32_t bars = tail + 4u * kMxEpilogueStage;
-    auto full = [&](uint32_t s) { return bars + s * 8u; };
-    auto scaled = [&](uint32_t s) { return bars + (kMxMaxStages + s) * 8u; };
-    auto empty = [&](uint32_t s) { return bars + (2u * kMxMaxStages + s) * 8u; };
-    const uint32_t done = bars + 3u * kMxMaxStages * 8u;
-    const uint32_t steps = (args.k + kMxStageK - 1u) / kMxStageK;
+    auto full = [&](uint32_t s) { return bars + s * 8u; };           // codes and scales are there
+    auto empty = [&](uint32_t s) { return bars + (kMxMaxStages + s) * 8u; };
+    auto summed = [&](uint32_t b) { return bars + (2u * kMxMaxStages + b) * 8u; };
+    auto taken = [&](uint32_t b) { return bars + (2u * kMxMaxStages + 2u + b) * 8u; };
+    const uint32_t x_bars = bars + (2u * kMxMaxStages + 4u) * 8u;
 
     if (warp == kMxMmaWarp) {
         tmem_alloc(smem_u32(&tmem_base), args.tmem_columns);
@@ -253,11 +440,16 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     if (threadIdx.x == 0u) {
         abort_flag = 0u;
         for (uint32_t s = 0; s < stages; ++s) {
-            mbar_init(full(s), 1u);
-            mbar_init(scaled(s), 4u);
+            mbar_init(full(s), 1u + 128u);
             mbar_init(empty(s), 1u);
         }
-        mbar_init(done, 1u);
+        for (uint32_t b = 0; b < 2u; ++b) {
+            mbar_init(summed(b), 1u);
+            mbar_init(taken(b), 4u);
+        }
+        for (uint32_t s = 0; s < args.slots; ++s) {
+            mbar_init(x_bars + s * 8u, 4u);
+        }
         mbar_init_fence();
     }
     tc_fence_before_sync();
@@ -265,159 +457,290 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     tc_fence_after_sync();
     const uint32_t tmem = tmem_base;
 
-    // which rows
-    const uint32_t row0 = blockIdx.x * kMxRows;              // of the expert's n
-    MxTile tile = {0u, blockIdx.y * args.ntok, 0u};
-    bool early = false;                                      // may the weights come before the work before this has ended?
+    // which tiles there are
+    const uint32_t steps = (args.k + kMxStageK - 1u) / kMxStageK;
+    const uint32_t row_tiles = (args.n + kMxRows - 1u) / kMxRows;
+    uint32_t live = args.x_rows;
+    uint32_t tok_tiles = (args.x_rows + args.ntok - 1u) / args.ntok;
+    uint32_t tiles = tok_tiles * row_tiles;
+    bool waited = false;                   // has everything before this launch ended?
     if (args.offsets != nullptr) {
         grid_dependency_wait();
-        tile = mx_group_tile(args, blockIdx.y, scratch);
-    } else if (args.m_dev != nullptr) {
+        waited = true;
+        tiles = mx_groups(args, groups, row_tiles);
+    } else if (args.m_dev != nullptr && tok_tiles > 1u) {
         grid_dependency_wait();
-        const uint32_t live = *args.m_dev < args.x_rows ? *args.m_dev : args.x_rows;
-        tile.rows = live > tile.first ? (live - tile.first < args.ntok ? live - tile.first : args.ntok) : 0u;
-    } else {
-        tile.rows = args.x_rows - tile.first < args.ntok ? args.x_rows - tile.first : args.ntok;
-        early = args.weights_late == 0u;
+        waited = true;
+        live = *args.m_dev < args.x_rows ? *args.m_dev : args.x_rows;
+        tok_tiles = (live + args.ntok - 1u) / args.ntok;
+        tiles = tok_tiles * row_tiles;
     }
-    const uint32_t w_row0 = tile.expert * args.n + row0;
+    const bool early = !waited && args.weights_late == 0u;
+    const unsigned long long units = (unsigned long long)tiles * steps;
+    MxPieces mine;
+    mine.unit = mx_run_begin(blockIdx.x, gridDim.x, units);
+    mine.end = mx_run_begin(blockIdx.x + 1u, gridDim.x, units);
+    mine.steps = steps;
+    const unsigned long long run = mine.end - mine.unit;
+    const uint32_t first_step = (uint32_t)(mine.unit % steps);
+    // (a batch of one tile is multiplied whole, however much of it lives)
+    const auto live_rows = [&]() {
+        if (args.m_dev != nullptr && tok_tiles == 1u && !waited) {
+            const uint32_t on_device = *args.m_dev;
+            return on_device < args.x_rows ? on_device : args.x_rows;
+        }
+        return live;
+    };
 
-    if (tile.rows != 0u) {
-        if (warp == kMxCopyWarp) {
-            if (elect_one()) {
-                const uint32_t bytes = (kMxRows + args.ntok) * kMxStageBytes;
-                uint32_t begun = 0;
-                if (early) {
-                    // weights into every stage, then x behind them
-                    begun = steps < stages ? steps : stages;
-                    for (uint32_t it = 0; it < begun; ++it) {
-                        mbar_expect_tx(full(it), bytes);
-                        tma_load_2d(base + it * args.stage_bytes, &map_w, full(it), (int)(it * kMxStageBytes), (int)w_row0);
+    if (warp == kMxCopyWarp) {
+        if (elect_one()) {
+            const uint32_t bytes = kMxRows * kMxStageBytes + (stays ? 0u : args.ntok * kMxStageBytes);
+            auto copy_w = [&](uint32_t s, uint32_t step, uint32_t w_row) {
+                mbar_expect_tx(full(s), bytes);
+                tma_load_2d(base + s * args.stage_bytes, &map_w, full(s), (int)(step * kMxStageBytes), (int)w_row);
+            };
+            uint32_t begun = 0;
+            if (early) {
+                // weights into every stage, then x behind them
+                MxPieces ahead = mine;
+                while (begun < stages && ahead.next()) {
+                    const MxTile tile = mx_tile(args, groups, ahead.tile, tok_tiles, live);
+                    for (uint32_t step = ahead.from; step < ahead.to && begun < stages; ++step) {
+                        copy_w(begun++, step, tile.w_row);
                     }
-                }
-                grid_dependency_wait();
-                uint32_t it = 0;
-                for (; it < steps; ++it) {
-                    const uint32_t s = it % stages;
-                    const uint32_t at = base + s * args.stage_bytes;
-                    if (it >= begun) {
-                        if (it >= stages && !mbar_wait(empty(s), (it / stages + 1u) & 1u, &abort_flag, args.status)) {
-                            break;
-                        }
-                        mbar_expect_tx(full(s), bytes);
-                        tma_load_2d(at, &map_w, full(s), (int)(it * kMxStageBytes), (int)w_row0);
-                    }
-                    tma_load_2d(at + x_codes_at, &map_x, full(s), (int)(it * kMxStageBytes), (int)tile.first);
-                }
-                // No copy is on its way when the block ends, whatever became of the MMAs that wait for them too.
-                for (uint32_t last = it > stages ? it - stages : 0u; last < it; ++last) {
-                    mbar_wait(full(last % stages), (last / stages) & 1u, &abort_flag, args.status);
                 }
             }
-        } else if (warp == kMxMmaWarp) {
-            if (elect_one()) {
-                const uint32_t idesc[2] = {mx_idesc(args.ntok, 0u), mx_idesc(args.ntok, 1u)};
-                const uint32_t columns = 2u * 4u * (1u + x_blocks);   // of scales, per stage
-                bool ok = true;
-                for (uint32_t it = 0; it < steps && ok; ++it) {
-                    const uint32_t s = it % stages;
-                    const uint32_t parity = (it / stages) & 1u;
-                    ok = mbar_wait(scaled(s), parity, &abort_flag, args.status)
-                      && mbar_wait(full(s), parity, &abort_flag, args.status);
-                    if (!ok) {
+            if (!stays || !early) {
+                grid_dependency_wait();
+            }
+            uint32_t it = 0;
+            MxRing ring;
+            bool ok = true;
+            while (ok && mine.next()) {
+                const MxTile tile = mx_tile(args, groups, mine.tile, tok_tiles, live);
+                for (uint32_t step = mine.from; step < mine.to; ++step, ++it, ring.next(stages)) {
+                    if (it >= begun) {
+                        if (it >= stages && !mbar_wait_hot(empty(ring.at), ring.parity ^ 1u, &abort_flag, args.status)) {
+                            ok = false;
+                            break;
+                        }
+                        copy_w(ring.at, step, tile.w_row);
+                    }
+                    if (!stays) {
+                        tma_load_2d(base + ring.at * args.stage_bytes + x_codes_at, &map_x, full(ring.at),
+                                    (int)(step * kMxStageBytes), (int)tile.first);
+                    }
+                }
+            }
+            // Everything is on its way: the blocks of the next launch may take their places as these leave them.  (Behind this
+            // block's own wait, so that what runs early overlaps nothing before it.)
+            grid_dependency_wait();
+            grid_launch_dependents();
+            // No copy is on its way when the block ends, whatever became of the MMAs that wait for them too.
+            for (uint32_t last = it > stages ? it - stages : 0u; last < it; ++last) {
+                mbar_wait(full(last % stages), (last / stages) & 1u, &abort_flag, args.status);
+            }
+        }
+    } else if (warp == kMxMmaWarp) {
+        if (elect_one()) {
+            const uint32_t idesc0 = mx_idesc(args.ntok, 0u);
+            const uint32_t idesc1 = mx_idesc(args.ntok, 1u);
+            const uint32_t columns = 2u * 4u * (1u + x_blocks);   // of scales, per stage
+            const uint32_t scales_at = tmem + args.accumulators * args.ntok;
+            const uint64_t codes_desc = umma_desc_sw128(0u);
+            const uint64_t scale_desc = mx_scale_desc(0u);
+            uint32_t it = 0, piece = 0;
+            MxRing ring, slot, sums_ring;
+            bool ok = true;
+            for (; ok && mine.next(); ++piece, sums_ring.next(args.accumulators)) {
+                const uint32_t sums = tmem + sums_ring.at * args.ntok;
+                if (piece >= args.accumulators
+                    && !mbar_wait(taken(sums_ring.at), sums_ring.parity ^ 1u, &abort_flag, args.status)) {
+                    break;
+                }
+                for (uint32_t step = mine.from; step < mine.to; ++step, ++it, ring.next(stages), slot.next(args.slots)) {
+                    if ((stays && it < args.slots && !mbar_wait_hot(x_bars + slot.at * 8u, 0u, &abort_flag, args.status))
+                        || !mbar_wait_hot(full(ring.at), ring.parity, &abort_flag, args.status)) {
+                        ok = false;
                         break;
                     }
                     tc_fence_after_sync();
-                    const uint32_t at = base + s * args.stage_bytes;
-                    const uint32_t w_scales = tmem + args.ntok + s * columns;
+                    fence_proxy_async_smem();        // the scales came by ordinary copies
+                    const uint32_t at = base + ring.at * args.stage_bytes;
+                    const uint32_t x_at = stays ? place + slot.at * slot_bytes : at + x_codes_at;
+                    const uint32_t w_scales = scales_at + ring.at * columns;
                     const uint32_t x_scales = w_scales + 8u;
-                    for (uint32_t c = 0; c < 2u; ++c) {
-                        tmem_copy_scales(w_scales + 4u * c, mx_scale_desc(at + w_scales_at + c * kMxScaleBlock));
-                        for (uint32_t b = 0; b < x_blocks; ++b) {
-                            tmem_copy_scales(x_scales + 4u * (c * x_blocks + b),
-                                             mx_scale_desc(at + x_scales_at + (c * x_blocks + b) * kMxScaleBlock));
-                        }
+                    const uint64_t w_from = scale_desc | ((at + w_scales_at) >> 4);
+                    const uint64_t x_from = scale_desc | ((x_at + args.ntok * kMxStageBytes) >> 4);
+                    tmem_copy_scales(w_scales, w_from);
+                    tmem_copy_scales(w_scales + 4u, w_from + (kMxScaleBlock >> 4));
+                    tmem_copy_scales(x_scales, x_from);
+                    tmem_copy_scales(x_scales + 4u, x_from + (kMxScaleBlock >> 4));
+                    if (x_blocks == 2u) {
+                        tmem_copy_scales(x_scales + 8u, x_from + 2u * (kMxScaleBlock >> 4));
+                        tmem_copy_scales(x_scales + 12u, x_from + 3u * (kMxScaleBlock >> 4));
                     }
-                    const uint64_t a = umma_desc_sw128(at);
-                    const uint64_t b = umma_desc_sw128(at + x_codes_at);
-                    const uint32_t left = args.k - it * kMxStageK;
-                    const uint32_t pieces = left >= kMxStageK ? 4u : (left + 63u) / 64u;
-                    for (uint32_t p = 0; p < pieces; ++p) {
-                        // 64 values are 32 bytes of a row
-                        umma_mx4(tmem, a + 2u * p, b + 2u * p, idesc[p & 1u], w_scales + 4u * (p >> 1),
-                                 x_scales + 4u * x_blocks * (p >> 1), (it | p) != 0u);
+                    // 64 values are 32 bytes of a row, and half of a word of scales
+                    const uint64_t a = codes_desc | (at >> 4);
+                    const uint64_t b = codes_desc | (x_at >> 4);
+                    const uint32_t x_next = x_scales + 4u * x_blocks;
+                    umma_mx4(sums, a, b, idesc0, w_scales, x_scales, step != mine.from);
+                    const uint32_t left = args.k - step * kMxStageK;
+                    if (left > 64u) {
+                        umma_mx4(sums, a + 2u, b + 2u, idesc1, w_scales, x_scales, 1u);
                     }
-                    umma_commit(empty(s));
+                    if (left > 128u) {
+                        umma_mx4(sums, a + 4u, b + 4u, idesc0, w_scales + 4u, x_next, 1u);
+                    }
+                    if (left > 192u) {
+                        umma_mx4(sums, a + 6u, b + 6u, idesc1, w_scales + 4u, x_next, 1u);
+                    }
+                    umma_commit(empty(ring.at));
                 }
-                umma_commit(done);
+                umma_commit(summed(sums_ring.at));
             }
-        } else if (warp >= kMxScaleWarp && warp < kMxCopyWarp) {
-            // Row t of either operand's tile, and row t + 128 of x.
+        }
+    } else if (warp >= kMxScaleWarp && warp < kMxCopyWarp) {
+        // Row t of either operand's tile, and row t + 128 of x.
+        if (!stays || !early) {
             grid_dependency_wait();
-            const uint32_t t = threadIdx.x - kMxScaleWarp * 32u;
-            const uint32_t cell = (t % 32u) * 16u + (t / 32u) * 4u;
-            const uint32_t w_row = w_row0 + t;
-            const uint32_t ahead = kMxAhead < stages - 1u ? kMxAhead : stages - 1u;
-            auto give = [&](uint32_t it) {
-                fence_proxy_async_smem();
+        }
+        const uint32_t t = threadIdx.x - kMxScaleWarp * 32u;
+        const uint32_t cell = (t % 32u) * 16u + (t / 32u) * 4u;
+        uint32_t it = 0;
+        MxRing ring;
+        bool ok = true;
+        while (ok && mine.next()) {
+            const MxTile tile = mx_tile(args, groups, mine.tile, tok_tiles, live);
+            const uint32_t w_row = tile.w_row + t;
+            const bool w_in = w_row < args.w_rows;
+            const bool x_in = t < tile.rows;
+            const bool x_in_2 = t + 128u < tile.rows;
+            // (a row outside the tensor is not read, whatever its address)
+            const uint32_t *w_from = args.w_scales + (w_in ? (size_t)(2u * mine.from) * args.w_rows + w_row : 0u);
+            const uint32_t *x_from = stays ? nullptr : args.x_scales + (x_in ? (size_t)(2u * mine.from) * args.x_rows + tile.first + t : 0u);
+            for (uint32_t step = mine.from; step < mine.to; ++step, ++it, ring.next(stages)) {
+                if (it >= stages && !mbar_wait_hot(empty(ring.at), ring.parity ^ 1u, &abort_flag, args.status)) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t at = base + ring.at * args.stage_bytes + cell;
+                const bool second = 2u * step + 1u < args.chunks;
+                copy_async_4(at + w_scales_at, w_from, w_in ? 4u : 0u);
+                copy_async_4(at + w_scales_at + kMxScaleBlock, second ? w_from + args.w_rows : w_from, w_in && second ? 4u : 0u);
+                w_from += w_in && second ? 2u * (size_t)args.w_rows : 0u;
+                if (!stays) {
+                    const uint32_t *x_second = x_in && second ? x_from + args.x_rows : x_from;
+                    copy_async_4(at + x_scales_at, x_from, x_in ? 4u : 0u);
+                    copy_async_4(at + x_scales_at + x_blocks * kMxScaleBlock, x_second, x_in && second ? 4u : 0u);
+                    if (x_blocks == 2u) {
+                        copy_async_4(at + x_scales_at + kMxScaleBlock, x_in_2 ? x_from + 128u : x_from, x_in_2 ? 4u : 0u);
+                        copy_async_4(at + x_scales_at + 3u * kMxScaleBlock, x_in_2 && second ? x_second + 128u : x_from,
+                                     x_in_2 && second ? 4u : 0u);
+                    }
+                    x_from += x_in && second ? 2u * (size_t)args.x_rows : 0u;
+                }
+                copy_async_arrive(full(ring.at));
+            }
+        }
+        copy_async_wait_all();
+    } else if (warp < kMxScaleWarp) {
+        grid_dependency_wait();       // x, y, the row map and the scratch
+        const uint32_t valid = live_rows();
+        if (stays) {
+            const uint32_t slots = run < args.slots ? (uint32_t)run : args.slots;
+            switch (args.x_type) {
+            case 0u:
+                mx_quantize_x(args, static_cast<const float *>(args.x), place, slot_bytes, x_bars, first_step, slots, steps, valid);
+                break;
+            case 1u:
+                mx_quantize_x(args, static_cast<const __half *>(args.x), place, slot_bytes, x_bars, first_step, slots, steps, valid);
+                break;
+            default:
+                mx_quantize_x(args, static_cast<const __nv_bfloat16 *>(args.x), place, slot_bytes, x_bars, first_step, slots, steps,
+                              valid);
+                break;
+            }
+        }
+        const uint32_t stage = tail + warp * kMxEpilogueStage;
+        const uint32_t lane_taddr = tmem + ((warp * 32u) << 16);
+        for (MxRing ring; mine.next(); ring.next(args.accumulators)) {
+            const uint32_t buffer = ring.at;
+            const MxTile tile = mx_tile(args, groups, mine.tile, tok_tiles, live);
+            if (!mbar_wait(summed(buffer), ring.parity, &abort_flag, args.status)) {
+                break;
+            }
+            tc_fence_after_sync();
+            const uint32_t sums = lane_taddr + buffer * args.ntok;
+            auto release = [&] {
+                tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0u) {
-                    mbar_arrive(scaled(it % stages));
+                    mbar_arrive(taken(buffer));
                 }
             };
-            for (uint32_t it = 0; it < steps + ahead; ++it) {
-                if (it < steps) {
-                    const uint32_t s = it % stages;
-                    if (it >= stages && !mbar_wait(empty(s), (it / stages + 1u) & 1u, &abort_flag, args.status)) {
-                        break;
-                    }
-                    const uint32_t at = base + s * args.stage_bytes;
-                    for (uint32_t c = 0; c < 2u; ++c) {
-                        const uint32_t chunk = 2u * it + c;
-                        const bool in = chunk < args.chunks;
-                        const bool w_in = in && w_row < args.w_rows;
-                        copy_async_4(at + w_scales_at + c * kMxScaleBlock + cell,
-                                     args.w_scales + (w_in ? (size_t)chunk * args.w_rows + w_row : 0u), w_in ? 4u : 0u);
-                        for (uint32_t b = 0; b < x_blocks; ++b) {
-                            const uint32_t r = t + 128u * b;
-                            const bool x_in = in && r < tile.rows;
-                            copy_async_4(at + x_scales_at + (c * x_blocks + b) * kMxScaleBlock + cell,
-                                         args.x_scales + (x_in ? (size_t)chunk * args.x_rows + tile.first + r : 0u),
-                                         x_in ? 4u : 0u);
-                        }
-                    }
-                }
-                copy_async_commit();
-                if (it >= ahead) {
-                    // (the groups of the stages after this one may still be on their way)
-                    switch (ahead) {
-                    case 1u: copy_async_wait<1>(); break;
-                    case 2u: copy_async_wait<2>(); break;
-                    default: copy_async_wait<3>(); break;
-                    }
-                    give(it - ahead);
-                }
-            }
-            copy_async_wait_all();
-        } else if (warp < kMxScaleWarp) {
-            grid_dependency_wait();       // y, and the row map
-            if (mbar_wait(done, 0u, &abort_flag, args.status)) {
-                tc_fence_after_sync();
-                const uint32_t stage = tail + warp * kMxEpilogueStage;
-                const uint32_t j0 = row0 + warp * 32u;
-                const uint32_t mine = args.n > j0 ? (args.n - j0 < 32u ? args.n - j0 : 32u) : 0u;
-                const uint32_t first_col = GATED ? j0 / 2u : j0;
-                const uint32_t columns = GATED ? mine / 2u : mine;
+            if (mine.from != 0u) {
+                // Another block owns the tile: its sums go to the scratch.
+                float *out = args.partial + blockIdx.x * args.tile_floats + warp * 32u + lane;
                 for (uint32_t c0 = 0; c0 < tile.rows; c0 += 16u) {
                     uint32_t v[16];
-                    tmem_ld_32x16(tmem + ((warp * 32u) << 16) + c0, v);
+                    tmem_ld_32x16(sums + c0, v);
                     tmem_ld_wait();
-                    mx_store<YT, GATED>(args, stage, lane, first_col, columns, tile.first + c0, tile.first + tile.rows, v);
+#pragma unroll
+                    for (uint32_t i = 0; i < 16u; ++i) {
+                        __stcg(out + (size_t)(c0 + i) * kMxRows, __uint_as_float(v[i]));
+                    }
+                }
+                release();
+                __syncwarp();
+                if (lane == 0u) {
+                    __threadfence();
+                    st_release_gpu(args.flags + blockIdx.x * kFlagWords + warp, 1u);
+                }
+                continue;
+            }
+            // The blocks behind this one that hold the rest of its depth.
+            uint32_t others = 0u;
+            if (mine.to < steps) {
+                const unsigned long long tile_end = (unsigned long long)(mine.tile + 1u) * steps;
+                while (mx_run_begin(blockIdx.x + others + 1u, gridDim.x, units) < tile_end) {
+                    ++others;
+                }
+                bool there = true;
+                for (uint32_t o = lane; o < others; o += 32u) {
+                    there = there && mx_wait_flag(args.flags + (blockIdx.x + 1u + o) * kFlagWords + warp, &abort_flag, args.status);
+                }
+                if (!__all_sync(0xFFFFFFFFu, there)) {
+                    break;
+                }
+                __syncwarp();
+            }
+            const uint32_t j0 = tile.row0 + warp * 32u;
+            const uint32_t width = args.n > j0 ? (args.n - j0 < 32u ? args.n - j0 : 32u) : 0u;
+            const uint32_t first_col = GATED ? j0 / 2u : j0;
+            const uint32_t columns = GATED ? width / 2u : width;
+            const uint32_t last_row = tile.first + tile.rows < valid || args.offsets != nullptr ? tile.first + tile.rows : valid;
+            for (uint32_t c0 = 0; c0 < tile.rows; c0 += 16u) {
+                uint32_t v[16];
+                tmem_ld_32x16(sums + c0, v);
+                tmem_ld_wait();
+                if (c0 + 16u >= tile.rows) {
+                    release();
+                }
+                if (others != 0u) {
+                    add_partial_sums(v, args.partial + (blockIdx.x + 1u) * args.tile_floats + (size_t)c0 * kMxRows + warp * 32u + lane,
+                                     args.tile_floats, others);
+                }
+                mx_store<YT, GATED>(args, stage, lane, first_col, columns, tile.first + c0, last_row, v);
+            }
+            if (others != 0u) {
+                __syncwarp();
+                for (uint32_t o = lane; o < others; o += 32u) {
+                    args.flags[(blockIdx.x + 1u + o) * kFlagWords + warp] = 0u;   // for the next launch
                 }
             }
         }
     }
-    // (Behind this block's own wait: what runs early after it then overlaps nothing before it.)
     grid_dependency_wait();
     grid_launch_dependents();
     tc_fence_before_sync();
@@ -478,9 +801,45 @@ static cudaError_t launch_typed(cudaStream_t stream, dim3 grid, const CUtensorMa
          : launch_kernel_early(overlap, mx4_product_kernel<YT, false>, grid, kMxThreads, kMxSmem, stream, map_w, map_x, args);
 }
 
-cudaError_t launch_mx4_product(cudaStream_t stream, unsigned int sm_count, const Mx4Product &p)
+// Rows of x per tile: equal parts of at most 256.  By expert, about what one has.
+static uint32_t token_tile(const Mx4Product &p)
 {
-    (void)sm_count;
+    const uint32_t typical = p.offsets != nullptr ? (p.m + p.experts - 1u) / p.experts : p.m;
+    const uint32_t parts = (typical + kMxMaxTok - 1u) / kMxMaxTok;
+    return up_to((typical + parts - 1u) / parts, 16u);
+}
+
+// Blocks of the grid: never more than steps, of which a block has a few at least.
+static uint32_t grid_of(unsigned long long units, uint32_t sm_count)
+{
+    const unsigned long long blocks = (units + kMxFewSteps - 1u) / kMxFewSteps;
+    return blocks < sm_count ? (uint32_t)blocks : sm_count;
+}
+
+// Stages of x that a block of mx4_linear keeps, 0 if that many rows are quantised by a launch of their own.
+static uint32_t linear_slots(uint32_t n, uint32_t k, uint32_t m, uint32_t sm_count)
+{
+    if (m > kMxFusedRows) {
+        return 0u;
+    }
+    const uint32_t ntok = up_to(m, 16u);
+    const uint32_t steps = (k + kMxStageK - 1u) / kMxStageK;
+    const unsigned long long units = (unsigned long long)((n + kMxRows - 1u) / kMxRows) * steps;
+    const uint32_t grid = grid_of(units, sm_count);
+    const unsigned long long run = (units + grid - 1u) / grid;
+    const uint32_t slots = run < steps ? (uint32_t)run : steps;
+    const uint32_t bytes = ntok * kMxStageBytes + 2u * kMxScaleBlock;
+    return slots <= kMxMaxSlots && slots * bytes <= kMxRings / 2u ? slots : 0u;
+}
+
+bool mx4_linear_quantizes(uint32_t n, uint32_t k, uint32_t m, unsigned int sm_count)
+{
+    return linear_slots(n, k, m, sm_count) != 0u;
+}
+
+cudaError_t launch_mx4_product(cudaStream_t stream, const UmmaScratch &scratch, unsigned int sm_count, unsigned int set,
+                               const Mx4Product &p)
+{
     const EncodeTiledFn encode = encode_tiled();
     if (encode == nullptr) {
         return cudaErrorNotSupported;
@@ -501,31 +860,45 @@ cudaError_t launch_mx4_product(cudaStream_t stream, unsigned int sm_count, const
     args.y = p.y;
     args.ldy = p.epilogue == kEpilogueSwiglu ? p.n / 2u : p.n;
     args.epilogue = p.epilogue;
-    args.status = p.status;
+    args.status = scratch.status;
     args.weights_late = p.weights_late ? 1u : 0u;
+    args.partial = scratch.partial + (unsigned long long)(set & 1u) * scratch.blocks * scratch.tile_floats;
+    args.flags = scratch.flags + (unsigned long long)(set & 1u) * scratch.blocks * kFlagWords;
+    args.tile_floats = scratch.tile_floats;
     const uint32_t size = p.y_dtype == 0 ? 4u : 2u;
     args.wide = (reinterpret_cast<uintptr_t>(p.y) & (4u * size - 1u)) == 0u && args.ldy % 4u == 0u;
-    // Rows of x per tile: equal parts of at most 256.  By expert, about what one has.
-    const uint32_t typical = p.offsets != nullptr ? (p.m + p.experts - 1u) / p.experts : p.m;
-    const uint32_t parts = (typical + kMxMaxTok - 1u) / kMxMaxTok;
-    args.ntok = up_to((typical + parts - 1u) / parts, 16u);
-    const uint32_t tok_tiles = p.offsets != nullptr ? p.m / args.ntok + (p.experts < p.m ? p.experts : p.m)
-                                                    : (p.m + args.ntok - 1u) / args.ntok;
+    args.ntok = token_tile(p);
+    const uint32_t blocks = sm_count < scratch.blocks ? sm_count : scratch.blocks;
+    if (p.x != nullptr) {
+        args.x = p.x;
+        args.x_type = (uint32_t)p.x_dtype;
+        args.ldx = p.ldx;
+        args.x_aligned = (reinterpret_cast<uintptr_t>(p.x) & 15u) == 0u && (p.ldx * (p.x_dtype == 0 ? 4u : 2u)) % 16u == 0u;
+        args.slots = linear_slots(p.n, p.k, p.m, blocks);
+    }
     const uint32_t x_blocks = mx_scale_blocks(args.ntok);
-    args.stage_bytes = up_to((kMxRows + args.ntok) * kMxStageBytes + 2u * (1u + x_blocks) * kMxScaleBlock, 1024u);
-    const uint32_t fit = (kMxSmem - 1024u - kMxTail) / args.stage_bytes;
+    const uint32_t x_bytes = args.ntok * kMxStageBytes + 2u * x_blocks * kMxScaleBlock;
+    args.stage_bytes = kMxRows * kMxStageBytes + 2u * kMxScaleBlock + (args.slots != 0u ? 0u : x_bytes);
+    const uint32_t fit = (kMxRings - args.slots * x_bytes) / args.stage_bytes;
     args.stages = fit < kMxMaxStages ? fit : kMxMaxStages;
-    const uint32_t columns = args.ntok + args.stages * 8u * (1u + x_blocks);
+    // Tensor memory: two accumulators where they fit beside the scales of the stages.
+    const uint32_t scale_columns = args.stages * 8u * (1u + x_blocks);
+    args.accumulators = 2u * args.ntok + scale_columns <= 512u ? 2u : 1u;
+    const uint32_t columns = args.accumulators * args.ntok + scale_columns;
     args.tmem_columns = 32u;
     while (args.tmem_columns < columns) {
         args.tmem_columns *= 2u;
     }
-    CUtensorMap map_w, map_x;
+    CUtensorMap map_w, map_x = {};
     if (!map_codes(encode, &map_w, p.w_codes, args.w_rows, p.k, kMxRows)
-        || !map_codes(encode, &map_x, p.x_codes, p.m, p.k, args.ntok)) {
+        || (args.slots == 0u && !map_codes(encode, &map_x, p.x_codes, p.m, p.k, args.ntok))) {
         return cudaErrorInvalidValue;
     }
-    const dim3 grid((p.n + kMxRows - 1u) / kMxRows, tok_tiles, 1);
+    // Tiles at most (by expert and live batch the device knows how many).
+    const unsigned long long tok_tiles = p.offsets != nullptr ? p.m / args.ntok + (p.experts < p.m ? p.experts : p.m)
+                                                              : (p.m + args.ntok - 1u) / args.ntok;
+    const unsigned long long units = tok_tiles * ((p.n + kMxRows - 1u) / kMxRows) * ((p.k + kMxStageK - 1u) / kMxStageK);
+    const dim3 grid(grid_of(units, blocks), 1, 1);
     switch (p.y_dtype) {
     case 0:
         return launch_typed<float>(stream, grid, map_w, map_x, args, p.overlap);

@@ -39,6 +39,17 @@ __device__ __forceinline__ void copy_async_4(uint32_t dst, const void *src, uint
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
+// Arrive on a barrier when all of this thread's own copies so far have landed (counted among the barrier's arrivals).
+__device__ __forceinline__ void copy_async_arrive(uint32_t bar)
+{
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void st_shared_b8(uint32_t addr, uint32_t value)
+{
+    asm volatile("{ .reg .b16 h; cvt.u16.u32 h, %1; st.shared.b8 [%0], h; }" ::"r"(addr), "r"(value) : "memory");
+}
+
 // 32 rows of 16 bytes from shared memory (a descriptor without swizzle) to four columns of tensor memory, the same in each
 // quarter of the lanes: the way a block of scales is laid down for the MMA.
 __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc)

@@ -8,8 +8,7 @@
 #include <cuda_fp16.h>
 
 #include "mx4.h"
-#include "mx4_ptx.cuh"
-#include "q8_common.cuh"
+#include "mx4_block.cuh"
 #include "q8_launch.h"
 
 namespace q8 {
@@ -19,70 +18,6 @@ namespace q8 {
 constexpr uint32_t kQuantThreads = 256;
 constexpr uint32_t kQuantRows = kQuantThreads / 16u;
 constexpr uint32_t kQuantChunks = 4;
-
-template <typename T>
-struct Eight;
-
-template <>
-struct Eight<float> {
-    uint4 a, b;
-    __device__ __forceinline__ void load(const float *p, bool aligned)
-    {
-        if (aligned) {
-            a = *reinterpret_cast<const uint4 *>(p);
-            b = *reinterpret_cast<const uint4 *>(p + 4);
-        } else {
-            const uint32_t *w = reinterpret_cast<const uint32_t *>(p);
-            a = make_uint4(w[0], w[1], w[2], w[3]);
-            b = make_uint4(w[4], w[5], w[6], w[7]);
-        }
-    }
-    __device__ __forceinline__ void floats(float (&v)[8]) const
-    {
-        v[0] = __uint_as_float(a.x), v[1] = __uint_as_float(a.y), v[2] = __uint_as_float(a.z), v[3] = __uint_as_float(a.w);
-        v[4] = __uint_as_float(b.x), v[5] = __uint_as_float(b.y), v[6] = __uint_as_float(b.z), v[7] = __uint_as_float(b.w);
-    }
-};
-
-struct Eight16 {
-    uint32_t w[4];
-    __device__ __forceinline__ void load(const void *p, bool aligned)
-    {
-        if (aligned) {
-            const uint4 a = *static_cast<const uint4 *>(p);
-            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
-        } else {
-            const unsigned short *h = static_cast<const unsigned short *>(p);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                w[i] = (uint32_t)h[2 * i] | (uint32_t)h[2 * i + 1] << 16;
-            }
-        }
-    }
-};
-
-template <>
-struct Eight<__half> : Eight16 {
-    __device__ __forceinline__ void floats(float (&v)[8]) const
-    {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-            v[2 * i] = f.x, v[2 * i + 1] = f.y;
-        }
-    }
-};
-
-template <>
-struct Eight<__nv_bfloat16> : Eight16 {
-    __device__ __forceinline__ void floats(float (&v)[8]) const
-    {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        }
-    }
-};
 
 template <typename T>
 __global__ void __launch_bounds__(kQuantThreads)
@@ -122,24 +57,11 @@ mx4_quantize_kernel(const T *x, uint32_t x_rows, unsigned long long ldx, uint32_
             if (in[i]) {
                 raw[i].floats(v);
             }
-            // magnitudes as whole numbers: a NaN is above everything
-            uint32_t largest = 0u;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t bits = __float_as_uint(v[j]) & 0x7FFFFFFFu;
-                largest = largest > bits ? largest : bits;
-            }
+            uint32_t largest = mx4_largest(v, 0u);
             largest = max(largest, __shfl_xor_sync(0xFFFFFFFFu, largest, 1u));
             largest = max(largest, __shfl_xor_sync(0xFFFFFFFFu, largest, 2u));
-            const uint32_t exponent = largest >> 23;
-            const bool finite = exponent != 255u;
-            const uint32_t scale = !finite ? 255u : (exponent > 2u ? exponent - 2u : 0u);
-            const float inverse = __uint_as_float((254u - (finite ? scale : 0u)) << 23);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[j] = finite ? v[j] * inverse : 0.0f;
-            }
-            const uint32_t word = cvt_e2m1x8(v);
+            const uint32_t scale = mx4_scale(largest);
+            const uint32_t word = mx4_codes(v, scale, mx4_inverse(scale));
             if (in[i]) {
                 codes[(unsigned long long)row * (k / 8u) + (c0 + i) * 16u + lane] = word;
             }

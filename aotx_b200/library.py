@@ -127,7 +127,7 @@ def declare_mx4(lib):
     lib.aotx_mx4_quantize.argtypes = [vp, vp, vp, i32, u32, u64, u32, vp, u32, vp, vp, vp]
     lib.aotx_mx4_dequant.argtypes = [vp, vp, vp, vp, u32, u32, u32, u32, vp, i32]
     lib.aotx_mx4_matmul.argtypes = [vp, vp, vp, vp, u32, u32, vp, vp, u32, vp, vp, i32, i32]
-    lib.aotx_mx4_linear_workspace_bytes.argtypes = [u32, u32]
+    lib.aotx_mx4_linear_workspace_bytes.argtypes = [vp, u32, u32, u32]
     lib.aotx_mx4_linear.argtypes = [vp, vp, vp, vp, u32, u32, vp, i32, u64, u32, vp, vp, i32, i32, vp, C.c_size_t]
     lib.aotx_mx4_moe_order.argtypes = [vp, vp, vp, u32, vp, u32, u32, vp, vp, vp]
     lib.aotx_mx4_matmul_grouped.argtypes = [vp, vp, vp, vp, u32, u32, u32, vp, vp, u32, vp, vp, u32, vp, i32, i32]

@@ -11,15 +11,21 @@ the rest of the context's methods they are for one thread at a time; tensors use
 EPILOGUE_STORE, EPILOGUE_ADD, EPILOGUE_SWIGLU = 0, 1, 2
 
 
+_module = None
+
+
 def _torch():
-    import torch
-    return torch
+    global _module
+    if _module is None:
+        import torch
+        _module = torch
+    return _module
 
 
 class Mx4Tensor:
     """`rows` rows of k values: codes uint8 [rows][k / 2] (value 2i in the low four bits of byte i), scales uint8
     [ceil(k / 128)][rows][4] (byte b of (c, r): values 128c + 32b .. of row r, 2^(byte - 127); 255 is NaN; 0 past k)."""
-    __slots__ = ("codes", "scales", "rows", "k")
+    __slots__ = ("rows", "k", "device", "_codes", "_scales", "_bytes", "_at")
 
     def __init__(self, codes, scales):
         torch = _torch()
@@ -30,66 +36,105 @@ class Mx4Tensor:
             raise ValueError("k is a multiple of 32 and scales are [ceil(k / 128)][rows][4]")
         if not codes.is_contiguous() or not scales.is_contiguous() or codes.device != scales.device:
             raise ValueError("codes and scales lie without gaps on one device")
-        self.codes, self.scales = codes, scales
+        self.device = codes.device
+        self._codes, self._scales = codes, scales
+        self._bytes = None
+        self._at = (codes.data_ptr(), scales.data_ptr())
 
     @classmethod
     def empty(cls, rows, k, device):
-        torch = _torch()
+        """Both arrays in one allocation; their tensors are made when they are asked for."""
         if k <= 0 or k % 32 != 0 or rows < 0:
             raise ValueError("k is a multiple of 32")
-        return cls(torch.empty((rows, k // 2), dtype=torch.uint8, device=device),
-                   torch.empty(((k + 127) // 128, rows, 4), dtype=torch.uint8, device=device))
+        torch = _torch()
+        t = cls.__new__(cls)
+        t.rows, t.k = rows, k
+        # (a row of codes is a multiple of 16 bytes, so the scales behind them lie on such a boundary too)
+        codes = rows * (k // 2)
+        t._bytes = torch.empty(codes + (k + 127) // 128 * rows * 4, dtype=torch.uint8, device=device)
+        t.device = t._bytes.device
+        t._codes = t._scales = None
+        at = t._bytes.data_ptr()
+        t._at = (at, at + codes)
+        return t
+
+    @property
+    def codes(self):
+        if self._codes is None:
+            self._codes = self._bytes[:self.rows * (self.k // 2)].view(self.rows, self.k // 2)
+        return self._codes
+
+    @property
+    def scales(self):
+        if self._scales is None:
+            self._scales = self._bytes[self.rows * (self.k // 2):].view((self.k + 127) // 128, self.rows, 4)
+        return self._scales
 
 
 def _pointer(t):
     return t.data_ptr() if t is not None else None
 
 
+_codes = {}
+
+
+def _dtype_code(dtype):
+    code = _codes.get(dtype)
+    if code is None:
+        torch = _torch()
+        _codes.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+        code = _codes.get(dtype)
+        if code is None:
+            raise ValueError("float32, float16 or bfloat16, not %s" % dtype)
+    return code
+
+
 class Mx4Calls:
     """The part of Q8Context that works on MX4 tensors."""
 
-    def _mx4_here(self, *tensors):
-        for t in tensors:
-            if t is not None and t.device != self.device:
-                raise ValueError("a tensor on %s, a context for %s" % (t.device, self.device))
+    def _mx4_elsewhere(self, t):
+        return ValueError("a tensor on %s, a context for %s" % (t.device, self.device))
 
     def _mx4_words(self, what, t, count=None):
-        """A device array of 32-bit whole numbers."""
-        torch = _torch()
+        """The address of a device array of 32-bit whole numbers, or none."""
         if t is None:
-            return
-        if t.dtype not in (torch.int32, torch.uint32) or not t.is_contiguous():
+            return None
+        torch = _torch()
+        if (t.dtype != torch.int32 and t.dtype != torch.uint32) or not t.is_contiguous():
             raise ValueError("%s is int32 or uint32 without gaps" % what)
         if count is not None and t.numel() != count:
             raise ValueError("%s has %d entries, not %d" % (what, t.numel(), count))
-
-    def _mx4_code(self, dtype):
-        from .q8 import _dtype_code
-        try:
-            return _dtype_code(dtype)
-        except KeyError:
-            raise ValueError("float32, float16 or bfloat16, not %s" % dtype) from None
+        if t.device != self.device:
+            raise self._mx4_elsewhere(t)
+        return t.data_ptr()
 
     def _mx4_rows_in(self, x):
-        """Rows of 16- or 32-bit values: the type's code and the distance of rows."""
-        code = self._mx4_code(x.dtype)
-        if x.dim() != 2 or x.shape[1] == 0 or x.shape[1] % 32 != 0:
+        """Rows of 16- or 32-bit values: their number, their length, the distance of rows."""
+        shape = x.shape
+        if len(shape) != 2 or shape[1] == 0 or shape[1] % 32 != 0:
             raise ValueError("x is [rows][k], k a multiple of 32")
-        if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        rows, k = shape
+        if x.device != self.device:
+            raise self._mx4_elsewhere(x)
+        if x.is_contiguous():
+            return rows, k, k
+        apart, side = x.stride()
+        if side != 1 or (rows > 1 and apart < k):
             raise ValueError("the values of a row lie side by side and rows do not overlap")
-        return code, max(x.stride(0), x.shape[1])
+        return rows, k, max(apart, k)
 
-    def _mx4_result(self, y, shape, y_dtype, epilogue):
-        torch = _torch()
-        if epilogue not in (EPILOGUE_STORE, EPILOGUE_ADD, EPILOGUE_SWIGLU):
+    def _mx4_result(self, y, rows, width, y_dtype, epilogue):
+        if epilogue != EPILOGUE_STORE and epilogue != EPILOGUE_ADD and epilogue != EPILOGUE_SWIGLU:
             raise ValueError("unknown epilogue")
         if y is None:
             if epilogue == EPILOGUE_ADD:
                 raise ValueError("EPILOGUE_ADD adds into a y that the caller gives")
-            return torch.empty(shape, dtype=y_dtype or torch.float32, device=self.device)
-        if tuple(y.shape) != shape or not y.is_contiguous() or (y_dtype is not None and y.dtype != y_dtype):
-            raise ValueError("y is %s without gaps" % (shape,))
-        self._mx4_here(y)
+            torch = _torch()
+            return torch.empty((rows, width), dtype=y_dtype or torch.float32, device=self.device)
+        if tuple(y.shape) != (rows, width) or not y.is_contiguous() or (y_dtype is not None and y.dtype != y_dtype):
+            raise ValueError("y is [%d][%d] without gaps" % (rows, width))
+        if y.device != self.device:
+            raise self._mx4_elsewhere(y)
         return y
 
     def _mx4_width(self, n, epilogue):
@@ -99,24 +144,34 @@ class Mx4Calls:
             return n // 2
         return n
 
+    def _mx4_pair(self, w, k, x=None):
+        if w.k != k:
+            raise ValueError("rows of %d and of %d values" % (w.k, k))
+        if w.device != self.device:
+            raise self._mx4_elsewhere(w)
+        if x is not None and x.device != self.device:
+            raise self._mx4_elsewhere(x)
+
     # -- quantisation -----------------------------------------------------------------------------------------------
     def mx4_quantize(self, x, rows=None, rows_dev=None, out=None):
         """Rows of x (float32, float16, bfloat16; rows may lie apart) as an Mx4Tensor.  `rows`: int32 row numbers of x, one
         for each row of the result (a number outside x leaves its row as it was).  `rows_dev`: device word with the
         live number of rows."""
-        code, stride = self._mx4_rows_in(x)
-        self._mx4_words("rows", rows)
-        self._mx4_words("rows_dev", rows_dev, 1)
-        self._mx4_here(x, rows, rows_dev)
-        count = x.shape[0] if rows is None else rows.numel()
+        code = _dtype_code(x.dtype)
+        have, k, stride = self._mx4_rows_in(x)
+        count = have if rows is None else rows.numel()
         if out is None:
-            out = Mx4Tensor.empty(count, x.shape[1], self.device)
-        elif out.rows != count or out.k != x.shape[1]:
+            out = Mx4Tensor.empty(count, k, self.device)
+        elif out.rows != count or out.k != k:
             raise ValueError("out has %d rows of %d values" % (out.rows, out.k))
-        self._mx4_here(out.codes)
-        self._check(self._mx4_quantize_call(
-            self._address, self._stream(), x.data_ptr(), code, x.shape[0], stride, x.shape[1], _pointer(rows), count,
-            _pointer(rows_dev), out.codes.data_ptr(), out.scales.data_ptr()))
+        elif out.device != self.device:
+            raise self._mx4_elsewhere(out)
+        codes, scales = out._at
+        result = self._mx4_quantize_call(self._address, self._stream(), x.data_ptr(), code, have, stride, k,
+                                         self._mx4_words("rows", rows), count, self._mx4_words("rows_dev", rows_dev, 1),
+                                         codes, scales)
+        if result != 0:
+            self._check(result)
         return out
 
     def mx4_dequant(self, t, first_row=0, rows=None, out=None, dtype=None):
@@ -125,41 +180,47 @@ class Mx4Calls:
         rows = t.rows - first_row if rows is None else rows
         if first_row < 0 or rows < 0 or first_row + rows > t.rows:
             raise ValueError("rows %d .. %d of %d" % (first_row, first_row + rows, t.rows))
+        if t.device != self.device:
+            raise self._mx4_elsewhere(t)
         if out is None:
-            out = torch.empty((rows, t.k), dtype=dtype or torch.float16, device=self.device)
-        elif tuple(out.shape) != (rows, t.k) or not out.is_contiguous() or (dtype is not None and out.dtype != dtype):
-            raise ValueError("out is [%d][%d] without gaps" % (rows, t.k))
-        code = self._mx4_code(out.dtype)
-        self._mx4_here(t.codes, out)
-        self._check(self._mx4_dequant_call(self._address, self._stream(), t.codes.data_ptr(), t.scales.data_ptr(), t.rows, t.k,
-                                           first_row, rows, out.data_ptr(), code))
+            dtype = dtype or torch.float16
+            code = _dtype_code(dtype)
+            out = torch.empty((rows, t.k), dtype=dtype, device=self.device)
+        else:
+            code = _dtype_code(out.dtype)
+            if tuple(out.shape) != (rows, t.k) or not out.is_contiguous() or (dtype is not None and out.dtype != dtype):
+                raise ValueError("out is [%d][%d] without gaps" % (rows, t.k))
+            if out.device != self.device:
+                raise self._mx4_elsewhere(out)
+        codes, scales = t._at
+        result = self._mx4_dequant_call(self._address, self._stream(), codes, scales, t.rows, t.k, first_row, rows,
+                                        out.data_ptr(), code)
+        if result != 0:
+            self._check(result)
         return out
 
     # -- products ---------------------------------------------------------------------------------------------------
     def mx4_matmul(self, w, x, m_dev=None, y=None, y_dtype=None, epilogue=EPILOGUE_STORE):
         """y[m][n] = x . w^T for two MX4 tensors; `m_dev`, `y` and `epilogue` as in `matmul_fused`."""
-        if w.k != x.k:
-            raise ValueError("rows of %d and of %d values" % (w.k, x.k))
-        self._mx4_words("m_dev", m_dev, 1)
-        y = self._mx4_result(y, (x.rows, self._mx4_width(w.rows, epilogue)), y_dtype, epilogue)
-        self._mx4_here(w.codes, x.codes, m_dev)
-        self._check(self._mx4_matmul_call(
-            self._address, self._stream(), w.codes.data_ptr(), w.scales.data_ptr(), w.rows, w.k, x.codes.data_ptr(),
-            x.scales.data_ptr(), x.rows, _pointer(m_dev), y.data_ptr(), self._mx4_code(y.dtype), epilogue))
+        self._mx4_pair(w, x.k, x)
+        y = self._mx4_result(y, x.rows, self._mx4_width(w.rows, epilogue), y_dtype, epilogue)
+        w_codes, w_scales = w._at
+        x_codes, x_scales = x._at
+        result = self._mx4_matmul_call(self._address, self._stream(), w_codes, w_scales, w.rows, w.k, x_codes, x_scales, x.rows,
+                                       self._mx4_words("m_dev", m_dev, 1), y.data_ptr(), _dtype_code(y.dtype), epilogue)
+        if result != 0:
+            self._check(result)
         return y
 
     def mx4_linear(self, w, x, m_dev=None, y=None, y_dtype=None, epilogue=EPILOGUE_STORE, workspace=None):
         """`mx4_matmul` of w with `mx4_quantize(x)`, the same y bit for bit; few rows are quantised by the kernel that
         multiplies them."""
-        code, stride = self._mx4_rows_in(x)
-        m, k = x.shape
-        if w.k != k:
-            raise ValueError("rows of %d and of %d values" % (w.k, k))
-        self._mx4_words("m_dev", m_dev, 1)
-        y = self._mx4_result(y, (m, self._mx4_width(w.rows, epilogue)), y_dtype, epilogue)
-        self._mx4_here(w.codes, x, m_dev, workspace)
-        size = self.lib.aotx_mx4_linear_workspace_bytes(m, k)
+        code = _dtype_code(x.dtype)
+        m, k, stride = self._mx4_rows_in(x)
+        self._mx4_pair(w, k)
+        y = self._mx4_result(y, m, self._mx4_width(w.rows, epilogue), y_dtype, epilogue)
         if workspace is None:
+            size = self.lib.aotx_mx4_linear_workspace_bytes(self._address, w.rows, k, m)
             if size:
                 torch = _torch()
                 workspace = torch.empty(size, dtype=torch.uint8, device=self.device)
@@ -167,9 +228,14 @@ class Mx4Calls:
             size = workspace.numel() * workspace.element_size()
             if not workspace.is_contiguous():
                 raise ValueError("the workspace has gaps")
-        self._check(self._mx4_linear_call(
-            self._address, self._stream(), w.codes.data_ptr(), w.scales.data_ptr(), w.rows, k, x.data_ptr(), code, stride, m,
-            _pointer(m_dev), y.data_ptr(), self._mx4_code(y.dtype), epilogue, _pointer(workspace), size))
+            if workspace.device != self.device:
+                raise self._mx4_elsewhere(workspace)
+        w_codes, w_scales = w._at
+        result = self._mx4_linear_call(self._address, self._stream(), w_codes, w_scales, w.rows, k, x.data_ptr(), code, stride,
+                                       m, self._mx4_words("m_dev", m_dev, 1), y.data_ptr(), _dtype_code(y.dtype), epilogue,
+                                       _pointer(workspace), size)
+        if result != 0:
+            self._check(result)
         return y
 
     # -- routed experts ---------------------------------------------------------------------------------------------
@@ -177,41 +243,46 @@ class Mx4Calls:
         """The (token, rank) pairs of ids [tokens][used] by expert: order (the pair at each place), their tokens, and
         offsets [experts + 1] of the experts' places; int32, places that no pair has hold -1."""
         torch = _torch()
-        self._mx4_words("ids", ids)
-        self._mx4_words("tokens_dev", tokens_dev, 1)
-        if ids.dim() != 2 or ids.shape[1] == 0:
+        shape = ids.shape
+        if len(shape) != 2 or shape[1] == 0:
             raise ValueError("ids is [tokens][used]")
-        self._mx4_here(ids, tokens_dev)
-        tokens, used = ids.shape
-        order = torch.empty(tokens * used, dtype=torch.int32, device=self.device)
-        token_of = torch.empty(tokens * used, dtype=torch.int32, device=self.device)
-        offsets = torch.empty(experts + 1, dtype=torch.int32, device=self.device)
-        self._check(self._mx4_order_call(self._address, self._stream(), ids.data_ptr(), tokens, _pointer(tokens_dev), used,
-                                         experts, order.data_ptr(), token_of.data_ptr(), offsets.data_ptr()))
+        if experts <= 0:
+            raise ValueError("no experts")
+        tokens, used = shape
+        at = self._mx4_words("ids", ids)
+        # one allocation, each part on a 16-byte boundary
+        room = (tokens * used + 3) // 4 * 4
+        words = torch.empty(2 * room + experts + 1, dtype=torch.int32, device=self.device)
+        order, token_of, offsets = words[:tokens * used], words[room:room + tokens * used], words[2 * room:]
+        base = words.data_ptr()
+        result = self._mx4_order_call(self._address, self._stream(), at, tokens, self._mx4_words("tokens_dev", tokens_dev, 1),
+                                      used, experts, base, base + 4 * room, base + 8 * room)
+        if result != 0:
+            self._check(result)
         return order, token_of, offsets
 
     def mx4_matmul_grouped(self, w, experts, x, offsets, y_rows=None, y=None, y_dtype=None, epilogue=EPILOGUE_STORE):
         """Rows offsets[e] .. offsets[e + 1] of x times expert e's rows of w (w.rows / experts each).  `y_rows`: int32, the row
         of y for each row of x (one outside y is left out).  Rows that no expert has are not written."""
-        if w.k != x.k:
-            raise ValueError("rows of %d and of %d values" % (w.k, x.k))
+        self._mx4_pair(w, x.k, x)
         if experts <= 0 or w.rows % experts != 0:
             raise ValueError("%d rows of w for %d experts" % (w.rows, experts))
         if epilogue == EPILOGUE_ADD:
             raise ValueError("grouped products store or apply the gated unit")
-        self._mx4_words("offsets", offsets, experts + 1)
-        self._mx4_words("y_rows", y_rows, x.rows)
         n = w.rows // experts
         width = self._mx4_width(n, epilogue)
         if y is not None and y.dim() != 2:
             raise ValueError("y is [rows][%d]" % width)
         rows = x.rows if y is None or y_rows is None else y.shape[0]
-        y = self._mx4_result(y, (rows, width), y_dtype, epilogue)
-        self._mx4_here(w.codes, x.codes, offsets, y_rows)
-        self._check(self._mx4_grouped_call(
-            self._address, self._stream(), w.codes.data_ptr(), w.scales.data_ptr(), experts, n, w.k, x.codes.data_ptr(),
-            x.scales.data_ptr(), x.rows, offsets.data_ptr(), _pointer(y_rows), rows, y.data_ptr(),
-            self._mx4_code(y.dtype), epilogue))
+        y = self._mx4_result(y, rows, width, y_dtype, epilogue)
+        w_codes, w_scales = w._at
+        x_codes, x_scales = x._at
+        result = self._mx4_grouped_call(self._address, self._stream(), w_codes, w_scales, experts, n, w.k, x_codes, x_scales,
+                                        x.rows, self._mx4_words("offsets", offsets, experts + 1),
+                                        self._mx4_words("y_rows", y_rows, x.rows), rows, y.data_ptr(), _dtype_code(y.dtype),
+                                        epilogue)
+        if result != 0:
+            self._check(result)
         return y
 
     def mx4_moe_ffn(self, w_gate_up, w_down, experts, x, prob, ids, tokens_dev=None, out=None, out_dtype=None):
@@ -228,9 +299,12 @@ class Mx4Calls:
             raise ValueError("w_gate_up is [experts][2 * ffn][hidden] and w_down [experts][hidden][ffn]")
         if ids.shape[1] > experts:
             raise ValueError("more selections than experts")
-        self._mx4_here(prob)
+        if prob.device != self.device:
+            raise self._mx4_elsewhere(prob)
         tokens, used = ids.shape
         hidden = x.shape[1]
+        if out is not None and (tuple(out.shape) != (tokens, hidden) or not out.is_contiguous() or out.device != self.device):
+            raise ValueError("out is [%d][%d] without gaps" % (tokens, hidden))
         order, token_of, offsets = self.moe_order(ids, experts, tokens_dev=tokens_dev)
         feed = self.mx4_quantize(x, rows=token_of)
         act = self.mx4_matmul_grouped(w_gate_up, experts, feed, offsets, y_dtype=torch.float16, epilogue=EPILOGUE_SWIGLU)

@@ -55,7 +55,7 @@ int aotx_mx4_matmul(aotx_q8_ctx *ctx, void *stream, const void *w_codes, const v
 /* aotx_mx4_quantize of x, then aotx_mx4_matmul: the same y, bit for bit.  Few rows are quantised by the kernel that
  * multiplies them; otherwise `workspace` (16-byte aligned device memory of aotx_mx4_linear_workspace_bytes; 0 where none is
  * needed) holds x in MX4 between the two. */
-size_t aotx_mx4_linear_workspace_bytes(uint32_t m, uint32_t k);
+size_t aotx_mx4_linear_workspace_bytes(const aotx_q8_ctx *ctx, uint32_t n, uint32_t k, uint32_t m);
 int aotx_mx4_linear(aotx_q8_ctx *ctx, void *stream, const void *w_codes, const void *w_scales, uint32_t n, uint32_t k,
                     const void *x, int x_dtype, uint64_t ldx, uint32_t m, const uint32_t *m_dev, void *y, int y_dtype,
                     int epilogue, void *workspace, size_t workspace_bytes);

@@ -105,7 +105,8 @@ def test_nothing_to_do_is_no_error(lib, ctx):
 
 def test_workspace_of_a_linear_call(lib, ctx):
     m, k = 300, 96
-    size = lib.aotx_mx4_linear_workspace_bytes(m, k)
+    n = GOOD["aotx_mx4_linear"]["n"]
+    size = lib.aotx_mx4_linear_workspace_bytes(ctx, n, k, m)
     assert size >= m * k // 2 + m * 4
     call = dict(GOOD["aotx_mx4_linear"], m=m, k=k, ldx=k)
     for wrong in (dict(workspace=0), dict(workspace=P + 8), dict(workspace_bytes=size - 1)):
@@ -127,7 +128,7 @@ class OnCpu(Mx4Calls):
         for name in ("quantize", "dequant", "matmul", "linear", "order", "grouped"):
             setattr(self, "_mx4_%s_call" % name, reached)
 
-    def aotx_mx4_linear_workspace_bytes(self, m, k):
+    def aotx_mx4_linear_workspace_bytes(self, ctx, n, k, m):
         return 64
 
     def _stream(self):
