@@ -10,7 +10,7 @@
 //     memory, so rows may start anywhere, as the rows of an expert do.
 //   * One thread issues the copies of the scales and the MMAs behind them (they run in that order).  Each stage has its own
 //     columns of tensor memory for scales, so that nothing is overwritten before its MMAs are done.
-//   * Four warps store: the sums of 16 rows of x are turned round in shared memory, 16 bytes a lane.
+//   * Eight warps store: the sums of 16 rows of x are turned round in shared memory, 16 bytes a lane.
 //   * The grid is at most one block per SM, and the steps of all tiles (a tile by one stage) are dealt to it in equal runs, so
 //     copies go on from tile to tile and every SM streams to the end.  A tile that is cut between blocks belongs to the one
 //     with its first step: the others leave their sums in the context's scratch and raise a flag per warp (a block does so
@@ -26,10 +26,11 @@
 
 namespace q8 {
 
-constexpr uint32_t kMxThreads = 320;
-constexpr uint32_t kMxScaleWarp = 4;        // the first of four
-constexpr uint32_t kMxCopyWarp = 8;
-constexpr uint32_t kMxMmaWarp = 9;
+constexpr uint32_t kMxThreads = 14 * 32;
+constexpr uint32_t kMxStoreWarps = 8;       // two for each quarter of tensor memory's lanes, which take its columns in turn
+constexpr uint32_t kMxScaleWarp = 8;        // the first of four
+constexpr uint32_t kMxCopyWarp = 12;
+constexpr uint32_t kMxMmaWarp = 13;
 constexpr uint32_t kMxRows = 128;           // rows of w per tile
 constexpr uint32_t kMxMaxTok = 256;         // rows of x per tile, at most
 constexpr uint32_t kMxStageK = 256;         // values of a row per stage
@@ -41,7 +42,7 @@ constexpr uint32_t kMxEpilogueStage = 16u * 32u * 4u;  // per storing warp
 constexpr uint32_t kMxFewSteps = 2;         // steps of a block, at least
 constexpr uint32_t kMxFusedRows = 32;       // rows of x that the kernel quantises itself, at most
 constexpr uint32_t kMxBars = 2 * kMxMaxStages + 4 + kMxMaxSlots;
-constexpr uint32_t kMxTail = 4u * kMxEpilogueStage + kMxBars * 8u;
+constexpr uint32_t kMxTail = kMxStoreWarps * kMxEpilogueStage + kMxBars * 8u;
 constexpr uint32_t kMxSmem = 223u * 1024u;
 constexpr uint32_t kMxRings = (kMxSmem - 1024u - kMxTail) / 1024u * 1024u;
 
@@ -247,67 +248,74 @@ __device__ __forceinline__ bool mx_wait_flag(const unsigned int *flag, volatile 
     return true;
 }
 
-// One block of 32 values of x for the MMA: 16 bytes of codes at `cell`, its scale's byte at `scale_at`.
-template <typename T>
-__device__ __forceinline__ void mx_quantize_block(const T *x, bool aligned, uint32_t cell, uint32_t scale_at)
-{
-    Eight<T> raw[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        raw[i].load(x + 8 * i, aligned);
-    }
-    float v[8];
-    uint32_t largest = 0u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        raw[i].floats(v);
-        largest = mx4_largest(v, largest);
-    }
-    const uint32_t scale = mx4_scale(largest);
-    const float inverse = mx4_inverse(scale);
-    uint32_t word[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        raw[i].floats(v);
-        word[i] = mx4_codes(v, scale, inverse);
-    }
-    st_shared_v4(cell, word[0], word[1], word[2], word[3]);
-    st_shared_b8(scale_at, scale);
-}
-
-// The stages of x that this block needs, in the order in which it needs them, by the 128 threads of four warps.  Each warp
-// arrives on a stage's barrier when its part of it is there.
+// The stages of x that this block needs, in the order in which it needs them, by the storing warps: a thread takes a block of
+// 32 values, the loads of several such blocks together.  Each warp arrives on a stage's barrier when its part of it is there.
 template <typename T>
 __device__ __forceinline__ void mx_quantize_x(const MxArgs &args, const T *x, uint32_t place, uint32_t slot_bytes,
                                               uint32_t bars, uint32_t first_step, uint32_t slots, uint32_t steps, uint32_t live)
 {
+    constexpr uint32_t kThreads = kMxStoreWarps * 32u;
+    constexpr uint32_t kTogether = sizeof(T) == 4u ? 2u : 4u;
     const uint32_t t = threadIdx.x;
+    const uint32_t items = live * 8u;      // blocks of 32 in a stage
+    const uint32_t all = slots * items;
     // rows past the last and values past k stay zero
-    for (uint32_t at = t * 16u; at < slots * slot_bytes; at += 128u * 16u) {
+    for (uint32_t at = t * 16u; at < slots * slot_bytes; at += kThreads * 16u) {
         st_shared_v4(place + at, 0u, 0u, 0u, 0u);
     }
-    named_bar_sync(1u, 128u);
-    const uint32_t items = live * 8u;      // blocks of 32 in a stage
+    named_bar_sync(1u, kThreads);
     uint32_t told = 0u;                    // stages whose barrier this warp has arrived on
-    for (uint32_t base = 0; base < slots * items; base += 128u) {
-        const uint32_t item = base + t;
-        if (item < slots * items) {
-            const uint32_t slot = item / items;
-            const uint32_t row = (item - slot * items) / 8u;
-            const uint32_t b = item & 7u;
-            const uint32_t step = first_step + slot < steps ? first_step + slot : first_step + slot - steps;
-            const uint32_t at = step * kMxStageK + b * 32u;
-            if (at < args.k) {
-                const uint32_t stage = place + slot * slot_bytes;
-                mx_quantize_block<T>(x + (unsigned long long)row * args.ldx + at, args.x_aligned != 0u,
-                                     stage + row * kMxStageBytes + ((b ^ (row & 7u)) * 16u),
-                                     stage + args.ntok * kMxStageBytes + (b / 4u) * kMxScaleBlock + (row % 32u) * 16u
-                                         + (row / 32u) * 4u + b % 4u);
+    for (uint32_t base = 0; base < all; base += kThreads * kTogether) {
+        Eight<T> raw[kTogether][4];
+        uint32_t cell[kTogether], scale_at[kTogether];
+#pragma unroll
+        for (uint32_t j = 0; j < kTogether; ++j) {
+            const uint32_t item = base + j * kThreads + t;
+            cell[j] = 0u;
+            if (item < all) {
+                const uint32_t slot = item / items;
+                const uint32_t row = (item - slot * items) / 8u;
+                const uint32_t b = item & 7u;
+                const uint32_t step = first_step + slot < steps ? first_step + slot : first_step + slot - steps;
+                const uint32_t at = step * kMxStageK + b * 32u;
+                if (at < args.k) {
+                    const uint32_t stage = place + slot * slot_bytes;
+                    const T *from = x + (unsigned long long)row * args.ldx + at;
+                    cell[j] = stage + row * kMxStageBytes + ((b ^ (row & 7u)) * 16u);
+                    scale_at[j] = stage + args.ntok * kMxStageBytes + (b / 4u) * kMxScaleBlock + (row % 32u) * 16u + b % 4u;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        raw[j][i].load(from + 8 * i, args.x_aligned != 0u);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kTogether; ++j) {
+            if (cell[j] != 0u) {
+                float v[8];
+                uint32_t largest = 0u;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    raw[j][i].floats(v);
+                    largest = mx4_largest(v, largest);
+                }
+                const uint32_t scale = mx4_scale(largest);
+                const float inverse = mx4_inverse(scale);
+                uint32_t word[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    raw[j][i].floats(v);
+                    word[i] = mx4_codes(v, scale, inverse);
+                }
+                st_shared_v4(cell[j], word[0], word[1], word[2], word[3]);
+                st_shared_b8(scale_at[j], scale);
             }
         }
         fence_proxy_async_smem();
         __syncwarp();
-        const uint32_t whole = base + 128u < slots * items ? (base + 128u) / items : slots;
+        const uint32_t through = base + kThreads * kTogether;
+        const uint32_t whole = through < all ? through / items : slots;
         for (; told < whole; ++told) {
             if ((t & 31u) == 0u) {
                 mbar_arrive(bars + told * 8u);
@@ -323,81 +331,105 @@ __device__ __forceinline__ void mx_quantize_x(const MxArgs &args, const T *x, ui
     }
 }
 
-// 16 rows of x (v: this lane's row of w for each) to y, rows `first` and up below `end`.
+// 16 rows of x (v: this lane's row of w for each) to y, rows `first` and up below `end`; `row_y`: lane i's is the row of y of row i.
+// They are turned round in the warp's own shared memory and written 16 bytes a lane.  GATED: neighbouring lanes hold gate
+// and up of a column (arithmetic of cuda/model/norm.cu:92-105); of two rows of x the even lane forms the first's value and
+// the odd lane the second's.
 template <typename YT, bool GATED>
 __device__ __forceinline__ void mx_store(const MxArgs &args, uint32_t stage, uint32_t lane, uint32_t first_col, uint32_t columns,
-                                         uint32_t first, uint32_t end, const uint32_t (&v)[16])
+                                         uint32_t row_y, const uint32_t (&v)[16])
 {
     constexpr uint32_t kColumns = GATED ? 16u : 32u;
     constexpr uint32_t kRowBytes = kColumns * sizeof(YT);
-    constexpr uint32_t kLanesPerRow = kColumns / 4u;
+    constexpr uint32_t kPiece = 16u / sizeof(YT);
+    constexpr uint32_t kLanesPerRow = kRowBytes / 16u;
     constexpr uint32_t kRowsPerStep = 32u / kLanesPerRow;
-    // lane i knows the row of y of row i
-    uint32_t row_y = 0xFFFFFFFFu;
-    if (lane < 16u && first + lane < end) {
-        row_y = args.y_rows_of != nullptr ? args.y_rows_of[first + lane] : first + lane;
-        if (row_y >= args.y_rows) {
-            row_y = 0xFFFFFFFFu;
-        }
-    }
-    const uint32_t column = GATED ? lane / 2u : lane;
-    __syncwarp();
-#pragma unroll
-    for (uint32_t i = 0; i < 16u; ++i) {
-        float value = __uint_as_float(v[i]);
-        if (GATED) {
-            const float other = __shfl_xor_sync(0xFFFFFFFFu, value, 1u);
-            value = gated_unit(value, other);
-        }
-        if (!GATED || (lane & 1u) == 0u) {
-            if (sizeof(YT) == 4) {
-                st_shared_b32(stage + i * kRowBytes + column * 4u, __float_as_uint(value));
-            } else {
-                st_shared_b16(stage + i * kRowBytes + column * 2u, out_bits<YT>(value));
-            }
-        }
-    }
-    __syncwarp();
-    const uint32_t part = lane % kLanesPerRow;
-    const bool adds = !GATED && sizeof(YT) == 4 && args.epilogue == kEpilogueAdd;
-#pragma unroll
-    for (uint32_t step = 0; step < 16u / kRowsPerStep; ++step) {
-        const uint32_t local = step * kRowsPerStep + lane / kLanesPerRow;
-        const uint32_t row = __shfl_sync(0xFFFFFFFFu, row_y, local);
-        const uint32_t from = stage + local * kRowBytes + part * 4u * sizeof(YT);
-        if (row == 0xFFFFFFFFu || part * 4u >= columns) {
-            continue;
-        }
-        YT *at = static_cast<YT *>(args.y) + (size_t)row * args.ldy + first_col + part * 4u;
-        uint32_t a, b, c = 0u, d = 0u;
+    auto put = [&](uint32_t row, uint32_t column, float value) {
         if (sizeof(YT) == 4) {
-            ld_shared_v4(from, a, b, c, d);
+            st_shared_b32(stage + row * kRowBytes + column * 4u, __float_as_uint(value));
         } else {
-            ld_shared_v2(from, a, b);
+            st_shared_b16(stage + row * kRowBytes + column * 2u, out_bits<YT>(value));
         }
-        if (args.wide != 0u) {
-            if (sizeof(YT) == 4) {
-                float4 piece = make_float4(__uint_as_float(a), __uint_as_float(b), __uint_as_float(c), __uint_as_float(d));
+    };
+    __syncwarp();                  // the rows before these are out of it
+    if (GATED) {
+        const bool odd = (lane & 1u) != 0u;
+#pragma unroll
+        for (uint32_t i = 0; i < 16u; i += 2u) {
+            const float give = __uint_as_float(odd ? v[i] : v[i + 1u]);
+            const float keep = __uint_as_float(odd ? v[i + 1u] : v[i]);
+            const float got = __shfl_xor_sync(0xFFFFFFFFu, give, 1u);
+            put(i + (odd ? 1u : 0u), lane / 2u, gated_unit(odd ? got : keep, odd ? keep : got));
+        }
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 16u; ++i) {
+            put(i, lane, __uint_as_float(v[i]));
+        }
+    }
+    __syncwarp();
+    const bool adds = !GATED && sizeof(YT) == 4 && args.epilogue == kEpilogueAdd;
+    if (args.wide != 0u) {
+        const uint32_t part = lane % kLanesPerRow;
+#pragma unroll
+        for (uint32_t step = 0; step < 16u / kRowsPerStep; ++step) {
+            const uint32_t local = step * kRowsPerStep + lane / kLanesPerRow;
+            const uint32_t row = __shfl_sync(0xFFFFFFFFu, row_y, local);
+            uint32_t a, b, c, d;
+            ld_shared_v4(stage + local * kRowBytes + part * 16u, a, b, c, d);
+            if (row != 0xFFFFFFFFu && part * kPiece < columns) {
+                YT *at = static_cast<YT *>(args.y) + (size_t)row * args.ldy + first_col + part * kPiece;
                 if (adds) {
                     const float4 before = *reinterpret_cast<const float4 *>(at);
-                    piece = make_float4(before.x + piece.x, before.y + piece.y, before.z + piece.z, before.w + piece.w);
+                    a = __float_as_uint(before.x + __uint_as_float(a));
+                    b = __float_as_uint(before.y + __uint_as_float(b));
+                    c = __float_as_uint(before.z + __uint_as_float(c));
+                    d = __float_as_uint(before.w + __uint_as_float(d));
                 }
-                *reinterpret_cast<float4 *>(at) = piece;
-            } else {
-                *reinterpret_cast<uint2 *>(at) = make_uint2(a, b);
+                *reinterpret_cast<uint4 *>(at) = make_uint4(a, b, c, d);
             }
-        } else {
-            const uint32_t words[4] = {a, b, c, d};
+        }
+    } else {
+        // rows of y off the boundary: a value a lane
+#pragma unroll 4
+        for (uint32_t i = 0; i < 16u; ++i) {
+            const uint32_t row = __shfl_sync(0xFFFFFFFFu, row_y, i);
+            if (row == 0xFFFFFFFFu || lane >= columns) {
+                continue;
+            }
+            YT *at = static_cast<YT *>(args.y) + (size_t)row * args.ldy + first_col + lane;
+            if (sizeof(YT) == 4) {
+                const float value = ld_shared_f32(stage + i * kRowBytes + lane * 4u);
+                *reinterpret_cast<float *>(at) = adds ? *reinterpret_cast<float *>(at) + value : value;
+            } else {
+                *reinterpret_cast<unsigned short *>(at) = ld_shared_u16(stage + i * kRowBytes + lane * 2u);
+            }
+        }
+    }
+}
+
+// What `others` blocks left of one piece (16 rows of x by 32 rows of w, a slot every `stride` floats), added in their order;
+// the values of up to three blocks are on their way together.
+__device__ __forceinline__ void mx_add_partials(uint32_t (&v)[16], const float *slots, unsigned long long stride, uint32_t others)
+{
+#pragma unroll 1
+    for (uint32_t o = 0; o < others; o += 3u) {
+        float more[3][16];
 #pragma unroll
-            for (uint32_t i = 0; i < 4u; ++i) {
-                if (part * 4u + i < columns) {
-                    if (sizeof(YT) == 4) {
-                        float *cell = reinterpret_cast<float *>(at) + i;
-                        const float piece = __uint_as_float(words[i]);
-                        *cell = adds ? *cell + piece : piece;
-                    } else {
-                        reinterpret_cast<unsigned short *>(at)[i] = (unsigned short)(words[i / 2u] >> (16u * (i & 1u)));
-                    }
+        for (uint32_t j = 0; j < 3u; ++j) {
+            if (o + j < others) {
+#pragma unroll
+                for (uint32_t i = 0; i < 16u; ++i) {
+                    more[j][i] = __ldcg(slots + (o + j) * stride + i * kMxRows);
+                }
+            }
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 3u; ++j) {
+            if (o + j < others) {
+#pragma unroll
+                for (uint32_t i = 0; i < 16u; ++i) {
+                    v[i] = __float_as_uint(__uint_as_float(v[i]) + more[j][i]);
                 }
             }
         }
@@ -426,7 +458,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const uint32_t place = base + stages * args.stage_bytes;
     const uint32_t slot_bytes = args.ntok * kMxStageBytes + 2u * x_blocks * kMxScaleBlock;
     const uint32_t tail = base + kMxRings;
-    const uint32_t bars = tail + 4u * kMxEpilogueStage;
+    const uint32_t bars = tail + kMxStoreWarps * kMxEpilogueStage;
     auto full = [&](uint32_t s) { return bars + s * 8u; };           // codes and scales are there
     auto empty = [&](uint32_t s) { return bars + (kMxMaxStages + s) * 8u; };
     auto summed = [&](uint32_t b) { return bars + (2u * kMxMaxStages + b) * 8u; };
@@ -445,10 +477,10 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         }
         for (uint32_t b = 0; b < 2u; ++b) {
             mbar_init(summed(b), 1u);
-            mbar_init(taken(b), 4u);
+            mbar_init(taken(b), kMxStoreWarps);
         }
         for (uint32_t s = 0; s < args.slots; ++s) {
-            mbar_init(x_bars + s * 8u, 4u);
+            mbar_init(x_bars + s * 8u, kMxStoreWarps);
         }
         mbar_init_fence();
     }
@@ -644,7 +676,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             }
         }
         copy_async_wait_all();
-    } else if (warp < kMxScaleWarp) {
+    } else if (warp < kMxStoreWarps) {
         grid_dependency_wait();       // x, y, the row map and the scratch
         const uint32_t valid = live_rows();
         if (stays) {
@@ -663,26 +695,28 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             }
         }
         const uint32_t stage = tail + warp * kMxEpilogueStage;
-        const uint32_t lane_taddr = tmem + ((warp * 32u) << 16);
+        const uint32_t quarter = (warp & 3u) * 32u;            // this warp's lanes of tensor memory, rows of w
+        const uint32_t c_first = (warp >> 2) * 16u;            // and its columns, rows of x: 16 of every 32
+        const uint32_t lane_taddr = tmem + (quarter << 16);
         for (MxRing ring; mine.next(); ring.next(args.accumulators)) {
-            const uint32_t buffer = ring.at;
             const MxTile tile = mx_tile(args, groups, mine.tile, tok_tiles, live);
-            if (!mbar_wait(summed(buffer), ring.parity, &abort_flag, args.status)) {
+            if (!mbar_wait(summed(ring.at), ring.parity, &abort_flag, args.status)) {
                 break;
             }
             tc_fence_after_sync();
-            const uint32_t sums = lane_taddr + buffer * args.ntok;
+            const uint32_t sums = lane_taddr + ring.at * args.ntok;
+            const uint32_t giving = taken(ring.at);
             auto release = [&] {
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0u) {
-                    mbar_arrive(taken(buffer));
+                    mbar_arrive(giving);
                 }
             };
             if (mine.from != 0u) {
                 // Another block owns the tile: its sums go to the scratch.
-                float *out = args.partial + blockIdx.x * args.tile_floats + warp * 32u + lane;
-                for (uint32_t c0 = 0; c0 < tile.rows; c0 += 16u) {
+                float *out = args.partial + blockIdx.x * args.tile_floats + quarter + lane;
+                for (uint32_t c0 = c_first; c0 < tile.rows; c0 += 32u) {
                     uint32_t v[16];
                     tmem_ld_32x16(sums + c0, v);
                     tmem_ld_wait();
@@ -692,7 +726,6 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     }
                 }
                 release();
-                __syncwarp();
                 if (lane == 0u) {
                     __threadfence();
                     st_release_gpu(args.flags + blockIdx.x * kFlagWords + warp, 1u);
@@ -715,29 +748,37 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 }
                 __syncwarp();
             }
-            const uint32_t j0 = tile.row0 + warp * 32u;
+            const uint32_t j0 = tile.row0 + quarter;
             const uint32_t width = args.n > j0 ? (args.n - j0 < 32u ? args.n - j0 : 32u) : 0u;
             const uint32_t first_col = GATED ? j0 / 2u : j0;
             const uint32_t columns = GATED ? width / 2u : width;
             const uint32_t last_row = tile.first + tile.rows < valid || args.offsets != nullptr ? tile.first + tile.rows : valid;
-            for (uint32_t c0 = 0; c0 < tile.rows; c0 += 16u) {
+            if (c_first >= tile.rows) {
+                release();
+            }
+            for (uint32_t c0 = c_first; c0 < tile.rows; c0 += 32u) {
+                // lane i knows the row of y of row i of x
+                uint32_t row_y = 0xFFFFFFFFu;
+                const uint32_t row_x = tile.first + c0 + lane;
+                if (lane < 16u && row_x < last_row) {
+                    row_y = args.y_rows_of != nullptr ? args.y_rows_of[row_x] : row_x;
+                    row_y = row_y < args.y_rows ? row_y : 0xFFFFFFFFu;
+                }
                 uint32_t v[16];
                 tmem_ld_32x16(sums + c0, v);
                 tmem_ld_wait();
-                if (c0 + 16u >= tile.rows) {
+                if (c0 + 32u >= tile.rows) {
                     release();
                 }
                 if (others != 0u) {
-                    add_partial_sums(v, args.partial + (blockIdx.x + 1u) * args.tile_floats + (size_t)c0 * kMxRows + warp * 32u + lane,
-                                     args.tile_floats, others);
+                    mx_add_partials(v, args.partial + (blockIdx.x + 1u) * args.tile_floats + (size_t)c0 * kMxRows + quarter + lane,
+                                    args.tile_floats, others);
                 }
-                mx_store<YT, GATED>(args, stage, lane, first_col, columns, tile.first + c0, last_row, v);
+                mx_store<YT, GATED>(args, stage, lane, first_col, columns, row_y, v);
             }
-            if (others != 0u) {
-                __syncwarp();
-                for (uint32_t o = lane; o < others; o += 32u) {
-                    args.flags[(blockIdx.x + 1u + o) * kFlagWords + warp] = 0u;   // for the next launch
-                }
+            __syncwarp();
+            for (uint32_t o = lane; o < others; o += 32u) {
+                args.flags[(blockIdx.x + 1u + o) * kFlagWords + warp] = 0u;   // for the next launch
             }
         }
     }
@@ -866,7 +907,7 @@ cudaError_t launch_mx4_product(cudaStream_t stream, const UmmaScratch &scratch, 
     args.flags = scratch.flags + (unsigned long long)(set & 1u) * scratch.blocks * kFlagWords;
     args.tile_floats = scratch.tile_floats;
     const uint32_t size = p.y_dtype == 0 ? 4u : 2u;
-    args.wide = (reinterpret_cast<uintptr_t>(p.y) & (4u * size - 1u)) == 0u && args.ldy % 4u == 0u;
+    args.wide = (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0u && (args.ldy * size) % 16u == 0u;
     args.ntok = token_tile(p);
     const uint32_t blocks = sm_count < scratch.blocks ? sm_count : scratch.blocks;
     if (p.x != nullptr) {

@@ -50,6 +50,13 @@ __device__ __forceinline__ void st_shared_b8(uint32_t addr, uint32_t value)
     asm volatile("{ .reg .b16 h; cvt.u16.u32 h, %1; st.shared.b8 [%0], h; }" ::"r"(addr), "r"(value) : "memory");
 }
 
+__device__ __forceinline__ unsigned short ld_shared_u16(uint32_t addr)
+{
+    unsigned short v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
+    return v;
+}
+
 // 32 rows of 16 bytes from shared memory (a descriptor without swizzle) to four columns of tensor memory, the same in each
 // quarter of the lanes: the way a block of scales is laid down for the MMA.
 __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc)
