@@ -40,8 +40,11 @@ constexpr uint32_t kMxMaxSlots = 64;        // stages of x that stay
 constexpr uint32_t kMxScaleBlock = 512;     // scales of 128 rows and 128 values
 constexpr uint32_t kMxEpilogueStage = 16u * 32u * 4u;  // per storing warp
 constexpr uint32_t kMxFewSteps = 2;         // steps of a block, at least
+constexpr uint32_t kMxMaxCluster = 8;
+constexpr uint32_t kMxClusterTiles = 72;    // tiles of a product that is multiplied by clusters, at most
+constexpr uint32_t kMxClusterTok = 128;     // and rows of x per tile
 constexpr uint32_t kMxFusedRows = 32;       // rows of x that the kernel quantises itself, at most
-constexpr uint32_t kMxBars = 2 * kMxMaxStages + 4 + kMxMaxSlots;
+constexpr uint32_t kMxBars = 2 * kMxMaxStages + 5 + kMxMaxSlots;
 constexpr uint32_t kMxTail = kMxStoreWarps * kMxEpilogueStage + kMxBars * 8u;
 constexpr uint32_t kMxSmem = 223u * 1024u;
 constexpr uint32_t kMxRings = (kMxSmem - 1024u - kMxTail) / 1024u * 1024u;
@@ -72,6 +75,8 @@ struct MxArgs {
     uint32_t x_aligned;
     unsigned long long ldx;
     uint32_t slots;                // 0: x is in MX4 and goes through the ring
+    uint32_t cluster;              // blocks that share a tile; 0: the steps of all tiles are dealt in equal runs
+    uint32_t share;                // columns of the tile that a block of the cluster adds up and stores
     float *partial;                // per block: [row of x][row of w], and its flags
     unsigned int *flags;
     unsigned long long tile_floats;
@@ -248,84 +253,79 @@ __device__ __forceinline__ bool mx_wait_flag(const unsigned int *flag, volatile 
     return true;
 }
 
-// The stages of x that this block needs, in the order in which it needs them, by the storing warps: a thread takes a block of
-// 32 values, the loads of several such blocks together.  Each warp arrives on a stage's barrier when its part of it is there.
+// The stages of x that this block needs, in the order in which it needs them, by the storing warps: a warp takes a row of a
+// stage, 8 values a lane and four lanes a block of 32, the loads of several such rows together.  A warp arrives on a stage's
+// barrier when its rows of it are there.  (The places hold zeros before: rows past the last, values past k.)
 template <typename T>
 __device__ __forceinline__ void mx_quantize_x(const MxArgs &args, const T *x, uint32_t place, uint32_t slot_bytes,
                                               uint32_t bars, uint32_t first_step, uint32_t slots, uint32_t steps, uint32_t live)
 {
-    constexpr uint32_t kThreads = kMxStoreWarps * 32u;
-    constexpr uint32_t kTogether = sizeof(T) == 4u ? 2u : 4u;
-    const uint32_t t = threadIdx.x;
-    const uint32_t items = live * 8u;      // blocks of 32 in a stage
-    const uint32_t all = slots * items;
-    // rows past the last and values past k stay zero
-    for (uint32_t at = t * 16u; at < slots * slot_bytes; at += kThreads * 16u) {
-        st_shared_v4(place + at, 0u, 0u, 0u, 0u);
-    }
-    named_bar_sync(1u, kThreads);
+    constexpr uint32_t kTogether = sizeof(T) == 4u ? 4u : 8u;
+    const uint32_t warp = threadIdx.x >> 5;
+    const uint32_t lane = threadIdx.x & 31u;
+    const uint32_t block = lane / 4u;
+    // the next row of the next stage, for the loads and for the stores
+    uint32_t slot = 0u, row = warp;
     uint32_t told = 0u;                    // stages whose barrier this warp has arrived on
-    for (uint32_t base = 0; base < all; base += kThreads * kTogether) {
-        Eight<T> raw[kTogether][4];
+    while (row >= live && slot < slots) {
+        row -= live;
+        ++slot;
+        if (live == 0u) {
+            slot = slots;
+        }
+    }
+    while (slot < slots) {
+        Eight<T> raw[kTogether];
         uint32_t cell[kTogether], scale_at[kTogether];
 #pragma unroll
         for (uint32_t j = 0; j < kTogether; ++j) {
-            const uint32_t item = base + j * kThreads + t;
             cell[j] = 0u;
-            if (item < all) {
-                const uint32_t slot = item / items;
-                const uint32_t row = (item - slot * items) / 8u;
-                const uint32_t b = item & 7u;
+            if (slot < slots) {
                 const uint32_t step = first_step + slot < steps ? first_step + slot : first_step + slot - steps;
-                const uint32_t at = step * kMxStageK + b * 32u;
+                const uint32_t at = step * kMxStageK + lane * 8u;
+                const uint32_t stage = place + slot * slot_bytes;
                 if (at < args.k) {
-                    const uint32_t stage = place + slot * slot_bytes;
-                    const T *from = x + (unsigned long long)row * args.ldx + at;
-                    cell[j] = stage + row * kMxStageBytes + ((b ^ (row & 7u)) * 16u);
-                    scale_at[j] = stage + args.ntok * kMxStageBytes + (b / 4u) * kMxScaleBlock + (row % 32u) * 16u + b % 4u;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        raw[j][i].load(from + 8 * i, args.x_aligned != 0u);
-                    }
+                    cell[j] = stage + row * kMxStageBytes + ((block ^ (row & 7u)) * 16u) + (lane & 3u) * 4u;
+                    raw[j].load(x + (unsigned long long)row * args.ldx + at, args.x_aligned != 0u);
+                }
+                scale_at[j] = stage + args.ntok * kMxStageBytes + (block / 4u) * kMxScaleBlock + (row % 32u) * 16u + block % 4u;
+                row += kMxStoreWarps;
+                while (row >= live) {
+                    row -= live;
+                    ++slot;
                 }
             }
         }
 #pragma unroll
         for (uint32_t j = 0; j < kTogether; ++j) {
+            float v[8] = {};
             if (cell[j] != 0u) {
-                float v[8];
-                uint32_t largest = 0u;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    raw[j][i].floats(v);
-                    largest = mx4_largest(v, largest);
+                raw[j].floats(v);
+            }
+            uint32_t largest = mx4_largest(v, 0u);
+            largest = max(largest, __shfl_xor_sync(0xFFFFFFFFu, largest, 1u));
+            largest = max(largest, __shfl_xor_sync(0xFFFFFFFFu, largest, 2u));
+            const uint32_t scale = mx4_scale(largest);
+            const uint32_t word = mx4_codes(v, scale, mx4_inverse(scale));
+            if (cell[j] != 0u) {
+                st_shared_b32(cell[j], word);
+                if ((lane & 3u) == 0u) {
+                    st_shared_b8(scale_at[j], scale);
                 }
-                const uint32_t scale = mx4_scale(largest);
-                const float inverse = mx4_inverse(scale);
-                uint32_t word[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    raw[j][i].floats(v);
-                    word[i] = mx4_codes(v, scale, inverse);
-                }
-                st_shared_v4(cell[j], word[0], word[1], word[2], word[3]);
-                st_shared_b8(scale_at[j], scale);
             }
         }
         fence_proxy_async_smem();
         __syncwarp();
-        const uint32_t through = base + kThreads * kTogether;
-        const uint32_t whole = through < all ? through / items : slots;
-        for (; told < whole; ++told) {
-            if ((t & 31u) == 0u) {
+        for (; told < slot && told < slots; ++told) {
+            if (lane == 0u) {
                 mbar_arrive(bars + told * 8u);
             }
         }
     }
     fence_proxy_async_smem();
     __syncwarp();
-    for (; told < slots; ++told) {         // (no live row: zeros all over)
-        if ((t & 31u) == 0u) {
+    for (; told < slots; ++told) {
+        if (lane == 0u) {
             mbar_arrive(bars + told * 8u);
         }
     }
@@ -353,13 +353,22 @@ __device__ __forceinline__ void mx_store(const MxArgs &args, uint32_t stage, uin
     };
     __syncwarp();                  // the rows before these are out of it
     if (GATED) {
+        // (exchanges, then arithmetic, then stores: each of the three keeps its place in the program, and a value at a time
+        // they wait for each other, 600 cycles for the 16 rows instead of 250)
         const bool odd = (lane & 1u) != 0u;
+        float got[8], value[8];
 #pragma unroll
-        for (uint32_t i = 0; i < 16u; i += 2u) {
-            const float give = __uint_as_float(odd ? v[i] : v[i + 1u]);
-            const float keep = __uint_as_float(odd ? v[i + 1u] : v[i]);
-            const float got = __shfl_xor_sync(0xFFFFFFFFu, give, 1u);
-            put(i + (odd ? 1u : 0u), lane / 2u, gated_unit(odd ? got : keep, odd ? keep : got));
+        for (uint32_t i = 0; i < 8u; ++i) {
+            got[i] = __shfl_xor_sync(0xFFFFFFFFu, __uint_as_float(odd ? v[2u * i] : v[2u * i + 1u]), 1u);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; ++i) {
+            const float keep = __uint_as_float(odd ? v[2u * i + 1u] : v[2u * i]);
+            value[i] = gated_unit(odd ? got[i] : keep, odd ? keep : got[i]);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; ++i) {
+            put(2u * i + (odd ? 1u : 0u), lane / 2u, value[i]);
         }
     } else {
 #pragma unroll
@@ -370,23 +379,36 @@ __device__ __forceinline__ void mx_store(const MxArgs &args, uint32_t stage, uin
     __syncwarp();
     const bool adds = !GATED && sizeof(YT) == 4 && args.epilogue == kEpilogueAdd;
     if (args.wide != 0u) {
+        constexpr uint32_t kSteps = 16u / kRowsPerStep;
         const uint32_t part = lane % kLanesPerRow;
+        uint4 piece[kSteps];
+        YT *at[kSteps];
 #pragma unroll
-        for (uint32_t step = 0; step < 16u / kRowsPerStep; ++step) {
+        for (uint32_t step = 0; step < kSteps; ++step) {
             const uint32_t local = step * kRowsPerStep + lane / kLanesPerRow;
             const uint32_t row = __shfl_sync(0xFFFFFFFFu, row_y, local);
-            uint32_t a, b, c, d;
-            ld_shared_v4(stage + local * kRowBytes + part * 16u, a, b, c, d);
-            if (row != 0xFFFFFFFFu && part * kPiece < columns) {
-                YT *at = static_cast<YT *>(args.y) + (size_t)row * args.ldy + first_col + part * kPiece;
-                if (adds) {
-                    const float4 before = *reinterpret_cast<const float4 *>(at);
-                    a = __float_as_uint(before.x + __uint_as_float(a));
-                    b = __float_as_uint(before.y + __uint_as_float(b));
-                    c = __float_as_uint(before.z + __uint_as_float(c));
-                    d = __float_as_uint(before.w + __uint_as_float(d));
-                }
-                *reinterpret_cast<uint4 *>(at) = make_uint4(a, b, c, d);
+            ld_shared_v4(stage + local * kRowBytes + part * 16u, piece[step].x, piece[step].y, piece[step].z, piece[step].w);
+            at[step] = row != 0xFFFFFFFFu && part * kPiece < columns
+                ? static_cast<YT *>(args.y) + (size_t)row * args.ldy + first_col + part * kPiece : nullptr;
+        }
+        if (adds) {
+            float4 before[kSteps];
+#pragma unroll
+            for (uint32_t step = 0; step < kSteps; ++step) {
+                before[step] = at[step] != nullptr ? *reinterpret_cast<const float4 *>(at[step]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+#pragma unroll
+            for (uint32_t step = 0; step < kSteps; ++step) {
+                piece[step].x = __float_as_uint(before[step].x + __uint_as_float(piece[step].x));
+                piece[step].y = __float_as_uint(before[step].y + __uint_as_float(piece[step].y));
+                piece[step].z = __float_as_uint(before[step].z + __uint_as_float(piece[step].z));
+                piece[step].w = __float_as_uint(before[step].w + __uint_as_float(piece[step].w));
+            }
+        }
+#pragma unroll
+        for (uint32_t step = 0; step < kSteps; ++step) {
+            if (at[step] != nullptr) {
+                *reinterpret_cast<uint4 *>(at[step]) = piece[step];
             }
         }
     } else {
@@ -436,6 +458,15 @@ __device__ __forceinline__ void mx_add_partials(uint32_t (&v)[16], const float *
     }
 }
 
+// Columns of a tile of `rows` rows of x that block `rank` of a cluster adds up (columns change hands by fours).
+__device__ __forceinline__ uint32_t mx_share(const MxArgs &args, uint32_t rank, uint32_t rows)
+{
+    const uint32_t first = rank * args.share;
+    const uint32_t all = (rows + 3u) & ~3u;
+    const uint32_t left = all > first ? all - first : 0u;
+    return left < args.share ? left : args.share;
+}
+
 template <typename YT, bool GATED>
 __global__ void __launch_bounds__(kMxThreads, 1)
 mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
@@ -463,7 +494,11 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     auto empty = [&](uint32_t s) { return bars + (kMxMaxStages + s) * 8u; };
     auto summed = [&](uint32_t b) { return bars + (2u * kMxMaxStages + b) * 8u; };
     auto taken = [&](uint32_t b) { return bars + (2u * kMxMaxStages + 2u + b) * 8u; };
-    const uint32_t x_bars = bars + (2u * kMxMaxStages + 4u) * 8u;
+    const uint32_t exchanged = bars + (2u * kMxMaxStages + 4u) * 8u;
+    const uint32_t x_bars = bars + (2u * kMxMaxStages + 5u) * 8u;
+    // a cluster's exchange: per block of it this block's columns, [block][four columns][row of w][column] floats, at the end of the rings
+    const uint32_t exchange = tail - args.cluster * args.share * kMxRows * 4u;
+    const uint32_t rank = args.cluster != 0u ? blockIdx.x % args.cluster : 0u;
 
     if (warp == kMxMmaWarp) {
         tmem_alloc(smem_u32(&tmem_base), args.tmem_columns);
@@ -482,7 +517,24 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         for (uint32_t s = 0; s < args.slots; ++s) {
             mbar_init(x_bars + s * 8u, kMxStoreWarps);
         }
+        mbar_init(exchanged, 1u);
         mbar_init_fence();
+        if (args.cluster != 0u) {
+            const uint32_t tok_tiles = (args.x_rows + args.ntok - 1u) / args.ntok;
+            const uint32_t skip = blockIdx.x / args.cluster % tok_tiles * args.ntok;
+            const uint32_t rows = args.x_rows - skip < args.ntok ? args.x_rows - skip : args.ntok;
+            mbar_expect_tx(exchanged, mx_share(args, rank, rows) * kMxRows * 4u * args.cluster);
+        }
+    }
+    if (args.cluster != 0u) {
+        // every block of the cluster has started, and its barrier counts, before the exchange
+        __syncwarp();
+        cluster_arrive_release();
+    }
+    if (stays && warp < kMxStoreWarps) {
+        for (uint32_t at = threadIdx.x * 16u; at < args.slots * slot_bytes; at += kMxStoreWarps * 32u * 16u) {
+            st_shared_v4(place + at, 0u, 0u, 0u, 0u);
+        }
     }
     tc_fence_before_sync();
     __syncthreads();
@@ -510,9 +562,15 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const bool early = !waited && args.weights_late == 0u;
     const unsigned long long units = (unsigned long long)tiles * steps;
     MxPieces mine;
-    mine.unit = mx_run_begin(blockIdx.x, gridDim.x, units);
-    mine.end = mx_run_begin(blockIdx.x + 1u, gridDim.x, units);
     mine.steps = steps;
+    if (args.cluster != 0u) {
+        const unsigned long long first = (unsigned long long)(blockIdx.x / args.cluster) * steps;
+        mine.unit = first + mx_run_begin(rank, args.cluster, steps);
+        mine.end = first + mx_run_begin(rank + 1u, args.cluster, steps);
+    } else {
+        mine.unit = mx_run_begin(blockIdx.x, gridDim.x, units);
+        mine.end = mx_run_begin(blockIdx.x + 1u, gridDim.x, units);
+    }
     const unsigned long long run = mine.end - mine.unit;
     const uint32_t first_step = (uint32_t)(mine.unit % steps);
     // (a batch of one tile is multiplied whole, however much of it lives)
@@ -698,6 +756,10 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         const uint32_t quarter = (warp & 3u) * 32u;            // this warp's lanes of tensor memory, rows of w
         const uint32_t c_first = (warp >> 2) * 16u;            // and its columns, rows of x: 16 of every 32
         const uint32_t lane_taddr = tmem + (quarter << 16);
+        if (args.cluster != 0u) {
+            __syncwarp();
+            cluster_wait_acquire();        // the others have started
+        }
         for (MxRing ring; mine.next(); ring.next(args.accumulators)) {
             const MxTile tile = mx_tile(args, groups, mine.tile, tok_tiles, live);
             if (!mbar_wait(summed(ring.at), ring.parity, &abort_flag, args.status)) {
@@ -713,6 +775,60 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     mbar_arrive(giving);
                 }
             };
+            const uint32_t j0 = tile.row0 + quarter;
+            const uint32_t width = args.n > j0 ? (args.n - j0 < 32u ? args.n - j0 : 32u) : 0u;
+            const uint32_t first_col = GATED ? j0 / 2u : j0;
+            const uint32_t columns = GATED ? width / 2u : width;
+            const uint32_t last_row = tile.first + tile.rows < valid || args.offsets != nullptr ? tile.first + tile.rows : valid;
+            if (args.cluster != 0u) {
+                // One piece per block: each column's sums go to the block of the cluster that adds them up.
+                for (uint32_t c0 = c_first; c0 < tile.rows; c0 += 32u) {
+                    uint32_t v[16];
+                    tmem_ld_32x16(sums + c0, v);
+                    tmem_ld_wait();
+                    uint32_t owner = c0 / args.share;
+                    uint32_t column = c0 - owner * args.share;
+#pragma unroll
+                    for (uint32_t i = 0; i < 16u; i += 4u) {
+                        if (c0 + i < tile.rows) {
+                            const uint32_t to = exchange + ((rank * args.share + column) * kMxRows + (quarter + lane) * 4u) * 4u;
+                            store_counted_v4(mapa_shared(to, owner), v[i], v[i + 1u], v[i + 2u], v[i + 3u],
+                                             mapa_shared(exchanged, owner));
+                        }
+                        column += 4u;
+                        if (column == args.share) {
+                            column = 0u;
+                            ++owner;
+                        }
+                    }
+                }
+                const uint32_t here = mx_share(args, rank, tile.rows);
+                if (here == 0u || !mbar_wait_counted(exchanged, 0u, &abort_flag, args.status)) {
+                    break;
+                }
+                for (uint32_t c0 = c_first; c0 < here; c0 += 32u) {
+                    uint32_t v[16] = {};
+                    for (uint32_t r = 0; r < args.cluster; ++r) {
+                        const uint32_t from = exchange + ((r * args.share + c0) * kMxRows + (quarter + lane) * 4u) * 4u;
+#pragma unroll
+                        for (uint32_t i = 0; i < 16u; i += 4u) {
+                            if (c0 + i < here) {
+                                uint32_t part[4];
+                                ld_shared_v4(from + i * kMxRows * 4u, part[0], part[1], part[2], part[3]);
+#pragma unroll
+                                for (uint32_t j = 0; j < 4u; ++j) {
+                                    v[i + j] = r == 0u ? part[j]
+                                                       : __float_as_uint(__uint_as_float(v[i + j]) + __uint_as_float(part[j]));
+                                }
+                            }
+                        }
+                    }
+                    const uint32_t row_x = tile.first + rank * args.share + c0 + lane;
+                    const bool stores = lane < 16u && c0 + lane < here && row_x < last_row;
+                    mx_store<YT, GATED>(args, stage, lane, first_col, columns, stores ? row_x : 0xFFFFFFFFu, v);
+                }
+                break;
+            }
             if (mine.from != 0u) {
                 // Another block owns the tile: its sums go to the scratch.
                 float *out = args.partial + blockIdx.x * args.tile_floats + quarter + lane;
@@ -748,11 +864,6 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 }
                 __syncwarp();
             }
-            const uint32_t j0 = tile.row0 + quarter;
-            const uint32_t width = args.n > j0 ? (args.n - j0 < 32u ? args.n - j0 : 32u) : 0u;
-            const uint32_t first_col = GATED ? j0 / 2u : j0;
-            const uint32_t columns = GATED ? width / 2u : width;
-            const uint32_t last_row = tile.first + tile.rows < valid || args.offsets != nullptr ? tile.first + tile.rows : valid;
             if (c_first >= tile.rows) {
                 release();
             }
@@ -786,6 +897,16 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     grid_launch_dependents();
     tc_fence_before_sync();
     __syncthreads();
+    if (args.cluster != 0u) {
+        // No block leaves while another of the cluster may store into it.
+        __syncwarp();
+        if (warp >= kMxStoreWarps) {
+            cluster_wait_acquire();
+        }
+        __syncwarp();
+        cluster_arrive_relaxed();
+        cluster_wait_acquire();
+    }
     if (warp == kMxMmaWarp) {
         tc_fence_after_sync();
         tmem_dealloc(tmem, args.tmem_columns);
@@ -826,50 +947,112 @@ static uint32_t up_to(uint32_t v, uint32_t multiple)
     return (v + multiple - 1u) / multiple * multiple;
 }
 
-template <typename YT>
-static cudaError_t launch_typed(cudaStream_t stream, dim3 grid, const CUtensorMap &map_w, const CUtensorMap &map_x,
-                                const MxArgs &args, bool overlap)
+template <typename YT, bool GATED>
+static cudaError_t launch_one(cudaStream_t stream, uint32_t grid, const CUtensorMap &map_w, const CUtensorMap &map_x,
+                              const MxArgs &args, bool overlap)
 {
-    if (args.epilogue == kEpilogueSwiglu) {
-        static unsigned long long configured = 0ull;
-        cudaError_t err = allow_shared_memory(mx4_product_kernel<YT, true>, kMxSmem, &configured);
-        return err != cudaSuccess ? err
-             : launch_kernel_early(overlap, mx4_product_kernel<YT, true>, grid, kMxThreads, kMxSmem, stream, map_w, map_x, args);
-    }
     static unsigned long long configured = 0ull;
-    cudaError_t err = allow_shared_memory(mx4_product_kernel<YT, false>, kMxSmem, &configured);
-    return err != cudaSuccess ? err
-         : launch_kernel_early(overlap, mx4_product_kernel<YT, false>, grid, kMxThreads, kMxSmem, stream, map_w, map_x, args);
+    const cudaError_t err = allow_shared_memory(mx4_product_kernel<YT, GATED>, kMxSmem, &configured);
+    if (err != cudaSuccess) {
+        return err;
+    }
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(grid, 1, 1);
+    config.blockDim = dim3(kMxThreads, 1, 1);
+    config.dynamicSmemBytes = kMxSmem;
+    config.stream = stream;
+    cudaLaunchAttribute attribute[2];
+    unsigned int count = 0;
+    if (overlap) {
+        attribute[count].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attribute[count].val.programmaticStreamSerializationAllowed = 1;
+        ++count;
+    }
+    if (args.cluster > 1u) {
+        attribute[count].id = cudaLaunchAttributeClusterDimension;
+        attribute[count].val.clusterDim.x = args.cluster;
+        attribute[count].val.clusterDim.y = 1;
+        attribute[count].val.clusterDim.z = 1;
+        ++count;
+    }
+    config.attrs = attribute;
+    config.numAttrs = count;
+    return cudaLaunchKernelEx(&config, mx4_product_kernel<YT, GATED>, map_w, map_x, args);
 }
 
-// Rows of x per tile: equal parts of at most 256.  By expert, about what one has.
+template <typename YT>
+static cudaError_t launch_typed(cudaStream_t stream, uint32_t grid, const CUtensorMap &map_w, const CUtensorMap &map_x,
+                                const MxArgs &args, bool overlap)
+{
+    return args.epilogue == kEpilogueSwiglu ? launch_one<YT, true>(stream, grid, map_w, map_x, args, overlap)
+                                            : launch_one<YT, false>(stream, grid, map_w, map_x, args, overlap);
+}
+
+// How the steps of a product of `tiles` tiles, `steps` deep, are dealt to at most `sms` blocks: in clusters that share a tile
+// where there are few tiles (`clustered`: the caller knows how many, and they are one batch of rows of x), else in equal runs.
+struct MxPlan {
+    uint32_t cluster;              // 0: equal runs
+    uint32_t grid;
+    uint32_t run;                  // steps of a block, at most
+};
+
+static MxPlan plan_of(unsigned long long tiles, uint32_t steps, uint32_t sms, bool clustered)
+{
+    MxPlan plan = {};
+    if (clustered) {
+        // the clusters of each size that a GPU of 148 SMs runs at the same time (its groups hold 16 to 20 SMs)
+        static const uint32_t together[kMxMaxCluster + 1u] = {0u, 148u, kMxClusterTiles, 48u, 32u, 24u, 24u, 16u, 16u};
+        for (uint32_t c = kMxMaxCluster; c >= 2u; --c) {
+            if (tiles <= together[c] && c <= steps) {
+                plan.cluster = c;
+                plan.grid = (uint32_t)tiles * c;
+                plan.run = (steps + c - 1u) / c;
+                return plan;
+            }
+        }
+    }
+    const unsigned long long units = tiles * steps;
+    const unsigned long long blocks = (units + kMxFewSteps - 1u) / kMxFewSteps;
+    plan.grid = blocks < sms ? (uint32_t)blocks : sms;
+    plan.run = (uint32_t)((units + plan.grid - 1u) / plan.grid);
+    return plan;
+}
+
+static uint32_t steps_of(uint32_t k)
+{
+    return (k + kMxStageK - 1u) / kMxStageK;
+}
+
+static uint32_t row_tiles_of(uint32_t n)
+{
+    return (n + kMxRows - 1u) / kMxRows;
+}
+
+// Rows of x per tile: equal parts of at most 256, or of 128 where the tiles are few enough for clusters (whose exchange
+// takes the shared memory of wider ones).  By expert, about what one has.
 static uint32_t token_tile(const Mx4Product &p)
 {
     const uint32_t typical = p.offsets != nullptr ? (p.m + p.experts - 1u) / p.experts : p.m;
-    const uint32_t parts = (typical + kMxMaxTok - 1u) / kMxMaxTok;
+    uint32_t parts = (typical + kMxMaxTok - 1u) / kMxMaxTok;
+    if (p.offsets == nullptr) {
+        const uint32_t halves = (p.m + kMxClusterTok - 1u) / kMxClusterTok;
+        if (halves * (unsigned long long)row_tiles_of(p.n) <= kMxClusterTiles) {
+            parts = halves;
+        }
+    }
     return up_to((typical + parts - 1u) / parts, 16u);
 }
 
-// Blocks of the grid: never more than steps, of which a block has a few at least.
-static uint32_t grid_of(unsigned long long units, uint32_t sm_count)
-{
-    const unsigned long long blocks = (units + kMxFewSteps - 1u) / kMxFewSteps;
-    return blocks < sm_count ? (uint32_t)blocks : sm_count;
-}
-
 // Stages of x that a block of mx4_linear keeps, 0 if that many rows are quantised by a launch of their own.
-static uint32_t linear_slots(uint32_t n, uint32_t k, uint32_t m, uint32_t sm_count)
+static uint32_t linear_slots(uint32_t n, uint32_t k, uint32_t m, uint32_t sms)
 {
     if (m > kMxFusedRows) {
         return 0u;
     }
-    const uint32_t ntok = up_to(m, 16u);
-    const uint32_t steps = (k + kMxStageK - 1u) / kMxStageK;
-    const unsigned long long units = (unsigned long long)((n + kMxRows - 1u) / kMxRows) * steps;
-    const uint32_t grid = grid_of(units, sm_count);
-    const unsigned long long run = (units + grid - 1u) / grid;
-    const uint32_t slots = run < steps ? (uint32_t)run : steps;
-    const uint32_t bytes = ntok * kMxStageBytes + 2u * kMxScaleBlock;
+    const uint32_t steps = steps_of(k);
+    const uint32_t run = plan_of(row_tiles_of(n), steps, sms, true).run;
+    const uint32_t slots = run < steps ? run : steps;
+    const uint32_t bytes = up_to(m, 16u) * kMxStageBytes + 2u * kMxScaleBlock;
     return slots <= kMxMaxSlots && slots * bytes <= kMxRings / 2u ? slots : 0u;
 }
 
@@ -920,7 +1103,16 @@ cudaError_t launch_mx4_product(cudaStream_t stream, const UmmaScratch &scratch, 
     const uint32_t x_blocks = mx_scale_blocks(args.ntok);
     const uint32_t x_bytes = args.ntok * kMxStageBytes + 2u * x_blocks * kMxScaleBlock;
     args.stage_bytes = kMxRows * kMxStageBytes + 2u * kMxScaleBlock + (args.slots != 0u ? 0u : x_bytes);
-    const uint32_t fit = (kMxRings - args.slots * x_bytes) / args.stage_bytes;
+    // Tiles at most (by expert and live batch the device knows how many).
+    const unsigned long long tok_tiles = p.offsets != nullptr ? p.m / args.ntok + (p.experts < p.m ? p.experts : p.m)
+                                                              : (p.m + args.ntok - 1u) / args.ntok;
+    const MxPlan plan = plan_of(tok_tiles * row_tiles_of(p.n), steps_of(p.k), blocks,
+                                p.offsets == nullptr && (p.m_dev == nullptr || tok_tiles == 1u) && args.ntok <= kMxClusterTok);
+    args.cluster = plan.cluster;
+    const uint32_t tile_rows = p.m < args.ntok ? p.m : args.ntok;
+    args.share = plan.cluster != 0u ? up_to((tile_rows + plan.cluster - 1u) / plan.cluster, 4u) : 0u;
+    const uint32_t exchange = args.cluster * args.share * kMxRows * 4u;
+    const uint32_t fit = (kMxRings - exchange - args.slots * x_bytes) / args.stage_bytes;
     args.stages = fit < kMxMaxStages ? fit : kMxMaxStages;
     // Tensor memory: two accumulators where they fit beside the scales of the stages.
     const uint32_t scale_columns = args.stages * 8u * (1u + x_blocks);
@@ -935,18 +1127,13 @@ cudaError_t launch_mx4_product(cudaStream_t stream, const UmmaScratch &scratch, 
         || (args.slots == 0u && !map_codes(encode, &map_x, p.x_codes, p.m, p.k, args.ntok))) {
         return cudaErrorInvalidValue;
     }
-    // Tiles at most (by expert and live batch the device knows how many).
-    const unsigned long long tok_tiles = p.offsets != nullptr ? p.m / args.ntok + (p.experts < p.m ? p.experts : p.m)
-                                                              : (p.m + args.ntok - 1u) / args.ntok;
-    const unsigned long long units = tok_tiles * ((p.n + kMxRows - 1u) / kMxRows) * ((p.k + kMxStageK - 1u) / kMxStageK);
-    const dim3 grid(grid_of(units, blocks), 1, 1);
     switch (p.y_dtype) {
     case 0:
-        return launch_typed<float>(stream, grid, map_w, map_x, args, p.overlap);
+        return launch_typed<float>(stream, plan.grid, map_w, map_x, args, p.overlap);
     case 1:
-        return launch_typed<__half>(stream, grid, map_w, map_x, args, p.overlap);
+        return launch_typed<__half>(stream, plan.grid, map_w, map_x, args, p.overlap);
     default:
-        return launch_typed<__nv_bfloat16>(stream, grid, map_w, map_x, args, p.overlap);
+        return launch_typed<__nv_bfloat16>(stream, plan.grid, map_w, map_x, args, p.overlap);
     }
 }
 

@@ -50,6 +50,15 @@ __device__ __forceinline__ void st_shared_b8(uint32_t addr, uint32_t value)
     asm volatile("{ .reg .b16 h; cvt.u16.u32 h, %1; st.shared.b8 [%0], h; }" ::"r"(addr), "r"(value) : "memory");
 }
 
+// Four words into the shared memory of a block of the cluster, counted on that block's barrier `bar` (addresses of mapa_shared,
+// 16-byte aligned).
+__device__ __forceinline__ void store_counted_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t bar)
+{
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(addr),
+                 "r"(a), "r"(b), "r"(c), "r"(d), "r"(bar)
+                 : "memory");
+}
+
 __device__ __forceinline__ unsigned short ld_shared_u16(uint32_t addr)
 {
     unsigned short v;

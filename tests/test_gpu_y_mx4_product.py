@@ -41,7 +41,8 @@ def random_codes(rows, k, seed, low, high):
 
 # one block; one tile; tiles cut by every edge; a depth that ends inside a stage, inside a word of scales
 SHAPES = [(128, 64, 16), (16, 32, 1), (1, 32, 3), (130, 96, 5), (127, 256, 17), (300, 416, 33), (129, 1056, 100), (512, 512, 128),
-          (260, 320, 129), (257, 288, 200), (200, 1024, 256), (140, 192, 257), (388, 544, 513), (64, 4096, 2), (2000, 2560, 300), (4100, 1312, 40)]
+          (260, 320, 129), (257, 288, 200), (200, 1024, 256), (140, 192, 257), (388, 544, 513), (64, 4096, 2), (2000, 2560, 300), (4100, 1312, 40), (2050, 1024, 20), (6144, 1024, 100),
+          (4096, 2080, 256), (1030, 8192, 3), (8192, 512, 130), (9000, 608, 16), (40000, 800, 9)]
 
 
 @pytest.mark.parametrize("n,k,m", SHAPES)
