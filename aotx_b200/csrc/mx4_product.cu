@@ -41,6 +41,8 @@ constexpr uint32_t kMxScaleBlock = 512;     // scales of 128 rows and 128 values
 constexpr uint32_t kMxEpilogueStage = 16u * 32u * 4u;  // per storing warp
 constexpr uint32_t kMxFewSteps = 2;         // steps of a block, at least
 constexpr uint32_t kMxMaxCluster = 8;
+constexpr uint32_t kMxPairTok = 224;        // rows of x per tile of a pair of blocks, at most: two accumulators beside the scales
+constexpr uint32_t kMxPairFrom = 129;       // rows of x that pairs take, at least
 constexpr uint32_t kMxClusterTiles = 72;    // tiles of a product that is multiplied by clusters, at most
 constexpr uint32_t kMxClusterTok = 128;     // and rows of x per tile
 constexpr uint32_t kMxFusedRows = 32;       // rows of x that the kernel quantises itself, at most
@@ -67,6 +69,7 @@ struct MxArgs {
     uint32_t ntok;                 // rows of x per tile, a multiple of 16
     uint32_t stages, stage_bytes;
     uint32_t tmem_columns, accumulators;
+    uint32_t scale_places;         // stages whose scales are in tensor memory at a time
     uint32_t weights_late;
     uint32_t wide;                 // rows of y lie on 16-byte boundaries
     // x in 16 or 32 bits, quantised here: its stages stay in `slots` places behind the ring
@@ -88,7 +91,7 @@ __host__ __device__ inline uint32_t mx_scale_blocks(uint32_t ntok)
 }
 
 // kind::mxf4: both operands E2M1 and K-major, scales powers of two; which half of a word of four scales the MMA's 64 values use.
-__host__ __device__ inline uint32_t mx_idesc(uint32_t ntok, uint32_t half)
+__host__ __device__ inline uint32_t mx_idesc(uint32_t rows, uint32_t ntok, uint32_t half)
 {
     uint32_t d = 0;
     d |= (2u * half) << 4;         // B's scales: bytes 0, 1 or 2, 3
@@ -96,7 +99,7 @@ __host__ __device__ inline uint32_t mx_idesc(uint32_t ntok, uint32_t half)
     d |= 1u << 10;                 // B: E2M1
     d |= (ntok >> 3) << 17;
     d |= 1u << 23;                 // scales: powers of two
-    d |= (kMxRows >> 4) << 24;
+    d |= (rows >> 4) << 24;
     d |= (2u * half) << 29;        // A's scales
     return d;
 }
@@ -160,15 +163,15 @@ __device__ __forceinline__ uint32_t mx_groups(const MxArgs &args, MxGroups &grou
     return groups.through[kMx4MaxExperts - 1u];
 }
 
-// A tile: 128 rows of w from w_row (row `row0` of n), and rows of x.
+// A tile: 128 rows of w (256 of a pair of blocks) from w_row (row `row0` of n), and rows of x.
 struct MxTile {
     uint32_t w_row, row0;
     uint32_t first, rows;
 };
 
 // Tile `index`; the tiles of one run of rows of w follow each other, so that the second finds it in L2.
-__device__ __forceinline__ MxTile mx_tile(const MxArgs &args, const MxGroups &groups, uint32_t index, uint32_t tok_tiles,
-                                          uint32_t live)
+__device__ __forceinline__ MxTile mx_tile(const MxArgs &args, const MxGroups &groups, uint32_t tile_rows, uint32_t index,
+                                          uint32_t tok_tiles, uint32_t live)
 {
     MxTile tile;
     uint32_t expert = 0u, first = 0u, rows = live;
@@ -191,7 +194,7 @@ __device__ __forceinline__ MxTile mx_tile(const MxArgs &args, const MxGroups &gr
     }
     const uint32_t row_tile = index / tok_tiles;
     const uint32_t skip = (index - row_tile * tok_tiles) * args.ntok;
-    tile.row0 = row_tile * kMxRows;
+    tile.row0 = row_tile * tile_rows;
     tile.w_row = expert * args.n + tile.row0;
     tile.first = first + skip;
     tile.rows = rows > skip ? (rows - skip < args.ntok ? rows - skip : args.ntok) : 0u;
@@ -467,7 +470,7 @@ __device__ __forceinline__ uint32_t mx_share(const MxArgs &args, uint32_t rank, 
     return left < args.share ? left : args.share;
 }
 
-template <typename YT, bool GATED>
+template <typename YT, bool GATED, bool PAIR>
 __global__ void __launch_bounds__(kMxThreads, 1)
 mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                    const __grid_constant__ MxArgs args)
@@ -481,11 +484,19 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const uint32_t lane = threadIdx.x & 31u;
     const uint32_t stages = args.stages;
     const uint32_t x_blocks = mx_scale_blocks(args.ntok);
-    const bool stays = args.slots != 0u;
+    const bool stays = !PAIR && args.slots != 0u;
+    const bool clusters = !PAIR && args.cluster != 0u;
+    // a pair of blocks is one worker: each has half of the tile's rows of w, its sums, and half of its rows of x
+    constexpr uint32_t kBlocks = PAIR ? 2u : 1u;
+    constexpr uint32_t kTileRows = kBlocks * kMxRows;
+    const uint32_t half = PAIR ? cluster_ctarank() : 0u;
+    const uint32_t worker = PAIR ? blockIdx.x / 2u : blockIdx.x;
+    const uint32_t workers = PAIR ? gridDim.x / 2u : gridDim.x;
+    const uint32_t x_rows = PAIR ? args.ntok / 2u : args.ntok;     // of a tile, in this block's shared memory
     // a stage: codes of w, scales of w, codes of x, scales of x; x that stays has places of its own behind the ring
     const uint32_t w_scales_at = kMxRows * kMxStageBytes;
     const uint32_t x_codes_at = w_scales_at + 2u * kMxScaleBlock;
-    const uint32_t x_scales_at = x_codes_at + args.ntok * kMxStageBytes;
+    const uint32_t x_scales_at = x_codes_at + x_rows * kMxStageBytes;
     const uint32_t place = base + stages * args.stage_bytes;
     const uint32_t slot_bytes = args.ntok * kMxStageBytes + 2u * x_blocks * kMxScaleBlock;
     const uint32_t tail = base + kMxRings;
@@ -497,37 +508,44 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const uint32_t exchanged = bars + (2u * kMxMaxStages + 4u) * 8u;
     const uint32_t x_bars = bars + (2u * kMxMaxStages + 5u) * 8u;
     // a cluster's exchange: per block of it this block's columns, [block][four columns][row of w][column] floats, at the end of the rings
-    const uint32_t exchange = tail - args.cluster * args.share * kMxRows * 4u;
-    const uint32_t rank = args.cluster != 0u ? blockIdx.x % args.cluster : 0u;
+    const uint32_t exchange = tail - (clusters ? args.cluster * args.share * kMxRows * 4u : 0u);
+    const uint32_t rank = clusters ? blockIdx.x % args.cluster : 0u;
 
     if (warp == kMxMmaWarp) {
-        tmem_alloc(smem_u32(&tmem_base), args.tmem_columns);
-        tmem_relinquish();
+        if (PAIR) {
+            pair_tmem_alloc(smem_u32(&tmem_base), args.tmem_columns);
+            pair_tmem_relinquish();
+        } else {
+            tmem_alloc(smem_u32(&tmem_base), args.tmem_columns);
+            tmem_relinquish();
+        }
     }
     if (threadIdx.x == 0u) {
         abort_flag = 0u;
         for (uint32_t s = 0; s < stages; ++s) {
-            mbar_init(full(s), 1u + 128u);
+            // the codes and the scales; of a pair the first block's counts the second block's scales as well, and the second
+            // block's counts its scales alone
+            mbar_init(full(s), PAIR ? (half == 0u ? 2u + 128u : 128u) : 1u + 128u);
             mbar_init(empty(s), 1u);
         }
         for (uint32_t b = 0; b < 2u; ++b) {
             mbar_init(summed(b), 1u);
-            mbar_init(taken(b), kMxStoreWarps);
+            mbar_init(taken(b), PAIR ? 2u * kMxStoreWarps : kMxStoreWarps);
         }
         for (uint32_t s = 0; s < args.slots; ++s) {
             mbar_init(x_bars + s * 8u, kMxStoreWarps);
         }
         mbar_init(exchanged, 1u);
         mbar_init_fence();
-        if (args.cluster != 0u) {
+        if (clusters) {
             const uint32_t tok_tiles = (args.x_rows + args.ntok - 1u) / args.ntok;
             const uint32_t skip = blockIdx.x / args.cluster % tok_tiles * args.ntok;
             const uint32_t rows = args.x_rows - skip < args.ntok ? args.x_rows - skip : args.ntok;
             mbar_expect_tx(exchanged, mx_share(args, rank, rows) * kMxRows * 4u * args.cluster);
         }
     }
-    if (args.cluster != 0u) {
-        // every block of the cluster has started, and its barrier counts, before the exchange
+    if (PAIR || clusters) {
+        // every block of the cluster has started, and its barriers count, before another block reaches into it
         __syncwarp();
         cluster_arrive_release();
     }
@@ -538,12 +556,16 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     }
     tc_fence_before_sync();
     __syncthreads();
+    if (PAIR) {
+        __syncwarp();
+        cluster_wait_acquire();
+    }
     tc_fence_after_sync();
     const uint32_t tmem = tmem_base;
 
     // which tiles there are
     const uint32_t steps = (args.k + kMxStageK - 1u) / kMxStageK;
-    const uint32_t row_tiles = (args.n + kMxRows - 1u) / kMxRows;
+    const uint32_t row_tiles = (args.n + kTileRows - 1u) / kTileRows;
     uint32_t live = args.x_rows;
     uint32_t tok_tiles = (args.x_rows + args.ntok - 1u) / args.ntok;
     uint32_t tiles = tok_tiles * row_tiles;
@@ -563,13 +585,13 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const unsigned long long units = (unsigned long long)tiles * steps;
     MxPieces mine;
     mine.steps = steps;
-    if (args.cluster != 0u) {
+    if (clusters) {
         const unsigned long long first = (unsigned long long)(blockIdx.x / args.cluster) * steps;
         mine.unit = first + mx_run_begin(rank, args.cluster, steps);
         mine.end = first + mx_run_begin(rank + 1u, args.cluster, steps);
     } else {
-        mine.unit = mx_run_begin(blockIdx.x, gridDim.x, units);
-        mine.end = mx_run_begin(blockIdx.x + 1u, gridDim.x, units);
+        mine.unit = mx_run_begin(worker, workers, units);
+        mine.end = mx_run_begin(worker + 1u, workers, units);
     }
     const unsigned long long run = mine.end - mine.unit;
     const uint32_t first_step = (uint32_t)(mine.unit % steps);
@@ -584,17 +606,28 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 
     if (warp == kMxCopyWarp) {
         if (elect_one()) {
-            const uint32_t bytes = kMxRows * kMxStageBytes + (stays ? 0u : args.ntok * kMxStageBytes);
+            // (a pair's codes all count on the first block's barrier, which that block arms for both)
+            const uint32_t bytes = kMxRows * kMxStageBytes + (stays ? 0u : x_rows * kMxStageBytes);
+            const uint32_t signal = PAIR ? mapa_shared(bars, 0u) : bars;
+            auto copy = [&](uint32_t to, const CUtensorMap *map, uint32_t s, uint32_t step, uint32_t row) {
+                if (PAIR) {
+                    pair_tma_load_2d(to, map, signal + s * 8u, (int)(step * kMxStageBytes), (int)row);
+                } else {
+                    tma_load_2d(to, map, signal + s * 8u, (int)(step * kMxStageBytes), (int)row);
+                }
+            };
             auto copy_w = [&](uint32_t s, uint32_t step, uint32_t w_row) {
-                mbar_expect_tx(full(s), bytes);
-                tma_load_2d(base + s * args.stage_bytes, &map_w, full(s), (int)(step * kMxStageBytes), (int)w_row);
+                if (!PAIR || half == 0u) {
+                    mbar_expect_tx(full(s), PAIR ? 2u * bytes : bytes);
+                }
+                copy(base + s * args.stage_bytes, &map_w, s, step, w_row + half * kMxRows);
             };
             uint32_t begun = 0;
             if (early) {
                 // weights into every stage, then x behind them
                 MxPieces ahead = mine;
                 while (begun < stages && ahead.next()) {
-                    const MxTile tile = mx_tile(args, groups, ahead.tile, tok_tiles, live);
+                    const MxTile tile = mx_tile(args, groups, kTileRows, ahead.tile, tok_tiles, live);
                     for (uint32_t step = ahead.from; step < ahead.to && begun < stages; ++step) {
                         copy_w(begun++, step, tile.w_row);
                     }
@@ -607,7 +640,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             MxRing ring;
             bool ok = true;
             while (ok && mine.next()) {
-                const MxTile tile = mx_tile(args, groups, mine.tile, tok_tiles, live);
+                const MxTile tile = mx_tile(args, groups, kTileRows, mine.tile, tok_tiles, live);
                 for (uint32_t step = mine.from; step < mine.to; ++step, ++it, ring.next(stages)) {
                     if (it >= begun) {
                         if (it >= stages && !mbar_wait_hot(empty(ring.at), ring.parity ^ 1u, &abort_flag, args.status)) {
@@ -617,8 +650,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                         copy_w(ring.at, step, tile.w_row);
                     }
                     if (!stays) {
-                        tma_load_2d(base + ring.at * args.stage_bytes + x_codes_at, &map_x, full(ring.at),
-                                    (int)(step * kMxStageBytes), (int)tile.first);
+                        copy(base + ring.at * args.stage_bytes + x_codes_at, &map_x, ring.at, step, tile.first + half * x_rows);
                     }
                 }
             }
@@ -627,20 +659,60 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             grid_dependency_wait();
             grid_launch_dependents();
             // No copy is on its way when the block ends, whatever became of the MMAs that wait for them too.
-            for (uint32_t last = it > stages ? it - stages : 0u; last < it; ++last) {
+            // (The first block of a pair waits for both; the second stays until the first has seen them.)
+            for (uint32_t last = it > stages ? it - stages : 0u; half == 0u && last < it; ++last) {
                 mbar_wait(full(last % stages), (last / stages) & 1u, &abort_flag, args.status);
+            }
+        }
+    } else if (PAIR && warp == kMxMmaWarp && half != 0u) {
+        // This block's scales are there: told to the first block, whose thread copies them to tensor memory.
+        if (elect_one()) {
+            const uint32_t signal = mapa_shared(bars, 0u);
+            MxRing ring;
+            bool ok = true;
+            while (ok && mine.next()) {
+                for (uint32_t step = mine.from; step < mine.to; ++step, ring.next(stages)) {
+                    if (!mbar_wait_hot(full(ring.at), ring.parity, &abort_flag, args.status)) {
+                        ok = false;
+                        break;
+                    }
+                    fence_proxy_async_smem();
+                    mbar_arrive_cluster_release(signal + ring.at * 8u);
+                }
             }
         }
     } else if (warp == kMxMmaWarp) {
         if (elect_one()) {
-            const uint32_t idesc0 = mx_idesc(args.ntok, 0u);
-            const uint32_t idesc1 = mx_idesc(args.ntok, 1u);
+            const uint32_t idesc0 = mx_idesc(kTileRows, args.ntok, 0u);
+            const uint32_t idesc1 = mx_idesc(kTileRows, args.ntok, 1u);
+            auto copy_scales = [&](uint32_t to, uint64_t from) {
+                if (PAIR) {
+                    pair_tmem_copy_scales(to, from);
+                } else {
+                    tmem_copy_scales(to, from);
+                }
+            };
+            auto multiply = [&](uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t a_scales, uint32_t b_scales,
+                                uint32_t accumulate) {
+                if (PAIR) {
+                    pair_mma_mx4(d, a, b, idesc, a_scales, b_scales, accumulate);
+                } else {
+                    umma_mx4(d, a, b, idesc, a_scales, b_scales, accumulate);
+                }
+            };
+            auto commit = [&](uint32_t bar) {
+                if (PAIR) {
+                    pair_commit(bar);
+                } else {
+                    umma_commit(bar);
+                }
+            };
             const uint32_t columns = 2u * 4u * (1u + x_blocks);   // of scales, per stage
             const uint32_t scales_at = tmem + args.accumulators * args.ntok;
             const uint64_t codes_desc = umma_desc_sw128(0u);
             const uint64_t scale_desc = mx_scale_desc(0u);
             uint32_t it = 0, piece = 0;
-            MxRing ring, slot, sums_ring;
+            MxRing ring, slot, sums_ring, scale_place, behind;
             bool ok = true;
             for (; ok && mine.next(); ++piece, sums_ring.next(args.accumulators)) {
                 const uint32_t sums = tmem + sums_ring.at * args.ntok;
@@ -648,46 +720,59 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     && !mbar_wait(taken(sums_ring.at), sums_ring.parity ^ 1u, &abort_flag, args.status)) {
                     break;
                 }
-                for (uint32_t step = mine.from; step < mine.to; ++step, ++it, ring.next(stages), slot.next(args.slots)) {
+                for (uint32_t step = mine.from; step < mine.to; ++step, ++it, ring.next(stages), slot.next(args.slots),
+                              scale_place.next(args.scale_places)) {
                     if ((stays && it < args.slots && !mbar_wait_hot(x_bars + slot.at * 8u, 0u, &abort_flag, args.status))
                         || !mbar_wait_hot(full(ring.at), ring.parity, &abort_flag, args.status)) {
                         ok = false;
                         break;
                     }
+                    if (PAIR) {
+                        // (the second block's arrival releases at the scope of the cluster)
+                        mbar_test_cluster(full(ring.at), ring.parity);
+                        // the scales that lie where these go have been used
+                        if (it >= args.scale_places) {
+                            if (!mbar_wait_hot(empty(behind.at), behind.parity, &abort_flag, args.status)) {
+                                ok = false;
+                                break;
+                            }
+                            behind.next(stages);
+                        }
+                    }
                     tc_fence_after_sync();
                     fence_proxy_async_smem();        // the scales came by ordinary copies
                     const uint32_t at = base + ring.at * args.stage_bytes;
                     const uint32_t x_at = stays ? place + slot.at * slot_bytes : at + x_codes_at;
-                    const uint32_t w_scales = scales_at + ring.at * columns;
+                    const uint32_t w_scales = scales_at + scale_place.at * columns;
                     const uint32_t x_scales = w_scales + 8u;
                     const uint64_t w_from = scale_desc | ((at + w_scales_at) >> 4);
-                    const uint64_t x_from = scale_desc | ((x_at + args.ntok * kMxStageBytes) >> 4);
-                    tmem_copy_scales(w_scales, w_from);
-                    tmem_copy_scales(w_scales + 4u, w_from + (kMxScaleBlock >> 4));
-                    tmem_copy_scales(x_scales, x_from);
-                    tmem_copy_scales(x_scales + 4u, x_from + (kMxScaleBlock >> 4));
+                    const uint64_t x_from = scale_desc | ((x_at + x_rows * kMxStageBytes) >> 4);
+                    copy_scales(w_scales, w_from);
+                    copy_scales(w_scales + 4u, w_from + (kMxScaleBlock >> 4));
+                    copy_scales(x_scales, x_from);
+                    copy_scales(x_scales + 4u, x_from + (kMxScaleBlock >> 4));
                     if (x_blocks == 2u) {
-                        tmem_copy_scales(x_scales + 8u, x_from + 2u * (kMxScaleBlock >> 4));
-                        tmem_copy_scales(x_scales + 12u, x_from + 3u * (kMxScaleBlock >> 4));
+                        copy_scales(x_scales + 8u, x_from + 2u * (kMxScaleBlock >> 4));
+                        copy_scales(x_scales + 12u, x_from + 3u * (kMxScaleBlock >> 4));
                     }
                     // 64 values are 32 bytes of a row, and half of a word of scales
                     const uint64_t a = codes_desc | (at >> 4);
                     const uint64_t b = codes_desc | (x_at >> 4);
                     const uint32_t x_next = x_scales + 4u * x_blocks;
-                    umma_mx4(sums, a, b, idesc0, w_scales, x_scales, step != mine.from);
+                    multiply(sums, a, b, idesc0, w_scales, x_scales, step != mine.from);
                     const uint32_t left = args.k - step * kMxStageK;
                     if (left > 64u) {
-                        umma_mx4(sums, a + 2u, b + 2u, idesc1, w_scales, x_scales, 1u);
+                        multiply(sums, a + 2u, b + 2u, idesc1, w_scales, x_scales, 1u);
                     }
                     if (left > 128u) {
-                        umma_mx4(sums, a + 4u, b + 4u, idesc0, w_scales + 4u, x_next, 1u);
+                        multiply(sums, a + 4u, b + 4u, idesc0, w_scales + 4u, x_next, 1u);
                     }
                     if (left > 192u) {
-                        umma_mx4(sums, a + 6u, b + 6u, idesc1, w_scales + 4u, x_next, 1u);
+                        multiply(sums, a + 6u, b + 6u, idesc1, w_scales + 4u, x_next, 1u);
                     }
-                    umma_commit(empty(ring.at));
+                    commit(empty(ring.at));
                 }
-                umma_commit(summed(sums_ring.at));
+                commit(summed(sums_ring.at));
             }
         }
     } else if (warp >= kMxScaleWarp && warp < kMxCopyWarp) {
@@ -701,8 +786,8 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         MxRing ring;
         bool ok = true;
         while (ok && mine.next()) {
-            const MxTile tile = mx_tile(args, groups, mine.tile, tok_tiles, live);
-            const uint32_t w_row = tile.w_row + t;
+            const MxTile tile = mx_tile(args, groups, kTileRows, mine.tile, tok_tiles, live);
+            const uint32_t w_row = tile.w_row + half * kMxRows + t;
             const bool w_in = w_row < args.w_rows;
             const bool x_in = t < tile.rows;
             const bool x_in_2 = t + 128u < tile.rows;
@@ -756,12 +841,13 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         const uint32_t quarter = (warp & 3u) * 32u;            // this warp's lanes of tensor memory, rows of w
         const uint32_t c_first = (warp >> 2) * 16u;            // and its columns, rows of x: 16 of every 32
         const uint32_t lane_taddr = tmem + (quarter << 16);
-        if (args.cluster != 0u) {
+        if (clusters) {
             __syncwarp();
             cluster_wait_acquire();        // the others have started
         }
+        const uint32_t signal = PAIR ? mapa_shared(bars, 0u) - bars : 0u;      // from this block's barriers to the first's
         for (MxRing ring; mine.next(); ring.next(args.accumulators)) {
-            const MxTile tile = mx_tile(args, groups, mine.tile, tok_tiles, live);
+            const MxTile tile = mx_tile(args, groups, kTileRows, mine.tile, tok_tiles, live);
             if (!mbar_wait(summed(ring.at), ring.parity, &abort_flag, args.status)) {
                 break;
             }
@@ -772,15 +858,19 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0u) {
-                    mbar_arrive(giving);
+                    if (PAIR) {
+                        mbar_arrive_cluster(giving + signal);
+                    } else {
+                        mbar_arrive(giving);
+                    }
                 }
             };
-            const uint32_t j0 = tile.row0 + quarter;
+            const uint32_t j0 = tile.row0 + half * kMxRows + quarter;
             const uint32_t width = args.n > j0 ? (args.n - j0 < 32u ? args.n - j0 : 32u) : 0u;
             const uint32_t first_col = GATED ? j0 / 2u : j0;
             const uint32_t columns = GATED ? width / 2u : width;
             const uint32_t last_row = tile.first + tile.rows < valid || args.offsets != nullptr ? tile.first + tile.rows : valid;
-            if (args.cluster != 0u) {
+            if (clusters) {
                 // One piece per block: each column's sums go to the block of the cluster that adds them up.
                 for (uint32_t c0 = c_first; c0 < tile.rows; c0 += 32u) {
                     uint32_t v[16];
@@ -852,12 +942,12 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             uint32_t others = 0u;
             if (mine.to < steps) {
                 const unsigned long long tile_end = (unsigned long long)(mine.tile + 1u) * steps;
-                while (mx_run_begin(blockIdx.x + others + 1u, gridDim.x, units) < tile_end) {
+                while (mx_run_begin(worker + others + 1u, workers, units) < tile_end) {
                     ++others;
                 }
                 bool there = true;
                 for (uint32_t o = lane; o < others; o += 32u) {
-                    there = there && mx_wait_flag(args.flags + (blockIdx.x + 1u + o) * kFlagWords + warp, &abort_flag, args.status);
+                    there = there && mx_wait_flag(args.flags + (blockIdx.x + (1u + o) * kBlocks) * kFlagWords + warp, &abort_flag, args.status);
                 }
                 if (!__all_sync(0xFFFFFFFFu, there)) {
                     break;
@@ -882,14 +972,14 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     release();
                 }
                 if (others != 0u) {
-                    mx_add_partials(v, args.partial + (blockIdx.x + 1u) * args.tile_floats + (size_t)c0 * kMxRows + quarter + lane,
-                                    args.tile_floats, others);
+                    mx_add_partials(v, args.partial + (blockIdx.x + kBlocks) * args.tile_floats + (size_t)c0 * kMxRows + quarter + lane,
+                                    kBlocks * args.tile_floats, others);
                 }
                 mx_store<YT, GATED>(args, stage, lane, first_col, columns, row_y, v);
             }
             __syncwarp();
             for (uint32_t o = lane; o < others; o += 32u) {
-                args.flags[(blockIdx.x + 1u + o) * kFlagWords + warp] = 0u;   // for the next launch
+                args.flags[(blockIdx.x + (1u + o) * kBlocks) * kFlagWords + warp] = 0u;   // for the next launch
             }
         }
     }
@@ -897,10 +987,10 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     grid_launch_dependents();
     tc_fence_before_sync();
     __syncthreads();
-    if (args.cluster != 0u) {
-        // No block leaves while another of the cluster may store into it.
+    if (PAIR || clusters) {
+        // No block leaves while another of the cluster may reach into it.
         __syncwarp();
-        if (warp >= kMxStoreWarps) {
+        if (clusters && warp >= kMxStoreWarps) {
             cluster_wait_acquire();
         }
         __syncwarp();
@@ -909,7 +999,11 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     }
     if (warp == kMxMmaWarp) {
         tc_fence_after_sync();
-        tmem_dealloc(tmem, args.tmem_columns);
+        if (PAIR) {
+            pair_tmem_dealloc(tmem, args.tmem_columns);
+        } else {
+            tmem_dealloc(tmem, args.tmem_columns);
+        }
     }
 }
 
@@ -947,12 +1041,12 @@ static uint32_t up_to(uint32_t v, uint32_t multiple)
     return (v + multiple - 1u) / multiple * multiple;
 }
 
-template <typename YT, bool GATED>
+template <typename YT, bool GATED, bool PAIR>
 static cudaError_t launch_one(cudaStream_t stream, uint32_t grid, const CUtensorMap &map_w, const CUtensorMap &map_x,
                               const MxArgs &args, bool overlap)
 {
     static unsigned long long configured = 0ull;
-    const cudaError_t err = allow_shared_memory(mx4_product_kernel<YT, GATED>, kMxSmem, &configured);
+    const cudaError_t err = allow_shared_memory(mx4_product_kernel<YT, GATED, PAIR>, kMxSmem, &configured);
     if (err != cudaSuccess) {
         return err;
     }
@@ -968,24 +1062,28 @@ static cudaError_t launch_one(cudaStream_t stream, uint32_t grid, const CUtensor
         attribute[count].val.programmaticStreamSerializationAllowed = 1;
         ++count;
     }
-    if (args.cluster > 1u) {
+    if (PAIR || args.cluster > 1u) {
         attribute[count].id = cudaLaunchAttributeClusterDimension;
-        attribute[count].val.clusterDim.x = args.cluster;
+        attribute[count].val.clusterDim.x = PAIR ? 2u : args.cluster;
         attribute[count].val.clusterDim.y = 1;
         attribute[count].val.clusterDim.z = 1;
         ++count;
     }
     config.attrs = attribute;
     config.numAttrs = count;
-    return cudaLaunchKernelEx(&config, mx4_product_kernel<YT, GATED>, map_w, map_x, args);
+    return cudaLaunchKernelEx(&config, mx4_product_kernel<YT, GATED, PAIR>, map_w, map_x, args);
 }
 
 template <typename YT>
-static cudaError_t launch_typed(cudaStream_t stream, uint32_t grid, const CUtensorMap &map_w, const CUtensorMap &map_x,
-                                const MxArgs &args, bool overlap)
+static cudaError_t launch_typed(cudaStream_t stream, uint32_t grid, bool pair, const CUtensorMap &map_w,
+                                const CUtensorMap &map_x, const MxArgs &args, bool overlap)
 {
-    return args.epilogue == kEpilogueSwiglu ? launch_one<YT, true>(stream, grid, map_w, map_x, args, overlap)
-                                            : launch_one<YT, false>(stream, grid, map_w, map_x, args, overlap);
+    if (args.epilogue == kEpilogueSwiglu) {
+        return pair ? launch_one<YT, true, true>(stream, grid, map_w, map_x, args, overlap)
+                    : launch_one<YT, true, false>(stream, grid, map_w, map_x, args, overlap);
+    }
+    return pair ? launch_one<YT, false, true>(stream, grid, map_w, map_x, args, overlap)
+                : launch_one<YT, false, false>(stream, grid, map_w, map_x, args, overlap);
 }
 
 // How the steps of a product of `tiles` tiles, `steps` deep, are dealt to at most `sms` blocks: in clusters that share a tile
@@ -1043,6 +1141,25 @@ static uint32_t token_tile(const Mx4Product &p)
     return up_to((typical + parts - 1u) / parts, 16u);
 }
 
+// Pairs of blocks: 256 rows of w by up to 224 of x.
+static uint32_t pair_token_tile(const Mx4Product &p)
+{
+    const uint32_t typical = p.offsets != nullptr ? (p.m + p.experts - 1u) / p.experts : p.m;
+    const uint32_t parts = (typical + kMxPairTok - 1u) / kMxPairTok;
+    return up_to((typical + parts - 1u) / parts, 32u);
+}
+
+static bool pair_takes(const Mx4Product &p, uint32_t sms)
+{
+    if (p.x != nullptr) {
+        return false;
+    }
+    const uint32_t typical = p.offsets != nullptr ? (p.m + p.experts - 1u) / p.experts : p.m;
+    const unsigned long long tiles = (unsigned long long)((typical + kMxPairTok - 1u) / kMxPairTok)
+                                   * ((p.n + 2u * kMxRows - 1u) / (2u * kMxRows)) * p.experts;
+    return typical >= kMxPairFrom && tiles >= sms / 2u;
+}
+
 // Stages of x that a block of mx4_linear keeps, 0 if that many rows are quantised by a launch of their own.
 static uint32_t linear_slots(uint32_t n, uint32_t k, uint32_t m, uint32_t sms)
 {
@@ -1091,8 +1208,9 @@ cudaError_t launch_mx4_product(cudaStream_t stream, const UmmaScratch &scratch, 
     args.tile_floats = scratch.tile_floats;
     const uint32_t size = p.y_dtype == 0 ? 4u : 2u;
     args.wide = (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0u && (args.ldy * size) % 16u == 0u;
-    args.ntok = token_tile(p);
     const uint32_t blocks = sm_count < scratch.blocks ? sm_count : scratch.blocks;
+    const bool pair = pair_takes(p, blocks);
+    args.ntok = pair ? pair_token_tile(p) : token_tile(p);
     if (p.x != nullptr) {
         args.x = p.x;
         args.x_type = (uint32_t)p.x_dtype;
@@ -1101,39 +1219,51 @@ cudaError_t launch_mx4_product(cudaStream_t stream, const UmmaScratch &scratch, 
         args.slots = linear_slots(p.n, p.k, p.m, blocks);
     }
     const uint32_t x_blocks = mx_scale_blocks(args.ntok);
-    const uint32_t x_bytes = args.ntok * kMxStageBytes + 2u * x_blocks * kMxScaleBlock;
+    const uint32_t x_rows = pair ? args.ntok / 2u : args.ntok;
+    const uint32_t x_bytes = x_rows * kMxStageBytes + 2u * x_blocks * kMxScaleBlock;
     args.stage_bytes = kMxRows * kMxStageBytes + 2u * kMxScaleBlock + (args.slots != 0u ? 0u : x_bytes);
     // Tiles at most (by expert and live batch the device knows how many).
     const unsigned long long tok_tiles = p.offsets != nullptr ? p.m / args.ntok + (p.experts < p.m ? p.experts : p.m)
                                                               : (p.m + args.ntok - 1u) / args.ntok;
-    const MxPlan plan = plan_of(tok_tiles * row_tiles_of(p.n), steps_of(p.k), blocks,
-                                p.offsets == nullptr && (p.m_dev == nullptr || tok_tiles == 1u) && args.ntok <= kMxClusterTok);
+    MxPlan plan;
+    if (pair) {
+        const unsigned long long tiles = tok_tiles * ((p.n + 2u * kMxRows - 1u) / (2u * kMxRows));
+        plan = plan_of(tiles, steps_of(p.k), blocks / 2u, false);
+        plan.grid *= 2u;
+    } else {
+        plan = plan_of(tok_tiles * row_tiles_of(p.n), steps_of(p.k), blocks,
+                       p.offsets == nullptr && (p.m_dev == nullptr || tok_tiles == 1u) && args.ntok <= kMxClusterTok);
+    }
     args.cluster = plan.cluster;
     const uint32_t tile_rows = p.m < args.ntok ? p.m : args.ntok;
     args.share = plan.cluster != 0u ? up_to((tile_rows + plan.cluster - 1u) / plan.cluster, 4u) : 0u;
     const uint32_t exchange = args.cluster * args.share * kMxRows * 4u;
     const uint32_t fit = (kMxRings - exchange - args.slots * x_bytes) / args.stage_bytes;
     args.stages = fit < kMxMaxStages ? fit : kMxMaxStages;
-    // Tensor memory: two accumulators where they fit beside the scales of the stages.
-    const uint32_t scale_columns = args.stages * 8u * (1u + x_blocks);
-    args.accumulators = 2u * args.ntok + scale_columns <= 512u ? 2u : 1u;
-    const uint32_t columns = args.accumulators * args.ntok + scale_columns;
+    // Tensor memory: two accumulators where they fit beside scales, and those of as many stages as then fit, two at least (a
+    // single block copies a stage's scales without asking for the place: it has one for each).
+    const uint32_t stage_columns = 8u * (1u + x_blocks);
+    const uint32_t least = pair ? 2u * stage_columns : args.stages * stage_columns;
+    args.accumulators = 2u * args.ntok + least <= 512u ? 2u : 1u;
+    const uint32_t places = (512u - args.accumulators * args.ntok) / stage_columns;
+    args.scale_places = places < args.stages ? places : args.stages;
+    const uint32_t columns = args.accumulators * args.ntok + args.scale_places * stage_columns;
     args.tmem_columns = 32u;
     while (args.tmem_columns < columns) {
         args.tmem_columns *= 2u;
     }
     CUtensorMap map_w, map_x = {};
     if (!map_codes(encode, &map_w, p.w_codes, args.w_rows, p.k, kMxRows)
-        || (args.slots == 0u && !map_codes(encode, &map_x, p.x_codes, p.m, p.k, args.ntok))) {
+        || (args.slots == 0u && !map_codes(encode, &map_x, p.x_codes, p.m, p.k, x_rows))) {
         return cudaErrorInvalidValue;
     }
     switch (p.y_dtype) {
     case 0:
-        return launch_typed<float>(stream, plan.grid, map_w, map_x, args, p.overlap);
+        return launch_typed<float>(stream, plan.grid, pair, map_w, map_x, args, p.overlap);
     case 1:
-        return launch_typed<__half>(stream, plan.grid, map_w, map_x, args, p.overlap);
+        return launch_typed<__half>(stream, plan.grid, pair, map_w, map_x, args, p.overlap);
     default:
-        return launch_typed<__nv_bfloat16>(stream, plan.grid, map_w, map_x, args, p.overlap);
+        return launch_typed<__nv_bfloat16>(stream, plan.grid, pair, map_w, map_x, args, p.overlap);
     }
 }
 

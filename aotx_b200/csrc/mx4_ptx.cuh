@@ -86,4 +86,30 @@ __device__ __forceinline__ void umma_mx4(uint32_t d_tmem, uint64_t a_desc, uint6
         : "memory");
 }
 
+// The same two for a pair of blocks (cta_group::2): scales from either block's shared memory into its own tensor memory, the same
+// offsets in both; D is 256 x N, each block 128 rows of it with their scales, B half of its columns in either block's shared
+// memory and the scales of all of them in both.
+__device__ __forceinline__ void pair_tmem_copy_scales(uint32_t taddr, uint64_t desc)
+{
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+__device__ __forceinline__ void pair_mma_mx4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scales,
+                                             uint32_t b_scales, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate)
+        : "memory");
+}
+
+// Arrive on a barrier of another block of the cluster (an address of mapa_shared); what this thread has seen is there for who
+// acquires it at the scope of the cluster.
+__device__ __forceinline__ void mbar_arrive_cluster_release(uint32_t bar)
+{
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
 } // namespace q8

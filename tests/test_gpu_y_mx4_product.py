@@ -39,13 +39,17 @@ def random_codes(rows, k, seed, low, high):
     return codes, np.ascontiguousarray(flat.reshape(rows, chunks, 4).transpose(1, 0, 2))
 
 
-# one block; one tile; tiles cut by every edge; a depth that ends inside a stage, inside a word of scales
+# one block; one tile; tiles cut by every edge; a depth that ends inside a stage, inside a word of scales; clusters of every size;
+# tiles cut between blocks
 SHAPES = [(128, 64, 16), (16, 32, 1), (1, 32, 3), (130, 96, 5), (127, 256, 17), (300, 416, 33), (129, 1056, 100), (512, 512, 128),
-          (260, 320, 129), (257, 288, 200), (200, 1024, 256), (140, 192, 257), (388, 544, 513), (64, 4096, 2), (2000, 2560, 300), (4100, 1312, 40), (2050, 1024, 20), (6144, 1024, 100),
-          (4096, 2080, 256), (1030, 8192, 3), (8192, 512, 130), (9000, 608, 16), (40000, 800, 9)]
+          (260, 320, 129), (257, 288, 200), (200, 1024, 256), (140, 192, 257), (388, 544, 513), (64, 4096, 2), (2000, 2560, 300),
+          (4100, 1312, 40), (2050, 1024, 20), (6144, 1024, 100), (4096, 2080, 256), (1030, 8192, 3), (8192, 512, 130),
+          (9000, 608, 16), (40000, 800, 9)]
+# pairs of blocks: whole tiles, cut ones, edges of either operand
+PAIRS = [(18944, 256, 129), (19000, 96, 130), (10001, 544, 300), (9472, 1312, 448), (4800, 800, 1000), (20000, 2080, 160)]
 
 
-@pytest.mark.parametrize("n,k,m", SHAPES)
+@pytest.mark.parametrize("n,k,m", PAIRS + SHAPES)
 def test_exact_sums(ctx, n, k, m):
     """Scales 2^-2 .. 2^2: products are multiples of 2^-6, and where the magnitudes of a sum add up to less than 2^18 floats hold
     every partial sum: the result is the sum itself."""
@@ -60,7 +64,8 @@ def test_exact_sums(ctx, n, k, m):
 
 
 @pytest.mark.parametrize("out", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("n,k,m", [(130, 96, 5), (300, 416, 33), (388, 544, 140), (256, 1024, 300), (1000, 512, 8)])
+@pytest.mark.parametrize("n,k,m", [(130, 96, 5), (300, 416, 33), (388, 544, 140), (256, 1024, 300), (1000, 512, 8),
+                                   (9600, 352, 290)])
 def test_types_and_epilogues(ctx, n, k, m, out):
     torch = torch_mod()
     w, x = random_codes(n, k, n, -9, -3), random_codes(m, k, m, -4, 3)
@@ -80,10 +85,11 @@ def test_types_and_epilogues(ctx, n, k, m, out):
         assert torch.equal(y, before + plain)
 
 
+@pytest.mark.parametrize("n", [200, 9600])
 @pytest.mark.parametrize("m,live", [(1, 0), (1, 1), (40, 17), (40, 99), (300, 0), (300, 5), (300, 256), (300, 290)])
-def test_live_batch(ctx, m, live):
+def test_live_batch(ctx, n, m, live):
     torch = torch_mod()
-    n, k = 200, 320
+    k = 320
     w, x = random_codes(n, k, 1, -2, 2), random_codes(m, k, 2, -2, 2)
     want = _mx4.values(*x) @ _mx4.values(*w).T
     y = torch.full((m, n), GUARD, device="cuda")
@@ -180,6 +186,15 @@ def test_order(ctx, tokens, used, experts):
                                     [300, 20, 257, 31]])
 @pytest.mark.parametrize("n,k", [(96, 160), (260, 512)])
 def test_grouped(ctx, counts, n, k):
+    grouped(ctx, counts, n, k)
+
+
+@pytest.mark.parametrize("counts", [[150] * 8, [0, 700, 1, 33, 0, 400, 65, 1]])
+def test_grouped_by_pairs_of_blocks(ctx, counts):
+    grouped(ctx, counts, 2404, 352)
+
+
+def grouped(ctx, counts, n, k):
     """Every expert's rows by its own matrix; rows behind the last expert's stay as they are."""
     torch = torch_mod()
     experts, spare = len(counts), 3
