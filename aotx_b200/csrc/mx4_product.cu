@@ -676,8 +676,10 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                         ok = false;
                         break;
                     }
+                    // (Without release at cluster scope, which takes this thread 1700 cycles: the scales are read from this block's
+                    // own shared memory into its own tensor memory, behind the fence.)
                     fence_proxy_async_smem();
-                    mbar_arrive_cluster_release(signal + ring.at * 8u);
+                    mbar_arrive_cluster(signal + ring.at * 8u);
                 }
             }
         }
@@ -714,34 +716,37 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             uint32_t it = 0, piece = 0;
             MxRing ring, slot, sums_ring, scale_place, behind;
             bool ok = true;
+            bool ready = false, unused = false;
             for (; ok && mine.next(); ++piece, sums_ring.next(args.accumulators)) {
                 const uint32_t sums = tmem + sums_ring.at * args.ntok;
                 if (piece >= args.accumulators
                     && !mbar_wait(taken(sums_ring.at), sums_ring.parity ^ 1u, &abort_flag, args.status)) {
                     break;
                 }
-                for (uint32_t step = mine.from; step < mine.to; ++step, ++it, ring.next(stages), slot.next(args.slots),
+                for (uint32_t step = mine.from; step < mine.to; ++step, ++it, slot.next(args.slots),
                               scale_place.next(args.scale_places)) {
-                    if ((stays && it < args.slots && !mbar_wait_hot(x_bars + slot.at * 8u, 0u, &abort_flag, args.status))
-                        || !mbar_wait_hot(full(ring.at), ring.parity, &abort_flag, args.status)) {
+                    if (!ready && ((stays && it < args.slots && !mbar_wait_hot(x_bars + slot.at * 8u, 0u, &abort_flag, args.status))
+                                   || !mbar_wait_hot(full(ring.at), ring.parity, &abort_flag, args.status))) {
                         ok = false;
                         break;
                     }
-                    if (PAIR) {
-                        // (the second block's arrival releases at the scope of the cluster)
-                        mbar_test_cluster(full(ring.at), ring.parity);
+                    if (PAIR && it >= args.scale_places) {
                         // the scales that lie where these go have been used
-                        if (it >= args.scale_places) {
-                            if (!mbar_wait_hot(empty(behind.at), behind.parity, &abort_flag, args.status)) {
-                                ok = false;
-                                break;
-                            }
-                            behind.next(stages);
+                        if (!unused && !mbar_wait_hot(empty(behind.at), behind.parity, &abort_flag, args.status)) {
+                            ok = false;
+                            break;
                         }
+                        behind.next(stages);
                     }
+                    // The next stage is asked for now: the answer comes while this one's instructions are issued (a wait takes 200
+                    // cycles even where nothing is missing, as much as these).
+                    const uint32_t now = ring.at;
+                    ring.next(stages);
+                    ready = (!stays || it + 1u >= args.slots) && mbar_test(full(ring.at), ring.parity) != 0u;
+                    unused = PAIR && mbar_test(empty(behind.at), behind.parity) != 0u;
                     tc_fence_after_sync();
                     fence_proxy_async_smem();        // the scales came by ordinary copies
-                    const uint32_t at = base + ring.at * args.stage_bytes;
+                    const uint32_t at = base + now * args.stage_bytes;
                     const uint32_t x_at = stays ? place + slot.at * slot_bytes : at + x_codes_at;
                     const uint32_t w_scales = scales_at + scale_place.at * columns;
                     const uint32_t x_scales = w_scales + 8u;
@@ -770,7 +775,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     if (left > 192u) {
                         multiply(sums, a + 6u, b + 6u, idesc1, w_scales + 4u, x_next, 1u);
                     }
-                    commit(empty(ring.at));
+                    commit(empty(now));
                 }
                 commit(summed(sums_ring.at));
             }

@@ -105,11 +105,18 @@ __device__ __forceinline__ void pair_mma_mx4(uint32_t d_tmem, uint64_t a_desc, u
         : "memory");
 }
 
-// Arrive on a barrier of another block of the cluster (an address of mapa_shared); what this thread has seen is there for who
-// acquires it at the scope of the cluster.
-__device__ __forceinline__ void mbar_arrive_cluster_release(uint32_t bar)
+// Has the phase ended?  Does not wait.
+__device__ __forceinline__ uint32_t mbar_test(uint32_t bar, uint32_t parity)
 {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return done;
 }
 
 } // namespace q8
