@@ -33,7 +33,7 @@ constexpr uint32_t kMxCopyWarp = 12;
 constexpr uint32_t kMxMmaWarp = 13;
 constexpr uint32_t kMxRows = 128;           // rows of w per tile
 constexpr uint32_t kMxMaxTok = 256;         // rows of x per tile, at most
-constexpr uint32_t kMxStageK = 256;         // values of a row per stage
+constexpr uint32_t kMxStageK = 256;         // values of a row per part of a stage: 128 bytes, a row of the swizzle
 constexpr uint32_t kMxStageBytes = kMxStageK / 2;
 constexpr uint32_t kMxMaxStages = 12;
 constexpr uint32_t kMxMaxSlots = 64;        // stages of x that stay
@@ -41,9 +41,13 @@ constexpr uint32_t kMxScaleBlock = 512;     // scales of 128 rows and 128 values
 constexpr uint32_t kMxEpilogueStage = 16u * 32u * 4u;  // per storing warp
 constexpr uint32_t kMxFewSteps = 2;         // steps of a block, at least
 constexpr uint32_t kMxMaxCluster = 8;
-constexpr uint32_t kMxPairTok = 224;        // rows of x per tile of a pair of blocks, at most: two accumulators beside the scales
-constexpr uint32_t kMxPairFrom = 129;       // rows of x that pairs take, at least
-constexpr uint32_t kMxClusterTiles = 72;    // tiles of a product that is multiplied by clusters, at most
+constexpr uint32_t kMxPairTok = 192;        // rows of x per tile of a pair of blocks, at most: two accumulators beside the scales
+constexpr uint32_t kMxPairFrom = 257;       // rows of x that pairs take, at least
+// Tiles of a product that is multiplied by clusters, at most: as many clusters of each size as the GPU runs at the same time.
+constexpr uint32_t kMxClustersOf8 = 12;
+constexpr uint32_t kMxClustersOf4 = 32;
+constexpr uint32_t kMxClusterTiles = 72;    // of two
+constexpr uint32_t kMxClusterSteps = 4;     // steps of a block of a larger cluster, at least
 constexpr uint32_t kMxClusterTok = 128;     // and rows of x per tile
 constexpr uint32_t kMxFusedRows = 32;       // rows of x that the kernel quantises itself, at most
 constexpr uint32_t kMxBars = 2 * kMxMaxStages + 5 + kMxMaxSlots;
@@ -84,6 +88,14 @@ struct MxArgs {
     unsigned int *flags;
     unsigned long long tile_floats;
 };
+
+// Parts of a stage.  A wait, a commit and what else the thread that issues the MMAs does for a stage take it as long as four MMAs of
+// 208 columns: pairs of blocks have two parts to a stage (28672 x 4096, 2048 rows, 125 -> PAIR_US us).  A single block has one, so
+// that few steps can be dealt evenly.
+__host__ __device__ constexpr uint32_t mx_parts(bool pair)
+{
+    return pair ? 2u : 1u;
+}
 
 __host__ __device__ inline uint32_t mx_scale_blocks(uint32_t ntok)
 {
@@ -169,37 +181,66 @@ struct MxTile {
     uint32_t first, rows;
 };
 
-// Tile `index`; the tiles of one run of rows of w follow each other, so that the second finds it in L2.
-__device__ __forceinline__ MxTile mx_tile(const MxArgs &args, const MxGroups &groups, uint32_t tile_rows, uint32_t index,
-                                          uint32_t tok_tiles, uint32_t live)
-{
-    MxTile tile;
-    uint32_t expert = 0u, first = 0u, rows = live;
-    if (args.offsets != nullptr) {
-        // the expert is the first whose tiles go past the index
-        uint32_t low = 0u, high = args.experts - 1u;
-        while (low < high) {
-            const uint32_t middle = (low + high) / 2u;
-            if (groups.through[middle] > index) {
-                high = middle;
-            } else {
-                low = middle + 1u;
+// Finds the tiles of a run one after the other; the tiles of one run of rows of w follow each other, so that the second finds
+// it in L2.
+struct MxTiles {
+    uint32_t expert = 0, begin = 0, end = 0;     // of tiles of the expert that the last one belonged to
+    uint32_t tok_tiles = 0;
+    uint32_t row_tile = 0, tok_tile = 0;         // the next one
+    bool known = false;
+
+    __device__ __forceinline__ MxTile next(const MxArgs &args, const MxGroups &groups, uint32_t tile_rows, uint32_t index,
+                                           uint32_t all_tok_tiles, uint32_t live)
+    {
+        if (!known) {
+            known = true;
+            uint32_t in = index;
+            tok_tiles = all_tok_tiles;
+            end = 0xFFFFFFFFu;
+            if (args.offsets != nullptr) {
+                // the expert is the first whose tiles go past the index
+                uint32_t low = 0u, high = args.experts - 1u;
+                while (low < high) {
+                    const uint32_t middle = (low + high) / 2u;
+                    if (groups.through[middle] > index) {
+                        high = middle;
+                    } else {
+                        low = middle + 1u;
+                    }
+                }
+                expert = low;
+                begin = expert != 0u ? groups.through[expert - 1u] : 0u;
+                end = groups.through[expert];
+                tok_tiles = (groups.rows[expert] + args.ntok - 1u) / args.ntok;
+                in -= begin;
             }
+            row_tile = in / tok_tiles;
+            tok_tile = in - row_tile * tok_tiles;
+        } else if (index == end) {
+            // the next expert that has tiles
+            do {
+                ++expert;
+                end = groups.through[expert];
+            } while (end == index);
+            tok_tiles = (groups.rows[expert] + args.ntok - 1u) / args.ntok;
+            row_tile = 0u;
+            tok_tile = 0u;
         }
-        expert = low;
-        index -= expert != 0u ? groups.through[expert - 1u] : 0u;
-        first = groups.first[expert];
-        rows = groups.rows[expert];
-        tok_tiles = (rows + args.ntok - 1u) / args.ntok;
+        const uint32_t first = args.offsets != nullptr ? groups.first[expert] : 0u;
+        const uint32_t rows = args.offsets != nullptr ? groups.rows[expert] : live;
+        const uint32_t skip = tok_tile * args.ntok;
+        MxTile tile;
+        tile.row0 = row_tile * tile_rows;
+        tile.w_row = expert * args.n + tile.row0;
+        tile.first = first + skip;
+        tile.rows = rows > skip ? (rows - skip < args.ntok ? rows - skip : args.ntok) : 0u;
+        if (++tok_tile == tok_tiles) {
+            tok_tile = 0u;
+            ++row_tile;
+        }
+        return tile;
     }
-    const uint32_t row_tile = index / tok_tiles;
-    const uint32_t skip = (index - row_tile * tok_tiles) * args.ntok;
-    tile.row0 = row_tile * tile_rows;
-    tile.w_row = expert * args.n + tile.row0;
-    tile.first = first + skip;
-    tile.rows = rows > skip ? (rows - skip < args.ntok ? rows - skip : args.ntok) : 0u;
-    return tile;
-}
+};
 
 // The run of steps of block b: of `units` in all, the first units % blocks blocks take one more.
 __host__ __device__ __forceinline__ unsigned long long mx_run_begin(uint32_t b, uint32_t blocks, unsigned long long units)
@@ -211,20 +252,33 @@ __host__ __device__ __forceinline__ unsigned long long mx_run_begin(uint32_t b, 
 
 // The pieces of a run: a tile and the steps [from, to) of its depth.
 struct MxPieces {
-    unsigned long long unit, end;
+    uint32_t left;                 // steps of the run that no piece has had
     uint32_t steps;
     uint32_t tile, from, to;
+    bool begun;
+
+    __device__ __forceinline__ void set(unsigned long long unit, unsigned long long end, uint32_t depth)
+    {
+        left = (uint32_t)(end - unit);
+        steps = depth;
+        tile = (uint32_t)(unit / depth);
+        from = (uint32_t)(unit - (unsigned long long)tile * depth);
+        to = from;
+        begun = false;
+    }
 
     __device__ __forceinline__ bool next()
     {
-        if (unit >= end) {
+        if (left == 0u) {
             return false;
         }
-        tile = (uint32_t)(unit / steps);
-        from = (uint32_t)(unit - (unsigned long long)tile * steps);
-        const unsigned long long left = end - unit;
-        to = left < steps - from ? from + (uint32_t)left : steps;
-        unit += to - from;
+        if (begun) {
+            ++tile;
+            from = 0u;
+        }
+        begun = true;
+        to = left < steps - from ? from + left : steps;
+        left -= to - from;
         return true;
     }
 };
@@ -334,6 +388,17 @@ __device__ __forceinline__ void mx_quantize_x(const MxArgs &args, const T *x, ui
     }
 }
 
+// silu(gate) * up.  For a float y as the Q8_0 products form it; for 16 bits by the approximate exponential and reciprocal, which are
+// off by 2^-18 of the result at most for gates from -14 on (2^-15 at -100), against 2^-11 and 2^-8 of the rounding: 6 instructions instead of 20, 16 rows 900 -> GATED_CYCLES cycles.
+template <typename YT>
+__device__ __forceinline__ float mx_gated(float gate, float up)
+{
+    if (sizeof(YT) == 4) {
+        return gated_unit(gate, up);
+    }
+    return gate * rcp_approx(1.0f + ex2_approx(gate * -1.4426950408889634f)) * up;
+}
+
 // 16 rows of x (v: this lane's row of w for each) to y, rows `first` and up below `end`; `row_y`: lane i's is the row of y of row i.
 // They are turned round in the warp's own shared memory and written 16 bytes a lane.  GATED: neighbouring lanes hold gate
 // and up of a column (arithmetic of cuda/model/norm.cu:92-105); of two rows of x the even lane forms the first's value and
@@ -367,7 +432,7 @@ __device__ __forceinline__ void mx_store(const MxArgs &args, uint32_t stage, uin
 #pragma unroll
         for (uint32_t i = 0; i < 8u; ++i) {
             const float keep = __uint_as_float(odd ? v[2u * i + 1u] : v[2u * i]);
-            value[i] = gated_unit(odd ? got[i] : keep, odd ? keep : got[i]);
+            value[i] = mx_gated<YT>(odd ? got[i] : keep, odd ? keep : got[i]);
         }
 #pragma unroll
         for (uint32_t i = 0; i < 8u; ++i) {
@@ -488,15 +553,17 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const bool clusters = !PAIR && args.cluster != 0u;
     // a pair of blocks is one worker: each has half of the tile's rows of w, its sums, and half of its rows of x
     constexpr uint32_t kBlocks = PAIR ? 2u : 1u;
+    constexpr uint32_t kParts = mx_parts(PAIR);
+    constexpr uint32_t kStepK = kParts * kMxStageK;
     constexpr uint32_t kTileRows = kBlocks * kMxRows;
     const uint32_t half = PAIR ? cluster_ctarank() : 0u;
     const uint32_t worker = PAIR ? blockIdx.x / 2u : blockIdx.x;
     const uint32_t workers = PAIR ? gridDim.x / 2u : gridDim.x;
     const uint32_t x_rows = PAIR ? args.ntok / 2u : args.ntok;     // of a tile, in this block's shared memory
     // a stage: codes of w, scales of w, codes of x, scales of x; x that stays has places of its own behind the ring
-    const uint32_t w_scales_at = kMxRows * kMxStageBytes;
-    const uint32_t x_codes_at = w_scales_at + 2u * kMxScaleBlock;
-    const uint32_t x_scales_at = x_codes_at + x_rows * kMxStageBytes;
+    const uint32_t w_scales_at = kParts * kMxRows * kMxStageBytes;
+    const uint32_t x_codes_at = w_scales_at + 2u * kParts * kMxScaleBlock;
+    const uint32_t x_scales_at = x_codes_at + kParts * x_rows * kMxStageBytes;
     const uint32_t place = base + stages * args.stage_bytes;
     const uint32_t slot_bytes = args.ntok * kMxStageBytes + 2u * x_blocks * kMxScaleBlock;
     const uint32_t tail = base + kMxRings;
@@ -564,7 +631,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const uint32_t tmem = tmem_base;
 
     // which tiles there are
-    const uint32_t steps = (args.k + kMxStageK - 1u) / kMxStageK;
+    const uint32_t steps = (args.k + kStepK - 1u) / kStepK;
     const uint32_t row_tiles = (args.n + kTileRows - 1u) / kTileRows;
     uint32_t live = args.x_rows;
     uint32_t tok_tiles = (args.x_rows + args.ntok - 1u) / args.ntok;
@@ -584,17 +651,18 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const bool early = !waited && args.weights_late == 0u;
     const unsigned long long units = (unsigned long long)tiles * steps;
     MxPieces mine;
-    mine.steps = steps;
     if (clusters) {
         const unsigned long long first = (unsigned long long)(blockIdx.x / args.cluster) * steps;
-        mine.unit = first + mx_run_begin(rank, args.cluster, steps);
-        mine.end = first + mx_run_begin(rank + 1u, args.cluster, steps);
+        mine.set(first + mx_run_begin(rank, args.cluster, steps), first + mx_run_begin(rank + 1u, args.cluster, steps), steps);
     } else {
-        mine.unit = mx_run_begin(worker, workers, units);
-        mine.end = mx_run_begin(worker + 1u, workers, units);
+        mine.set(mx_run_begin(worker, workers, units), mx_run_begin(worker + 1u, workers, units), steps);
     }
-    const unsigned long long run = mine.end - mine.unit;
-    const uint32_t first_step = (uint32_t)(mine.unit % steps);
+    const uint32_t run = mine.left;
+    const uint32_t first_step = mine.from;
+    MxTiles finder;
+    auto tile_at = [&](MxTiles &tiles_found, uint32_t index) {
+        return tiles_found.next(args, groups, kTileRows, index, tok_tiles, live);
+    };
     // (a batch of one tile is multiplied whole, however much of it lives)
     const auto live_rows = [&]() {
         if (args.m_dev != nullptr && tok_tiles == 1u && !waited) {
@@ -607,27 +675,32 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     if (warp == kMxCopyWarp) {
         if (elect_one()) {
             // (a pair's codes all count on the first block's barrier, which that block arms for both)
-            const uint32_t bytes = kMxRows * kMxStageBytes + (stays ? 0u : x_rows * kMxStageBytes);
+            const uint32_t bytes = kParts * (kMxRows + (stays ? 0u : x_rows)) * kMxStageBytes;
             const uint32_t signal = PAIR ? mapa_shared(bars, 0u) : bars;
-            auto copy = [&](uint32_t to, const CUtensorMap *map, uint32_t s, uint32_t step, uint32_t row) {
-                if (PAIR) {
-                    pair_tma_load_2d(to, map, signal + s * 8u, (int)(step * kMxStageBytes), (int)row);
-                } else {
-                    tma_load_2d(to, map, signal + s * 8u, (int)(step * kMxStageBytes), (int)row);
+            auto copy = [&](uint32_t to, const CUtensorMap *map, uint32_t s, uint32_t step, uint32_t row, uint32_t rows) {
+#pragma unroll
+                for (uint32_t part = 0; part < kParts; ++part) {
+                    const int from = (int)((step * kParts + part) * kMxStageBytes);
+                    if (PAIR) {
+                        pair_tma_load_2d(to + part * rows * kMxStageBytes, map, signal + s * 8u, from, (int)row);
+                    } else {
+                        tma_load_2d(to + part * rows * kMxStageBytes, map, signal + s * 8u, from, (int)row);
+                    }
                 }
             };
             auto copy_w = [&](uint32_t s, uint32_t step, uint32_t w_row) {
                 if (!PAIR || half == 0u) {
                     mbar_expect_tx(full(s), PAIR ? 2u * bytes : bytes);
                 }
-                copy(base + s * args.stage_bytes, &map_w, s, step, w_row + half * kMxRows);
+                copy(base + s * args.stage_bytes, &map_w, s, step, w_row + half * kMxRows, kMxRows);
             };
             uint32_t begun = 0;
             if (early) {
                 // weights into every stage, then x behind them
                 MxPieces ahead = mine;
+                MxTiles found;
                 while (begun < stages && ahead.next()) {
-                    const MxTile tile = mx_tile(args, groups, kTileRows, ahead.tile, tok_tiles, live);
+                    const MxTile tile = tile_at(found, ahead.tile);
                     for (uint32_t step = ahead.from; step < ahead.to && begun < stages; ++step) {
                         copy_w(begun++, step, tile.w_row);
                     }
@@ -640,7 +713,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             MxRing ring;
             bool ok = true;
             while (ok && mine.next()) {
-                const MxTile tile = mx_tile(args, groups, kTileRows, mine.tile, tok_tiles, live);
+                const MxTile tile = tile_at(finder, mine.tile);
                 for (uint32_t step = mine.from; step < mine.to; ++step, ++it, ring.next(stages)) {
                     if (it >= begun) {
                         if (it >= stages && !mbar_wait_hot(empty(ring.at), ring.parity ^ 1u, &abort_flag, args.status)) {
@@ -650,7 +723,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                         copy_w(ring.at, step, tile.w_row);
                     }
                     if (!stays) {
-                        copy(base + ring.at * args.stage_bytes + x_codes_at, &map_x, ring.at, step, tile.first + half * x_rows);
+                        copy(base + ring.at * args.stage_bytes + x_codes_at, &map_x, ring.at, step, tile.first + half * x_rows, x_rows);
                     }
                 }
             }
@@ -709,7 +782,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     umma_commit(bar);
                 }
             };
-            const uint32_t columns = 2u * 4u * (1u + x_blocks);   // of scales, per stage
+            const uint32_t columns = kParts * 8u * (1u + x_blocks);   // of scales, per stage
             const uint32_t scales_at = tmem + args.accumulators * args.ntok;
             const uint64_t codes_desc = umma_desc_sw128(0u);
             const uint64_t scale_desc = mx_scale_desc(0u);
@@ -745,35 +818,36 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     ready = (!stays || it + 1u >= args.slots) && mbar_test(full(ring.at), ring.parity) != 0u;
                     unused = PAIR && mbar_test(empty(behind.at), behind.parity) != 0u;
                     tc_fence_after_sync();
-                    fence_proxy_async_smem();        // the scales came by ordinary copies
+                    fence_proxy_async_smem();            // the scales came by ordinary copies
                     const uint32_t at = base + now * args.stage_bytes;
                     const uint32_t x_at = stays ? place + slot.at * slot_bytes : at + x_codes_at;
                     const uint32_t w_scales = scales_at + scale_place.at * columns;
-                    const uint32_t x_scales = w_scales + 8u;
+                    const uint32_t x_scales = w_scales + kParts * 8u;
                     const uint64_t w_from = scale_desc | ((at + w_scales_at) >> 4);
-                    const uint64_t x_from = scale_desc | ((x_at + x_rows * kMxStageBytes) >> 4);
-                    copy_scales(w_scales, w_from);
-                    copy_scales(w_scales + 4u, w_from + (kMxScaleBlock >> 4));
-                    copy_scales(x_scales, x_from);
-                    copy_scales(x_scales + 4u, x_from + (kMxScaleBlock >> 4));
+                    const uint64_t x_from = scale_desc | ((x_at + kParts * x_rows * kMxStageBytes) >> 4);
+                    // (a block of scales: 128 values of 128 rows)
+#pragma unroll
+                    for (uint32_t c = 0; c < 2u * kParts; ++c) {
+                        copy_scales(w_scales + 4u * c, w_from + c * (kMxScaleBlock >> 4));
+                        copy_scales(x_scales + 4u * c, x_from + c * (kMxScaleBlock >> 4));
+                    }
                     if (x_blocks == 2u) {
-                        copy_scales(x_scales + 8u, x_from + 2u * (kMxScaleBlock >> 4));
-                        copy_scales(x_scales + 12u, x_from + 3u * (kMxScaleBlock >> 4));
+#pragma unroll
+                        for (uint32_t c = 2u * kParts; c < 4u * kParts; ++c) {
+                            copy_scales(x_scales + 4u * c, x_from + c * (kMxScaleBlock >> 4));
+                        }
                     }
                     // 64 values are 32 bytes of a row, and half of a word of scales
-                    const uint64_t a = codes_desc | (at >> 4);
-                    const uint64_t b = codes_desc | (x_at >> 4);
-                    const uint32_t x_next = x_scales + 4u * x_blocks;
-                    multiply(sums, a, b, idesc0, w_scales, x_scales, step != mine.from);
-                    const uint32_t left = args.k - step * kMxStageK;
-                    if (left > 64u) {
-                        multiply(sums, a + 2u, b + 2u, idesc1, w_scales, x_scales, 1u);
-                    }
-                    if (left > 128u) {
-                        multiply(sums, a + 4u, b + 4u, idesc0, w_scales + 4u, x_next, 1u);
-                    }
-                    if (left > 192u) {
-                        multiply(sums, a + 6u, b + 6u, idesc1, w_scales + 4u, x_next, 1u);
+                    const uint32_t left = args.k - step * kStepK;
+#pragma unroll
+                    for (uint32_t p = 0; p < 4u * kParts; ++p) {
+                        if (p == 0u || left > 64u * p) {
+                            const uint32_t part = p / 4u;
+                            multiply(sums, codes_desc | ((at + part * kMxRows * kMxStageBytes) >> 4) + 2u * (p % 4u),
+                                     codes_desc | ((x_at + part * x_rows * kMxStageBytes) >> 4) + 2u * (p % 4u),
+                                     p % 2u == 0u ? idesc0 : idesc1, w_scales + 4u * (p / 2u), x_scales + 4u * x_blocks * (p / 2u),
+                                     p != 0u || step != mine.from);
+                        }
                     }
                     commit(empty(now));
                 }
@@ -787,38 +861,40 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         }
         const uint32_t t = threadIdx.x - kMxScaleWarp * 32u;
         const uint32_t cell = (t % 32u) * 16u + (t / 32u) * 4u;
+        // The copies of as many stages as the ring has are on their way together, and count themselves on the stage's barrier:
+        // the weights' scales come from memory.
         uint32_t it = 0;
         MxRing ring;
         bool ok = true;
         while (ok && mine.next()) {
-            const MxTile tile = mx_tile(args, groups, kTileRows, mine.tile, tok_tiles, live);
+            const MxTile tile = tile_at(finder, mine.tile);
             const uint32_t w_row = tile.w_row + half * kMxRows + t;
             const bool w_in = w_row < args.w_rows;
             const bool x_in = t < tile.rows;
             const bool x_in_2 = t + 128u < tile.rows;
             // (a row outside the tensor is not read, whatever its address)
-            const uint32_t *w_from = args.w_scales + (w_in ? (size_t)(2u * mine.from) * args.w_rows + w_row : 0u);
-            const uint32_t *x_from = stays ? nullptr : args.x_scales + (x_in ? (size_t)(2u * mine.from) * args.x_rows + tile.first + t : 0u);
+            const uint32_t *w_from = args.w_scales + (w_in ? (size_t)(2u * kParts * mine.from) * args.w_rows + w_row : 0u);
+            const uint32_t *x_from = stays ? nullptr
+                : args.x_scales + (x_in ? (size_t)(2u * kParts * mine.from) * args.x_rows + tile.first + t : 0u);
             for (uint32_t step = mine.from; step < mine.to; ++step, ++it, ring.next(stages)) {
                 if (it >= stages && !mbar_wait_hot(empty(ring.at), ring.parity ^ 1u, &abort_flag, args.status)) {
                     ok = false;
                     break;
                 }
                 const uint32_t at = base + ring.at * args.stage_bytes + cell;
-                const bool second = 2u * step + 1u < args.chunks;
-                copy_async_4(at + w_scales_at, w_from, w_in ? 4u : 0u);
-                copy_async_4(at + w_scales_at + kMxScaleBlock, second ? w_from + args.w_rows : w_from, w_in && second ? 4u : 0u);
-                w_from += w_in && second ? 2u * (size_t)args.w_rows : 0u;
-                if (!stays) {
-                    const uint32_t *x_second = x_in && second ? x_from + args.x_rows : x_from;
-                    copy_async_4(at + x_scales_at, x_from, x_in ? 4u : 0u);
-                    copy_async_4(at + x_scales_at + x_blocks * kMxScaleBlock, x_second, x_in && second ? 4u : 0u);
-                    if (x_blocks == 2u) {
-                        copy_async_4(at + x_scales_at + kMxScaleBlock, x_in_2 ? x_from + 128u : x_from, x_in_2 ? 4u : 0u);
-                        copy_async_4(at + x_scales_at + 3u * kMxScaleBlock, x_in_2 && second ? x_second + 128u : x_from,
-                                     x_in_2 && second ? 4u : 0u);
+#pragma unroll
+                for (uint32_t c = 0; c < 2u * kParts; ++c) {
+                    const bool in = 2u * kParts * step + c < args.chunks;
+                    copy_async_4(at + w_scales_at + c * kMxScaleBlock, w_from, w_in && in ? 4u : 0u);
+                    w_from += w_in && in ? args.w_rows : 0u;
+                    if (!stays) {
+                        copy_async_4(at + x_scales_at + c * x_blocks * kMxScaleBlock, x_from, x_in && in ? 4u : 0u);
+                        if (x_blocks == 2u) {
+                            copy_async_4(at + x_scales_at + (2u * c + 1u) * kMxScaleBlock, x_in_2 ? x_from + 128u : x_from,
+                                         x_in_2 && in ? 4u : 0u);
+                        }
+                        x_from += x_in && in ? args.x_rows : 0u;
                     }
-                    x_from += x_in && second ? 2u * (size_t)args.x_rows : 0u;
                 }
                 copy_async_arrive(full(ring.at));
             }
@@ -828,7 +904,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         grid_dependency_wait();       // x, y, the row map and the scratch
         const uint32_t valid = live_rows();
         if (stays) {
-            const uint32_t slots = run < args.slots ? (uint32_t)run : args.slots;
+            const uint32_t slots = run < args.slots ? run : args.slots;
             switch (args.x_type) {
             case 0u:
                 mx_quantize_x(args, static_cast<const float *>(args.x), place, slot_bytes, x_bars, first_step, slots, steps, valid);
@@ -852,7 +928,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         }
         const uint32_t signal = PAIR ? mapa_shared(bars, 0u) - bars : 0u;      // from this block's barriers to the first's
         for (MxRing ring; mine.next(); ring.next(args.accumulators)) {
-            const MxTile tile = mx_tile(args, groups, kTileRows, mine.tile, tok_tiles, live);
+            const MxTile tile = tile_at(finder, mine.tile);
             if (!mbar_wait(summed(ring.at), ring.parity, &abort_flag, args.status)) {
                 break;
             }
@@ -1103,15 +1179,20 @@ static MxPlan plan_of(unsigned long long tiles, uint32_t steps, uint32_t sms, bo
 {
     MxPlan plan = {};
     if (clustered) {
-        // the clusters of each size that a GPU of 148 SMs runs at the same time (its groups hold 16 to 20 SMs)
-        static const uint32_t together[kMxMaxCluster + 1u] = {0u, 148u, kMxClusterTiles, 48u, 32u, 24u, 24u, 16u, 16u};
-        for (uint32_t c = kMxMaxCluster; c >= 2u; --c) {
-            if (tiles <= together[c] && c <= steps) {
+        for (uint32_t c = kMxMaxCluster; c >= 2u; c >>= 1) {
+            if (tiles <= (c == 8u ? kMxClustersOf8 : c == 4u ? kMxClustersOf4 : kMxClusterTiles)
+                && steps >= (c == 2u ? c : c * kMxClusterSteps)) {
                 plan.cluster = c;
                 plan.grid = (uint32_t)tiles * c;
                 plan.run = (steps + c - 1u) / c;
                 return plan;
             }
+        }
+        if (tiles <= sms) {
+            // a tile a block: nothing is cut
+            plan.grid = (uint32_t)tiles;
+            plan.run = steps;
+            return plan;
         }
     }
     const unsigned long long units = tiles * steps;
@@ -1121,9 +1202,9 @@ static MxPlan plan_of(unsigned long long tiles, uint32_t steps, uint32_t sms, bo
     return plan;
 }
 
-static uint32_t steps_of(uint32_t k)
+static uint32_t steps_of(uint32_t k, bool pair = false)
 {
-    return (k + kMxStageK - 1u) / kMxStageK;
+    return (k + mx_parts(pair) * kMxStageK - 1u) / (mx_parts(pair) * kMxStageK);
 }
 
 static uint32_t row_tiles_of(uint32_t n)
@@ -1132,10 +1213,14 @@ static uint32_t row_tiles_of(uint32_t n)
 }
 
 // Rows of x per tile: equal parts of at most 256, or of 128 where the tiles are few enough for clusters (whose exchange
-// takes the shared memory of wider ones).  By expert, about what one has.
+// takes the shared memory of wider ones).  By expert, twice what one has on average, so that most need one tile and their
+// weights are read once.
 static uint32_t token_tile(const Mx4Product &p)
 {
     const uint32_t typical = p.offsets != nullptr ? (p.m + p.experts - 1u) / p.experts : p.m;
+    if (p.offsets != nullptr && typical <= kMxClusterTok / 2u) {
+        return up_to(2u * typical, 32u);
+    }
     uint32_t parts = (typical + kMxMaxTok - 1u) / kMxMaxTok;
     if (p.offsets == nullptr) {
         const uint32_t halves = (p.m + kMxClusterTok - 1u) / kMxClusterTok;
@@ -1146,7 +1231,7 @@ static uint32_t token_tile(const Mx4Product &p)
     return up_to((typical + parts - 1u) / parts, 16u);
 }
 
-// Pairs of blocks: 256 rows of w by up to 224 of x.
+// Pairs of blocks: 256 rows of w by up to 192 of x.
 static uint32_t pair_token_tile(const Mx4Product &p)
 {
     const uint32_t typical = p.offsets != nullptr ? (p.m + p.experts - 1u) / p.experts : p.m;
@@ -1225,15 +1310,15 @@ cudaError_t launch_mx4_product(cudaStream_t stream, const UmmaScratch &scratch, 
     }
     const uint32_t x_blocks = mx_scale_blocks(args.ntok);
     const uint32_t x_rows = pair ? args.ntok / 2u : args.ntok;
-    const uint32_t x_bytes = x_rows * kMxStageBytes + 2u * x_blocks * kMxScaleBlock;
-    args.stage_bytes = kMxRows * kMxStageBytes + 2u * kMxScaleBlock + (args.slots != 0u ? 0u : x_bytes);
+    const uint32_t x_bytes = mx_parts(pair) * (x_rows * kMxStageBytes + 2u * x_blocks * kMxScaleBlock);
+    args.stage_bytes = mx_parts(pair) * (kMxRows * kMxStageBytes + 2u * kMxScaleBlock) + (args.slots != 0u ? 0u : x_bytes);
     // Tiles at most (by expert and live batch the device knows how many).
     const unsigned long long tok_tiles = p.offsets != nullptr ? p.m / args.ntok + (p.experts < p.m ? p.experts : p.m)
                                                               : (p.m + args.ntok - 1u) / args.ntok;
     MxPlan plan;
     if (pair) {
         const unsigned long long tiles = tok_tiles * ((p.n + 2u * kMxRows - 1u) / (2u * kMxRows));
-        plan = plan_of(tiles, steps_of(p.k), blocks / 2u, false);
+        plan = plan_of(tiles, steps_of(p.k, true), blocks / 2u, false);
         plan.grid *= 2u;
     } else {
         plan = plan_of(tok_tiles * row_tiles_of(p.n), steps_of(p.k), blocks,
@@ -1247,7 +1332,7 @@ cudaError_t launch_mx4_product(cudaStream_t stream, const UmmaScratch &scratch, 
     args.stages = fit < kMxMaxStages ? fit : kMxMaxStages;
     // Tensor memory: two accumulators where they fit beside scales, and those of as many stages as then fit, two at least (a
     // single block copies a stage's scales without asking for the place: it has one for each).
-    const uint32_t stage_columns = 8u * (1u + x_blocks);
+    const uint32_t stage_columns = mx_parts(pair) * 8u * (1u + x_blocks);
     const uint32_t least = pair ? 2u * stage_columns : args.stages * stage_columns;
     args.accumulators = 2u * args.ntok + least <= 512u ? 2u : 1u;
     const uint32_t places = (512u - args.accumulators * args.ntok) / stage_columns;

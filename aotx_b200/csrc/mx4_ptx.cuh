@@ -33,6 +33,14 @@ __device__ __forceinline__ void cvt_f16x2_e2m1(uint32_t codes, uint32_t (&out)[4
         : "r"(codes));
 }
 
+// An approximate power of two (within two steps of a float).
+__device__ __forceinline__ float ex2_approx(float v)
+{
+    float r;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
 // A thread's own copy of four bytes, global to shared; zeros where `bytes` is 0 (the source is not read then).
 __device__ __forceinline__ void copy_async_4(uint32_t dst, const void *src, uint32_t bytes)
 {

@@ -54,12 +54,16 @@ def sum_bound(w, x):
     return np.abs(x) @ np.abs(w).T * (w.shape[1] * 2.0 ** -23)
 
 
-def gated_bound(y, error):
-    """The same behind the gated unit: silu has a slope below 1.1 and at most the size of its argument, the unit's own
-    arithmetic loses at most eight float steps (expf, sum, quotient, product: two each)."""
+def gated_bound(y, error, dtype):
+    """The same behind the gated unit: silu has a slope below 1.1 and at most the size of its argument.  For a float result the
+    unit's own arithmetic loses at most eight float steps (expf, sum, quotient, product: two each).  For 16 bits the
+    exponential's argument, gate times a rounded constant, is off by 2^-23 of itself, which makes |gate| 2^-23 of the
+    exponential; that is good to two units (2^-22), the reciprocal to one (2^-23), and there are three roundings more: in
+    halves of a unit, 2^-24, 2 |gate| + 4 + 2 + 3."""
     gate, up = np.abs(y[:, 0::2]), np.abs(y[:, 1::2])
     e_gate, e_up = error[:, 0::2], error[:, 1::2]
-    return 1.1 * e_gate * (up + e_up) + (gate + e_gate) * e_up + 8 * 2.0 ** -24 * gate * up
+    steps = 8 if dtype == "f32" else 9 + 2 * np.minimum(gate, 128)
+    return 1.1 * e_gate * (up + e_up) + (gate + e_gate) * e_up + steps * 2.0 ** -24 * gate * up
 
 
 def close(got, want, error, dtype):
