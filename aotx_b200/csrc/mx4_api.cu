@@ -119,8 +119,7 @@ extern "C" int aotx_mx4_quantize(aotx_q8_ctx *ctx, void *stream, const void *x, 
     ctx->written[1] = static_cast<const unsigned char *>(scales);
     ctx->written_bytes[1] = scale_bytes(rows, k);
     return code_of(ctx, q8::launch_mx4_quantize((cudaStream_t)stream, ctx->overlap != 0, x, x_dtype, x_rows, ldx, k, rows_of,
-                                                rows, rows_dev, static_cast<uint32_t *>(codes),
-                                                static_cast<uint32_t *>(scales)));
+                                                rows, rows_dev, codes, scales));
 }
 
 extern "C" int aotx_mx4_dequant(aotx_q8_ctx *ctx, void *stream, const void *codes, const void *scales, uint32_t total_rows,
@@ -137,9 +136,8 @@ extern "C" int aotx_mx4_dequant(aotx_q8_ctx *ctx, void *stream, const void *code
         return AOTX_Q8_ERR_ARGUMENT;
     }
     const OnDevice on(ctx);
-    return code_of(ctx, q8::launch_mx4_dequant((cudaStream_t)stream, ctx->overlap != 0, static_cast<const uint32_t *>(codes),
-                                               static_cast<const uint8_t *>(scales), total_rows, k, first_row, rows, out,
-                                               out_dtype));
+    return code_of(ctx, q8::launch_mx4_dequant((cudaStream_t)stream, ctx->overlap != 0, codes, scales, total_rows, k, first_row, rows,
+                                               out, out_dtype));
 }
 
 extern "C" int aotx_mx4_matmul(aotx_q8_ctx *ctx, void *stream, const void *w_codes, const void *w_scales, uint32_t n, uint32_t k,

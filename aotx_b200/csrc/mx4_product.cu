@@ -337,6 +337,7 @@ __device__ __forceinline__ void mx_quantize_x(const MxArgs &args, const T *x, ui
 #pragma unroll
         for (uint32_t j = 0; j < kTogether; ++j) {
             cell[j] = 0u;
+            raw[j].zero();
             if (slot < slots) {
                 const uint32_t step = first_step + slot < steps ? first_step + slot : first_step + slot - steps;
                 const uint32_t at = step * kMxStageK + lane * 8u;
@@ -355,15 +356,11 @@ __device__ __forceinline__ void mx_quantize_x(const MxArgs &args, const T *x, ui
         }
 #pragma unroll
         for (uint32_t j = 0; j < kTogether; ++j) {
-            float v[8] = {};
-            if (cell[j] != 0u) {
-                raw[j].floats(v);
-            }
-            uint32_t largest = mx4_largest(v, 0u);
+            uint32_t largest = Eight<T>::largest(raw[j], raw[j]);
             largest = max(largest, __shfl_xor_sync(0xFFFFFFFFu, largest, 1u));
             largest = max(largest, __shfl_xor_sync(0xFFFFFFFFu, largest, 2u));
             const uint32_t scale = mx4_scale(largest);
-            const uint32_t word = mx4_codes(v, scale, mx4_inverse(scale));
+            const uint32_t word = raw[j].codes(scale, mx4_inverse(scale));
             if (cell[j] != 0u) {
                 st_shared_b32(cell[j], word);
                 if ((lane & 3u) == 0u) {

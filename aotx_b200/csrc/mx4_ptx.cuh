@@ -33,6 +33,17 @@ __device__ __forceinline__ void cvt_f16x2_e2m1(uint32_t codes, uint32_t (&out)[4
         : "r"(codes));
 }
 
+// The same for four codes.
+__device__ __forceinline__ void cvt_f16x2_e2m1_4(unsigned short codes, uint32_t &low, uint32_t &high)
+{
+    asm("{\n\t.reg .b8 b0, b1;\n\t"
+        "mov.b16 {b0, b1}, %2;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t}"
+        : "=r"(low), "=r"(high)
+        : "h"(codes));
+}
+
 // An approximate power of two (within two steps of a float).
 __device__ __forceinline__ float ex2_approx(float v)
 {

@@ -13,65 +13,65 @@
 
 namespace q8 {
 
-// A lane takes eight values, so 16 lanes a chunk of 128 with its word of four scales, and a warp the same chunk of two
-// successive rows; a block 16 rows by kQuantChunks chunks, whose loads are issued together.
+// A lane takes half a block, 16 values, so eight lanes a chunk of 128 with its word of four scales, and a warp the same chunk of
+// four successive rows; a block 32 rows by kQuantChunks chunks, whose loads are issued together.  The largest magnitude of
+// 16-bit values is found two at a time, and the products by the scale's reciprocal are formed two at a time too.  Instructions were what bound the
+// first form of these kernels (eight values a lane, one at a time, 13 instructions a value).
 constexpr uint32_t kQuantThreads = 256;
-constexpr uint32_t kQuantRows = kQuantThreads / 16u;
+constexpr uint32_t kQuantRows = kQuantThreads / 8u;
 constexpr uint32_t kQuantChunks = 4;
 
 template <typename T>
 __global__ void __launch_bounds__(kQuantThreads)
 mx4_quantize_kernel(const T *x, uint32_t x_rows, unsigned long long ldx, uint32_t k, const uint32_t *rows_of, uint32_t rows,
-                    const uint32_t *rows_dev, uint32_t *__restrict__ codes, uint32_t *__restrict__ scales, bool aligned)
+                    const uint32_t *rows_dev, uint2 *__restrict__ codes, uint8_t *__restrict__ scales, bool aligned)
 {
+    constexpr uint32_t kTogether = sizeof(T) == 4u ? 2u : kQuantChunks;
     grid_dependency_wait();
     uint32_t live = rows;
     if (rows_dev != nullptr) {
         const uint32_t on_device = *rows_dev;
         live = on_device < rows ? on_device : rows;
     }
-    const uint32_t row = blockIdx.x * kQuantRows + threadIdx.x / 16u;
-    const uint32_t lane = threadIdx.x % 16u;
+    const uint32_t row = blockIdx.x * kQuantRows + threadIdx.x / 8u;
+    const uint32_t lane = threadIdx.x % 8u;
     uint32_t from = row;
     if (row < live && rows_of != nullptr) {
         from = rows_of[row];
     }
     // (all lanes go on: the exchanges below are among whole warps)
     const bool here = row < live && from < x_rows;
-    const uint32_t chunks = mx4_chunks(k);
-    const T *x_row = x + (here ? (unsigned long long)from * ldx : 0ull);
-    for (uint32_t c0 = blockIdx.y * kQuantChunks; c0 < chunks; c0 += gridDim.y * kQuantChunks) {
-        Eight<T> raw[kQuantChunks];
-        bool in[kQuantChunks];
+    const uint32_t chunks = here ? mx4_chunks(k) : 0u;
+    const uint32_t first = blockIdx.y * kQuantChunks;
+    const T *x_at = x + (here ? (unsigned long long)from * ldx : 0ull) + first * 128u + lane * 16u;
+    uint2 *code_at = codes + (unsigned long long)row * (k / 16u) + first * 8u + lane;
+    uint8_t *scale_at = scales + ((unsigned long long)first * rows + row) * 4u + lane / 2u;
 #pragma unroll
-        for (uint32_t i = 0; i < kQuantChunks; ++i) {
-            const uint32_t at = (c0 + i) * 128u + lane * 8u;
-            in[i] = here && at < k;
-            if (in[i]) {
-                raw[i].load(x_row + at, aligned);
+    for (uint32_t c0 = 0; c0 < kQuantChunks; c0 += kTogether) {
+        Eight<T> raw[kTogether][2];
+#pragma unroll
+        for (uint32_t i = 0; i < kTogether; ++i) {
+            raw[i][0].zero();
+            raw[i][1].zero();
+            if (here && (first + c0 + i) * 128u + lane * 16u < k) {
+                raw[i][0].load(x_at + (c0 + i) * 128u, aligned);
+                raw[i][1].load(x_at + (c0 + i) * 128u + 8u, aligned);
             }
         }
 #pragma unroll
-        for (uint32_t i = 0; i < kQuantChunks; ++i) {
-            float v[8] = {};
-            if (in[i]) {
-                raw[i].floats(v);
-            }
-            uint32_t largest = mx4_largest(v, 0u);
+        for (uint32_t i = 0; i < kTogether; ++i) {
+            const uint32_t c = first + c0 + i;
+            uint32_t largest = Eight<T>::largest(raw[i][0], raw[i][1]);
             largest = max(largest, __shfl_xor_sync(0xFFFFFFFFu, largest, 1u));
-            largest = max(largest, __shfl_xor_sync(0xFFFFFFFFu, largest, 2u));
             const uint32_t scale = mx4_scale(largest);
-            const uint32_t word = mx4_codes(v, scale, mx4_inverse(scale));
-            if (in[i]) {
-                codes[(unsigned long long)row * (k / 8u) + (c0 + i) * 16u + lane] = word;
+            const float inverse = mx4_inverse(scale);
+            const uint2 word = make_uint2(raw[i][0].codes(scale, inverse), raw[i][1].codes(scale, inverse));
+            const bool in = c * 128u + lane * 16u < k;
+            if (here && in) {
+                code_at[(c0 + i) * 8u] = word;
             }
-            // the chunk's four scales, from the first lane of each block, to its first lane; 0 past k
-            const uint32_t mine = in[i] ? scale : 0u;
-            const uint32_t s1 = __shfl_down_sync(0xFFFFFFFFu, mine, 4u, 16);
-            const uint32_t s2 = __shfl_down_sync(0xFFFFFFFFu, mine, 8u, 16);
-            const uint32_t s3 = __shfl_down_sync(0xFFFFFFFFu, mine, 12u, 16);
-            if (lane == 0u && in[i]) {
-                scales[(unsigned long long)(c0 + i) * rows + row] = mine | s1 << 8 | s2 << 16 | s3 << 24;
+            if (c < chunks && (lane & 1u) == 0u) {
+                scale_at[(unsigned long long)(c0 + i) * rows * 4u] = (uint8_t)(in ? scale : 0u);   // (0 past k)
             }
         }
     }
@@ -80,86 +80,119 @@ mx4_quantize_kernel(const T *x, uint32_t x_rows, unsigned long long ldx, uint32_
     grid_launch_dependents();
 }
 
-// A lane takes eight codes.
+// Values (pairs of halves) by their scale, as 16 bytes of T.
+__device__ __forceinline__ uint4 mx4_put(const uint32_t (&halves)[4], uint32_t scale, __half)
+{
+    uint32_t word[4];
+    if (scale - 114u <= 25u) {
+        // 2^-13 .. 2^12: the product of two halves is exact
+        const __half2 by = __half2half2(__ushort_as_half((unsigned short)((scale - 112u) << 10)));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const __half2 v = __hmul2(*reinterpret_cast<const __half2 *>(&halves[j]), by);
+            word[j] = *reinterpret_cast<const uint32_t *>(&v);
+        }
+    } else {
+        const float by = mx4_scale_value(scale);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&halves[j]));
+            const __half2 v = __floats2half2_rn(f.x * by, f.y * by);
+            word[j] = *reinterpret_cast<const uint32_t *>(&v);
+        }
+    }
+    return make_uint4(word[0], word[1], word[2], word[3]);
+}
+
+__device__ __forceinline__ uint4 mx4_put(const uint32_t (&halves)[4], uint32_t scale, __nv_bfloat16)
+{
+    uint32_t word[4];
+    const float by = mx4_scale_value(scale);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&halves[j]));
+        word[j] = cvt_bf16x2_rn(f.y * by, f.x * by);
+    }
+    return make_uint4(word[0], word[1], word[2], word[3]);
+}
+
+__device__ __forceinline__ uint4 mx4_put(const uint32_t (&halves)[4], uint32_t scale, float)
+{
+    const float by = mx4_scale_value(scale);
+    const float2 low = __half22float2(*reinterpret_cast<const __half2 *>(&halves[0]));
+    const float2 high = __half22float2(*reinterpret_cast<const __half2 *>(&halves[1]));
+    return make_uint4(__float_as_uint(low.x * by), __float_as_uint(low.y * by), __float_as_uint(high.x * by),
+                      __float_as_uint(high.y * by));
+}
+
+// A lane writes 16 bytes: eight 16-bit values or four floats.  (Twice as much a lane writes half sectors at a time, 28672 x 4096 to
+// binary16 DEQ_HALVES us.)
 template <typename T>
 __global__ void __launch_bounds__(kQuantThreads)
-mx4_dequant_kernel(const uint32_t *codes, const uint8_t *scales, uint32_t total_rows, uint32_t k, uint32_t first_row,
+mx4_dequant_kernel(const uint8_t *codes, const uint8_t *scales, uint32_t total_rows, uint32_t k, uint32_t first_row,
                    uint32_t rows, T *__restrict__ out, bool aligned)
 {
+    constexpr uint32_t kValues = 16u / sizeof(T);
+    constexpr uint32_t kLanes = 128u / kValues;          // a chunk
     grid_dependency_wait();
     grid_launch_dependents();
-    const uint32_t row = blockIdx.x * kQuantRows + threadIdx.x / 16u;
-    const uint32_t lane = threadIdx.x % 16u;
-    const uint32_t chunks = mx4_chunks(k);
+    const uint32_t row = blockIdx.x * (kQuantThreads / kLanes) + threadIdx.x / kLanes;
+    const uint32_t lane = threadIdx.x % kLanes;
     if (row >= rows) {
         return;
     }
+    const uint32_t first = blockIdx.y * kQuantChunks;
     const unsigned long long tensor_row = (unsigned long long)first_row + row;
-    for (uint32_t c0 = blockIdx.y * kQuantChunks; c0 < chunks; c0 += gridDim.y * kQuantChunks) {
-        uint32_t word[kQuantChunks];
-        uint32_t scale[kQuantChunks];
+    const uint8_t *code_at = codes + tensor_row * (k / 2u) + first * 64u + lane * (kValues / 2u);
+    const uint8_t *scale_at = scales + ((unsigned long long)first * total_rows + tensor_row) * 4u + lane * kValues / 32u;
+    T *to = out + (unsigned long long)row * k + first * 128u + lane * kValues;
+    uint32_t word[kQuantChunks];
+    uint32_t scale[kQuantChunks];
 #pragma unroll
-        for (uint32_t i = 0; i < kQuantChunks; ++i) {
-            const uint32_t c = c0 + i;
-            word[i] = 0u;
-            scale[i] = 0u;
-            if (c * 128u + lane * 8u < k) {
-                word[i] = codes[tensor_row * (k / 8u) + c * 16u + lane];
-                scale[i] = scales[((unsigned long long)c * total_rows + tensor_row) * 4u + lane / 4u];
-            }
+    for (uint32_t i = 0; i < kQuantChunks; ++i) {
+        if ((first + i) * 128u + lane * kValues < k) {
+            word[i] = kValues == 8u ? *reinterpret_cast<const uint32_t *>(code_at + i * 64u)
+                                    : (uint32_t)*reinterpret_cast<const uint16_t *>(code_at + i * 64u);
+            scale[i] = scale_at[(unsigned long long)i * total_rows * 4u];
         }
+    }
 #pragma unroll
-        for (uint32_t i = 0; i < kQuantChunks; ++i) {
-            const uint32_t at = (c0 + i) * 128u + lane * 8u;
-            if (at >= k) {
-                continue;
-            }
-            // 2^(scale - 127); the smallest is half of the smallest normal float
-            const float by = __uint_as_float(scale[i] == 255u ? 0x7FC00000u : (scale[i] == 0u ? 0x00400000u : scale[i] << 23));
-            uint32_t halves[4];
+    for (uint32_t i = 0; i < kQuantChunks; ++i) {
+        if ((first + i) * 128u + lane * kValues >= k) {
+            continue;
+        }
+        uint32_t halves[4] = {};
+        if (kValues == 8u) {
             cvt_f16x2_e2m1(word[i], halves);
-            float v[8];
+        } else {
+            cvt_f16x2_e2m1_4((unsigned short)word[i], halves[0], halves[1]);
+        }
+        const uint4 piece = mx4_put(halves, scale[i], T());
+        if (aligned) {
+            *reinterpret_cast<uint4 *>(to + i * 128u) = piece;
+        } else {
+            const T *value = reinterpret_cast<const T *>(&piece);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&halves[j]));
-                v[2 * j] = f.x * by, v[2 * j + 1] = f.y * by;
-            }
-            T *to = out + (unsigned long long)row * k + at;
-            alignas(16) T rounded[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                store_out<T>(rounded, j, v[j]);
-            }
-            if (aligned) {
-#pragma unroll
-                for (uint32_t j = 0; j < sizeof(T) / 2u; ++j) {
-                    reinterpret_cast<uint4 *>(to)[j] = reinterpret_cast<const uint4 *>(rounded)[j];
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    to[j] = rounded[j];
-                }
+            for (uint32_t j = 0; j < kValues; ++j) {
+                to[i * 128u + j] = value[j];
             }
         }
     }
 }
 
-static dim3 quant_grid(uint32_t rows, uint32_t k)
+static dim3 quant_grid(uint32_t rows, uint32_t rows_a_block, uint32_t k)
 {
-    const uint32_t blocks = (rows + kQuantRows - 1u) / kQuantRows;
-    const uint32_t steps = (mx4_chunks(k) + kQuantChunks - 1u) / kQuantChunks;
-    return dim3(blocks, steps < 65535u ? steps : 65535u, 1);
+    return dim3((rows + rows_a_block - 1u) / rows_a_block, (mx4_chunks(k) + kQuantChunks - 1u) / kQuantChunks, 1);
 }
 
 cudaError_t launch_mx4_quantize(cudaStream_t stream, bool overlap, const void *x, int x_dtype, uint32_t x_rows,
                                 unsigned long long ldx, uint32_t k, const uint32_t *rows_of, uint32_t rows,
-                                const uint32_t *rows_dev, uint32_t *codes, uint32_t *scales)
+                                const uint32_t *rows_dev, void *codes, void *scales)
 {
     auto launch = [&](auto kernel, auto *typed) {
         const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15u) == 0u && (ldx * sizeof(*typed)) % 16u == 0u;
-        return launch_kernel_early(overlap, kernel, quant_grid(rows, k), kQuantThreads, 0, stream, typed, x_rows, ldx, k,
-                                   rows_of, rows, rows_dev, codes, scales, aligned);
+        return launch_kernel_early(overlap, kernel, quant_grid(rows, kQuantRows, k), kQuantThreads, 0, stream, typed, x_rows, ldx, k,
+                                   rows_of, rows, rows_dev, static_cast<uint2 *>(codes), static_cast<uint8_t *>(scales), aligned);
     };
     switch (x_dtype) {
     case 0:
@@ -171,13 +204,14 @@ cudaError_t launch_mx4_quantize(cudaStream_t stream, bool overlap, const void *x
     }
 }
 
-cudaError_t launch_mx4_dequant(cudaStream_t stream, bool overlap, const uint32_t *codes, const uint8_t *scales,
+cudaError_t launch_mx4_dequant(cudaStream_t stream, bool overlap, const void *codes, const void *scales,
                                uint32_t total_rows, uint32_t k, uint32_t first_row, uint32_t rows, void *out, int out_dtype)
 {
     const bool aligned = (reinterpret_cast<uintptr_t>(out) & 15u) == 0u;
     auto launch = [&](auto kernel, auto *typed) {
-        return launch_kernel_early(overlap, kernel, quant_grid(rows, k), kQuantThreads, 0, stream, codes, scales, total_rows, k,
-                                   first_row, rows, typed, aligned);
+        const uint32_t rows_a_block = kQuantThreads / (128u / (16u / sizeof(*typed)));
+        return launch_kernel_early(overlap, kernel, quant_grid(rows, rows_a_block, k), kQuantThreads, 0, stream, static_cast<const uint8_t *>(codes),
+                                   static_cast<const uint8_t *>(scales), total_rows, k, first_row, rows, typed, aligned);
     };
     switch (out_dtype) {
     case 0:
