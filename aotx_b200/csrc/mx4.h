@@ -16,9 +16,10 @@ __host__ __device__ inline uint32_t mx4_chunks(uint32_t k)
     return (k + 127u) / 128u;   // words of four scales in a row
 }
 
+// `activations`: no weights are written, so the launch behind this one, which may read its weights early, may start early.
 cudaError_t launch_mx4_quantize(cudaStream_t stream, bool overlap, const void *x, int x_dtype, uint32_t x_rows,
                                 unsigned long long ldx, uint32_t k, const uint32_t *rows_of, uint32_t rows,
-                                const uint32_t *rows_dev, void *codes, void *scales);
+                                const uint32_t *rows_dev, void *codes, void *scales, bool activations);
 cudaError_t launch_mx4_dequant(cudaStream_t stream, bool overlap, const void *codes, const void *scales,
                                uint32_t total_rows, uint32_t k, uint32_t first_row, uint32_t rows, void *out, int out_dtype);
 

@@ -49,7 +49,13 @@ constexpr uint32_t kMxClustersOf4 = 32;
 constexpr uint32_t kMxClusterTiles = 72;    // of two
 constexpr uint32_t kMxClusterSteps = 4;     // steps of a block of a larger cluster, at least
 constexpr uint32_t kMxClusterTok = 128;     // and rows of x per tile
-constexpr uint32_t kMxFusedRows = 32;       // rows of x that the kernel quantises itself, at most
+// Rows of x that the kernel quantises itself: up to 8, or as many as make 128 with the stages of a block.  Every block turns the
+// stages that it needs by itself, so more cost more than a launch of their own does: 28672 x 4096, 8 rows (16 stages), 17.3 us against
+// 19.6, 16 rows 20.7 against 19.9; 4096 x 14336, 8 rows (14 stages) 13.0 against 13.9, 16 rows 16.5 against 14.1; 4096 x 4096,
+// 16 rows (4 stages), 8.1 against 9.5.
+constexpr uint32_t kMxFusedRows = 16;
+constexpr uint32_t kMxFusedAnyway = 8;
+constexpr uint32_t kMxFusedStages = 128;
 constexpr uint32_t kMxBars = 2 * kMxMaxStages + 5 + kMxMaxSlots;
 constexpr uint32_t kMxTail = kMxStoreWarps * kMxEpilogueStage + kMxBars * 8u;
 constexpr uint32_t kMxSmem = 223u * 1024u;
@@ -317,7 +323,7 @@ template <typename T>
 __device__ __forceinline__ void mx_quantize_x(const MxArgs &args, const T *x, uint32_t place, uint32_t slot_bytes,
                                               uint32_t bars, uint32_t first_step, uint32_t slots, uint32_t steps, uint32_t live)
 {
-    constexpr uint32_t kTogether = sizeof(T) == 4u ? 4u : 8u;
+    constexpr uint32_t kTogether = 2u;
     const uint32_t warp = threadIdx.x >> 5;
     const uint32_t lane = threadIdx.x & 31u;
     const uint32_t block = lane / 4u;
@@ -584,29 +590,30 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             tmem_relinquish();
         }
     }
-    if (threadIdx.x == 0u) {
-        abort_flag = 0u;
-        for (uint32_t s = 0; s < stages; ++s) {
+    // A barrier a thread: one after the other they take a microsecond of the smallest launches.
+    if (threadIdx.x < kMxBars) {
+        const uint32_t i = threadIdx.x;
+        uint32_t count = kMxStoreWarps;                          // taken, and the stages of x that stay
+        if (i < kMxMaxStages) {
             // the codes and the scales; of a pair the first block's counts the second block's scales as well, and the second
             // block's counts its scales alone
-            mbar_init(full(s), PAIR ? (half == 0u ? 2u + 128u : 128u) : 1u + 128u);
-            mbar_init(empty(s), 1u);
+            count = PAIR ? (half == 0u ? 2u + 128u : 128u) : 1u + 128u;
+        } else if (i < 2u * kMxMaxStages + 2u || i == 2u * kMxMaxStages + 4u) {
+            count = 1u;                                          // empty, summed, exchanged
+        } else if (PAIR && i < 2u * kMxMaxStages + 4u) {
+            count = 2u * kMxStoreWarps;
         }
-        for (uint32_t b = 0; b < 2u; ++b) {
-            mbar_init(summed(b), 1u);
-            mbar_init(taken(b), PAIR ? 2u * kMxStoreWarps : kMxStoreWarps);
-        }
-        for (uint32_t s = 0; s < args.slots; ++s) {
-            mbar_init(x_bars + s * 8u, kMxStoreWarps);
-        }
-        mbar_init(exchanged, 1u);
+        mbar_init(bars + i * 8u, count);
         mbar_init_fence();
-        if (clusters) {
+        if (clusters && i == 2u * kMxMaxStages + 4u) {
             const uint32_t tok_tiles = (args.x_rows + args.ntok - 1u) / args.ntok;
             const uint32_t skip = blockIdx.x / args.cluster % tok_tiles * args.ntok;
             const uint32_t rows = args.x_rows - skip < args.ntok ? args.x_rows - skip : args.ntok;
             mbar_expect_tx(exchanged, mx_share(args, rank, rows) * kMxRows * 4u * args.cluster);
         }
+    }
+    if (threadIdx.x == 0u) {
+        abort_flag = 0u;
     }
     if (PAIR || clusters) {
         // every block of the cluster has started, and its barriers count, before another block reaches into it
@@ -1257,7 +1264,8 @@ static uint32_t linear_slots(uint32_t n, uint32_t k, uint32_t m, uint32_t sms)
     const uint32_t run = plan_of(row_tiles_of(n), steps, sms, true).run;
     const uint32_t slots = run < steps ? run : steps;
     const uint32_t bytes = up_to(m, 16u) * kMxStageBytes + 2u * kMxScaleBlock;
-    return slots <= kMxMaxSlots && slots * bytes <= kMxRings / 2u ? slots : 0u;
+    return slots <= kMxMaxSlots && slots * bytes <= kMxRings / 2u && (m <= kMxFusedAnyway || m * slots <= kMxFusedStages)
+        ? slots : 0u;
 }
 
 bool mx4_linear_quantizes(uint32_t n, uint32_t k, uint32_t m, unsigned int sm_count)
