@@ -793,11 +793,11 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             uint32_t it = 0, piece = 0;
             MxRing ring, slot, sums_ring, scale_place, behind;
             bool ok = true;
-            bool ready = false, unused = false;
+            bool ready = false, unused = false, empty_sums = false;
             for (; ok && mine.next(); ++piece, sums_ring.next(args.accumulators)) {
                 const uint32_t sums = tmem + sums_ring.at * args.ntok;
-                if (piece >= args.accumulators
-                    && !mbar_wait(taken(sums_ring.at), sums_ring.parity ^ 1u, &abort_flag, args.status)) {
+                if (piece >= args.accumulators && !empty_sums
+                    && !mbar_wait_hot(taken(sums_ring.at), sums_ring.parity ^ 1u, &abort_flag, args.status)) {
                     break;
                 }
                 for (uint32_t step = mine.from; step < mine.to; ++step, ++it, slot.next(args.slots),
@@ -821,6 +821,11 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     ring.next(stages);
                     ready = (!stays || it + 1u >= args.slots) && mbar_test(full(ring.at), ring.parity) != 0u;
                     unused = PAIR && mbar_test(empty(behind.at), behind.parity) != 0u;
+                    if (step + 1u == mine.to) {
+                        MxRing after = sums_ring;
+                        after.next(args.accumulators);
+                        empty_sums = mbar_test(taken(after.at), after.parity ^ 1u) != 0u;
+                    }
                     tc_fence_after_sync();
                     fence_proxy_async_smem();            // the scales came by ordinary copies
                     const uint32_t at = base + now * args.stage_bytes;
@@ -933,7 +938,20 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         const uint32_t signal = PAIR ? mapa_shared(bars, 0u) - bars : 0u;      // from this block's barriers to the first's
         for (MxRing ring; mine.next(); ring.next(args.accumulators)) {
             const MxTile tile = tile_at(finder, mine.tile);
-            if (!mbar_wait(summed(ring.at), ring.parity, &abort_flag, args.status)) {
+            const uint32_t last_row = tile.first + tile.rows < valid || args.offsets != nullptr ? tile.first + tile.rows : valid;
+            // Lane i knows the row of y of row i of 16 of x (fetched before the sums are waited for, and those of the next 16
+            // beside the stores of these).
+            auto row_of = [&](uint32_t c0) {
+                const uint32_t row_x = tile.first + c0 + lane;
+                uint32_t row_y = 0xFFFFFFFFu;
+                if (lane < 16u && row_x < last_row) {
+                    row_y = args.y_rows_of != nullptr ? args.y_rows_of[row_x] : row_x;
+                    row_y = row_y < args.y_rows ? row_y : 0xFFFFFFFFu;
+                }
+                return row_y;
+            };
+            uint32_t next_row = row_of(c_first);
+            if (!mbar_wait_hot(summed(ring.at), ring.parity, &abort_flag, args.status)) {
                 break;
             }
             tc_fence_after_sync();
@@ -954,7 +972,6 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             const uint32_t width = args.n > j0 ? (args.n - j0 < 32u ? args.n - j0 : 32u) : 0u;
             const uint32_t first_col = GATED ? j0 / 2u : j0;
             const uint32_t columns = GATED ? width / 2u : width;
-            const uint32_t last_row = tile.first + tile.rows < valid || args.offsets != nullptr ? tile.first + tile.rows : valid;
             if (clusters) {
                 // One piece per block: each column's sums go to the block of the cluster that adds them up.
                 for (uint32_t c0 = c_first; c0 < tile.rows; c0 += 32u) {
@@ -1043,13 +1060,8 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 release();
             }
             for (uint32_t c0 = c_first; c0 < tile.rows; c0 += 32u) {
-                // lane i knows the row of y of row i of x
-                uint32_t row_y = 0xFFFFFFFFu;
-                const uint32_t row_x = tile.first + c0 + lane;
-                if (lane < 16u && row_x < last_row) {
-                    row_y = args.y_rows_of != nullptr ? args.y_rows_of[row_x] : row_x;
-                    row_y = row_y < args.y_rows ? row_y : 0xFFFFFFFFu;
-                }
+                const uint32_t row_y = next_row;
+                next_row = row_of(c0 + 32u);
                 uint32_t v[16];
                 tmem_ld_32x16(sums + c0, v);
                 tmem_ld_wait();
