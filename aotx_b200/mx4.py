@@ -46,15 +46,19 @@ class Mx4Tensor:
         """Both arrays in one allocation; their tensors are made when they are asked for."""
         if k <= 0 or k % 32 != 0 or rows < 0:
             raise ValueError("k is a multiple of 32")
+        return cls._make(rows, k, device)
+
+    @classmethod
+    def _make(cls, rows, k, device):
         torch = _torch()
         t = cls.__new__(cls)
         t.rows, t.k = rows, k
         # (a row of codes is a multiple of 16 bytes, so the scales behind them lie on such a boundary too)
         codes = rows * (k // 2)
-        t._bytes = torch.empty(codes + (k + 127) // 128 * rows * 4, dtype=torch.uint8, device=device)
-        t.device = t._bytes.device
+        t._bytes = held = torch.empty(codes + (k + 127) // 128 * rows * 4, dtype=torch.uint8, device=device)
+        t.device = held.device
         t._codes = t._scales = None
-        at = t._bytes.data_ptr()
+        at = held.data_ptr()
         t._at = (at, at + codes)
         return t
 
@@ -130,7 +134,7 @@ class Mx4Calls:
             if epilogue == EPILOGUE_ADD:
                 raise ValueError("EPILOGUE_ADD adds into a y that the caller gives")
             torch = _torch()
-            return torch.empty((rows, width), dtype=y_dtype or torch.float32, device=self.device)
+            return torch.empty(rows, width, dtype=y_dtype or torch.float32, device=self.device)
         if tuple(y.shape) != (rows, width) or not y.is_contiguous() or (y_dtype is not None and y.dtype != y_dtype):
             raise ValueError("y is [%d][%d] without gaps" % (rows, width))
         if y.device != self.device:
@@ -157,19 +161,22 @@ class Mx4Calls:
         """Rows of x (float32, float16, bfloat16; rows may lie apart) as an Mx4Tensor.  `rows`: int32 row numbers of x, one
         for each row of the result (a number outside x leaves its row as it was).  `rows_dev`: device word with the
         live number of rows."""
-        code = _dtype_code(x.dtype)
+        code = _codes.get(x.dtype)
+        if code is None:
+            code = _dtype_code(x.dtype)
         have, k, stride = self._mx4_rows_in(x)
         count = have if rows is None else rows.numel()
         if out is None:
-            out = Mx4Tensor.empty(count, k, self.device)
+            out = Mx4Tensor._make(count, k, self.device)
         elif out.rows != count or out.k != k:
             raise ValueError("out has %d rows of %d values" % (out.rows, out.k))
         elif out.device != self.device:
             raise self._mx4_elsewhere(out)
         codes, scales = out._at
-        result = self._mx4_quantize_call(self._address, self._stream(), x.data_ptr(), code, have, stride, k,
-                                         self._mx4_words("rows", rows), count, self._mx4_words("rows_dev", rows_dev, 1),
-                                         codes, scales)
+        result = self._mx4_quantize_call(
+            self._address, self._stream(), x.data_ptr(), code, have, stride, k,
+            None if rows is None else self._mx4_words("rows", rows), count,
+            None if rows_dev is None else self._mx4_words("rows_dev", rows_dev, 1), codes, scales)
         if result != 0:
             self._check(result)
         return out
@@ -185,7 +192,7 @@ class Mx4Calls:
         if out is None:
             dtype = dtype or torch.float16
             code = _dtype_code(dtype)
-            out = torch.empty((rows, t.k), dtype=dtype, device=self.device)
+            out = torch.empty(rows, t.k, dtype=dtype, device=self.device)
         else:
             code = _dtype_code(out.dtype)
             if tuple(out.shape) != (rows, t.k) or not out.is_contiguous() or (dtype is not None and out.dtype != dtype):
@@ -207,7 +214,7 @@ class Mx4Calls:
         w_codes, w_scales = w._at
         x_codes, x_scales = x._at
         result = self._mx4_matmul_call(self._address, self._stream(), w_codes, w_scales, w.rows, w.k, x_codes, x_scales, x.rows,
-                                       self._mx4_words("m_dev", m_dev, 1), y.data_ptr(), _dtype_code(y.dtype), epilogue)
+                                       None if m_dev is None else self._mx4_words("m_dev", m_dev, 1), y.data_ptr(), _dtype_code(y.dtype), epilogue)
         if result != 0:
             self._check(result)
         return y
@@ -232,7 +239,7 @@ class Mx4Calls:
                 raise self._mx4_elsewhere(workspace)
         w_codes, w_scales = w._at
         result = self._mx4_linear_call(self._address, self._stream(), w_codes, w_scales, w.rows, k, x.data_ptr(), code, stride,
-                                       m, self._mx4_words("m_dev", m_dev, 1), y.data_ptr(), _dtype_code(y.dtype), epilogue,
+                                       m, None if m_dev is None else self._mx4_words("m_dev", m_dev, 1), y.data_ptr(), _dtype_code(y.dtype), epilogue,
                                        _pointer(workspace), size)
         if result != 0:
             self._check(result)
