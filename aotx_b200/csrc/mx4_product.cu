@@ -26,40 +26,53 @@
 
 namespace q8 {
 
-constexpr uint32_t kMxThreads = 14 * 32;
-constexpr uint32_t kMxStoreWarps = 8;       // two for each quarter of tensor memory's lanes, which take its columns in turn
-constexpr uint32_t kMxScaleWarp = 8;        // the first of four
-constexpr uint32_t kMxCopyWarp = 12;
-constexpr uint32_t kMxMmaWarp = 13;
+// The forms of the kernel: a block to an SM, two, or a pair of blocks on neighbouring SMs that work on one tile.
+enum MxForm { kMxOne, kMxTwo, kMxPair };
+// Warps of a block: those that store, four that bring scales, one that copies codes, one that issues MMAs.  Two storing warps for each
+// quarter of tensor memory's lanes, which take its columns in turn; one where there are few columns.
+__host__ __device__ constexpr uint32_t mx_store_warps(MxForm form)
+{
+    return form == kMxTwo ? 4u : 8u;
+}
+__host__ __device__ constexpr uint32_t mx_threads(MxForm form)
+{
+    return (mx_store_warps(form) + 6u) * 32u;
+}
 constexpr uint32_t kMxRows = 128;           // rows of w per tile
 constexpr uint32_t kMxMaxTok = 256;         // rows of x per tile, at most
 constexpr uint32_t kMxStageK = 256;         // values of a row per part of a stage: 128 bytes, a row of the swizzle
 constexpr uint32_t kMxStageBytes = kMxStageK / 2;
 constexpr uint32_t kMxMaxStages = 12;
-constexpr uint32_t kMxMaxSlots = 64;        // stages of x that stay
+constexpr uint32_t kMxMaxSlots = 9;         // stages of x that stay
 constexpr uint32_t kMxScaleBlock = 512;     // scales of 128 rows and 128 values
 constexpr uint32_t kMxEpilogueStage = 16u * 32u * 4u;  // per storing warp
-constexpr uint32_t kMxFewSteps = 2;         // steps of a block, at least
-constexpr uint32_t kMxMaxCluster = 8;
+constexpr uint32_t kMxFewSteps = 8;
 constexpr uint32_t kMxPairTok = 192;        // rows of x per tile of a pair of blocks, at most: two accumulators beside the scales
+constexpr uint32_t kMxTwoTok = 64;          // rows of x per tile where two blocks share an SM, at most
+constexpr uint32_t kMxTwoClusterTok = 32;   // and where they are a cluster's
 constexpr uint32_t kMxPairFrom = 257;       // rows of x that pairs take, at least
 // Tiles of a product that is multiplied by clusters, at most: as many clusters of each size as the GPU runs at the same time.
 constexpr uint32_t kMxClustersOf8 = 12;
 constexpr uint32_t kMxClustersOf4 = 32;
-constexpr uint32_t kMxClusterTiles = 72;    // of two
+constexpr uint32_t kMxClustersOf2 = 72;
 constexpr uint32_t kMxClusterSteps = 4;     // steps of a block of a larger cluster, at least
 constexpr uint32_t kMxClusterTok = 128;     // and rows of x per tile
-// Rows of x that the kernel quantises itself: up to 8, or as many as make 128 with the stages of a block.  Every block turns the
-// stages that it needs by itself, so more cost more than a launch of their own does: 28672 x 4096, 8 rows (16 stages), 17.3 us against
-// 19.6, 16 rows 20.7 against 19.9; 4096 x 14336, 8 rows (14 stages) 13.0 against 13.9, 16 rows 16.5 against 14.1; 4096 x 4096,
-// 16 rows (4 stages), 8.1 against 9.5.
+// What the kernel quantises of x itself: few rows, and few stages of them.  Every block turns the stages that it needs by itself; a launch
+// of its own costs a microsecond more than the product alone.  4096 x 4096 (4 stages a block), 1 row, 6.3 us against 7.3, 8 rows 6.8 against
+// 7.4, 16 rows 9.2 against 7.6; 20000 x 4096 (9 stages), 2 rows, 12.0 against 12.9, 8 rows 14.2 against 13.1; 12288 x 4096
+// (16 stages), 1 row, 11.4 against 10.0.
 constexpr uint32_t kMxFusedRows = 16;
-constexpr uint32_t kMxFusedAnyway = 8;
-constexpr uint32_t kMxFusedStages = 128;
+constexpr uint32_t kMxFusedWork = 32;       // rows times stages
 constexpr uint32_t kMxBars = 2 * kMxMaxStages + 5 + kMxMaxSlots;
-constexpr uint32_t kMxTail = kMxStoreWarps * kMxEpilogueStage + kMxBars * 8u;
-constexpr uint32_t kMxSmem = 223u * 1024u;
-constexpr uint32_t kMxRings = (kMxSmem - 1024u - kMxTail) / 1024u * 1024u;
+__host__ __device__ constexpr uint32_t mx_smem(MxForm form)
+{
+    return (form == kMxTwo ? 109u : 223u) * 1024u;
+}
+// Shared memory for stages and what stays, the first part; the rest is the storing warps' and the barriers.
+__host__ __device__ constexpr uint32_t mx_rings(MxForm form)
+{
+    return (mx_smem(form) - 1024u - mx_store_warps(form) * kMxEpilogueStage - kMxBars * 8u) / 1024u * 1024u;
+}
 
 struct MxArgs {
     const uint32_t *w_scales;
@@ -98,9 +111,9 @@ struct MxArgs {
 // Parts of a stage.  A wait, a commit and what else the thread that issues the MMAs does for a stage take it as long as four MMAs of
 // 208 columns: pairs of blocks have two parts to a stage (28672 x 4096, 2048 rows, 125 -> PAIR_US us).  A single block has one, so
 // that few steps can be dealt evenly.
-__host__ __device__ constexpr uint32_t mx_parts(bool pair)
+__host__ __device__ constexpr uint32_t mx_parts(MxForm form)
 {
-    return pair ? 2u : 1u;
+    return form == kMxPair ? 2u : 1u;
 }
 
 __host__ __device__ inline uint32_t mx_scale_blocks(uint32_t ntok)
@@ -256,6 +269,15 @@ __host__ __device__ __forceinline__ unsigned long long mx_run_begin(uint32_t b, 
     return b * share + (b < more ? b : more);
 }
 
+// Workers that `units` steps are enough for: a run is shorter than a tile's depth only if it is kMxFewSteps parts of 256 values or
+// more, because cutting a tile costs as much as several steps.
+__host__ __device__ __forceinline__ unsigned long long mx_workers(unsigned long long units, uint32_t steps, uint32_t parts)
+{
+    const uint32_t few = steps < kMxFewSteps / parts ? steps : kMxFewSteps / parts;
+    const unsigned long long workers = units / few;
+    return workers != 0ull ? workers : 1ull;
+}
+
 // The pieces of a run: a tile and the steps [from, to) of its depth.
 struct MxPieces {
     uint32_t left;                 // steps of the run that no piece has had
@@ -319,7 +341,7 @@ __device__ __forceinline__ bool mx_wait_flag(const unsigned int *flag, volatile 
 // The stages of x that this block needs, in the order in which it needs them, by the storing warps: a warp takes a row of a
 // stage, 8 values a lane and four lanes a block of 32, the loads of several such rows together.  A warp arrives on a stage's
 // barrier when its rows of it are there.  (The places hold zeros before: rows past the last, values past k.)
-template <typename T>
+template <typename T, uint32_t WARPS>
 __device__ __forceinline__ void mx_quantize_x(const MxArgs &args, const T *x, uint32_t place, uint32_t slot_bytes,
                                               uint32_t bars, uint32_t first_step, uint32_t slots, uint32_t steps, uint32_t live)
 {
@@ -353,7 +375,7 @@ __device__ __forceinline__ void mx_quantize_x(const MxArgs &args, const T *x, ui
                     raw[j].load(x + (unsigned long long)row * args.ldx + at, args.x_aligned != 0u);
                 }
                 scale_at[j] = stage + args.ntok * kMxStageBytes + (block / 4u) * kMxScaleBlock + (row % 32u) * 16u + block % 4u;
-                row += kMxStoreWarps;
+                row += WARPS;
                 while (row >= live) {
                     row -= live;
                     ++slot;
@@ -502,14 +524,15 @@ __device__ __forceinline__ void mx_store(const MxArgs &args, uint32_t stage, uin
 }
 
 // What `others` blocks left of one piece (16 rows of x by 32 rows of w, a slot every `stride` floats), added in their order;
-// the values of up to three blocks are on their way together.
+// the values of TOGETHER blocks are on their way at a time.
+template <uint32_t TOGETHER>
 __device__ __forceinline__ void mx_add_partials(uint32_t (&v)[16], const float *slots, unsigned long long stride, uint32_t others)
 {
 #pragma unroll 1
-    for (uint32_t o = 0; o < others; o += 3u) {
-        float more[3][16];
+    for (uint32_t o = 0; o < others; o += TOGETHER) {
+        float more[TOGETHER][16];
 #pragma unroll
-        for (uint32_t j = 0; j < 3u; ++j) {
+        for (uint32_t j = 0; j < TOGETHER; ++j) {
             if (o + j < others) {
 #pragma unroll
                 for (uint32_t i = 0; i < 16u; ++i) {
@@ -518,7 +541,7 @@ __device__ __forceinline__ void mx_add_partials(uint32_t (&v)[16], const float *
             }
         }
 #pragma unroll
-        for (uint32_t j = 0; j < 3u; ++j) {
+        for (uint32_t j = 0; j < TOGETHER; ++j) {
             if (o + j < others) {
 #pragma unroll
                 for (uint32_t i = 0; i < 16u; ++i) {
@@ -538,11 +561,16 @@ __device__ __forceinline__ uint32_t mx_share(const MxArgs &args, uint32_t rank, 
     return left < args.share ? left : args.share;
 }
 
-template <typename YT, bool GATED, bool PAIR>
-__global__ void __launch_bounds__(kMxThreads, 1)
+template <typename YT, bool GATED, MxForm FORM>
+__global__ void __launch_bounds__(mx_threads(FORM), FORM == kMxTwo ? 2 : 1)
 mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                    const __grid_constant__ MxArgs args)
 {
+    constexpr bool PAIR = FORM == kMxPair;
+    constexpr uint32_t kStoreWarps = mx_store_warps(FORM);
+    constexpr uint32_t kScaleWarp = kStoreWarps;
+    constexpr uint32_t kCopyWarp = kStoreWarps + 4u;
+    constexpr uint32_t kMmaWarp = kStoreWarps + 5u;
     extern __shared__ unsigned char smem_raw[];
     __shared__ MxGroups groups;
     __shared__ uint32_t abort_flag;
@@ -556,12 +584,12 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const bool clusters = !PAIR && args.cluster != 0u;
     // a pair of blocks is one worker: each has half of the tile's rows of w, its sums, and half of its rows of x
     constexpr uint32_t kBlocks = PAIR ? 2u : 1u;
-    constexpr uint32_t kParts = mx_parts(PAIR);
+    constexpr uint32_t kParts = mx_parts(FORM);
     constexpr uint32_t kStepK = kParts * kMxStageK;
     constexpr uint32_t kTileRows = kBlocks * kMxRows;
     const uint32_t half = PAIR ? cluster_ctarank() : 0u;
     const uint32_t worker = PAIR ? blockIdx.x / 2u : blockIdx.x;
-    const uint32_t workers = PAIR ? gridDim.x / 2u : gridDim.x;
+    uint32_t workers = PAIR ? gridDim.x / 2u : gridDim.x;
     const uint32_t x_rows = PAIR ? args.ntok / 2u : args.ntok;     // of a tile, in this block's shared memory
     // a stage: codes of w, scales of w, codes of x, scales of x; x that stays has places of its own behind the ring
     const uint32_t w_scales_at = kParts * kMxRows * kMxStageBytes;
@@ -569,8 +597,8 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const uint32_t x_scales_at = x_codes_at + kParts * x_rows * kMxStageBytes;
     const uint32_t place = base + stages * args.stage_bytes;
     const uint32_t slot_bytes = args.ntok * kMxStageBytes + 2u * x_blocks * kMxScaleBlock;
-    const uint32_t tail = base + kMxRings;
-    const uint32_t bars = tail + kMxStoreWarps * kMxEpilogueStage;
+    const uint32_t tail = base + mx_rings(FORM);
+    const uint32_t bars = tail + kStoreWarps * kMxEpilogueStage;
     auto full = [&](uint32_t s) { return bars + s * 8u; };           // codes and scales are there
     auto empty = [&](uint32_t s) { return bars + (kMxMaxStages + s) * 8u; };
     auto summed = [&](uint32_t b) { return bars + (2u * kMxMaxStages + b) * 8u; };
@@ -581,7 +609,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const uint32_t exchange = tail - (clusters ? args.cluster * args.share * kMxRows * 4u : 0u);
     const uint32_t rank = clusters ? blockIdx.x % args.cluster : 0u;
 
-    if (warp == kMxMmaWarp) {
+    if (warp == kMmaWarp) {
         if (PAIR) {
             pair_tmem_alloc(smem_u32(&tmem_base), args.tmem_columns);
             pair_tmem_relinquish();
@@ -593,7 +621,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     // A barrier a thread: one after the other they take a microsecond of the smallest launches.
     if (threadIdx.x < kMxBars) {
         const uint32_t i = threadIdx.x;
-        uint32_t count = kMxStoreWarps;                          // taken, and the stages of x that stay
+        uint32_t count = kStoreWarps;                          // taken, and the stages of x that stay
         if (i < kMxMaxStages) {
             // the codes and the scales; of a pair the first block's counts the second block's scales as well, and the second
             // block's counts its scales alone
@@ -601,7 +629,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         } else if (i < 2u * kMxMaxStages + 2u || i == 2u * kMxMaxStages + 4u) {
             count = 1u;                                          // empty, summed, exchanged
         } else if (PAIR && i < 2u * kMxMaxStages + 4u) {
-            count = 2u * kMxStoreWarps;
+            count = 2u * kStoreWarps;
         }
         mbar_init(bars + i * 8u, count);
         mbar_init_fence();
@@ -620,8 +648,8 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         __syncwarp();
         cluster_arrive_release();
     }
-    if (stays && warp < kMxStoreWarps) {
-        for (uint32_t at = threadIdx.x * 16u; at < args.slots * slot_bytes; at += kMxStoreWarps * 32u * 16u) {
+    if (stays && warp < kStoreWarps) {
+        for (uint32_t at = threadIdx.x * 16u; at < args.slots * slot_bytes; at += kStoreWarps * 32u * 16u) {
             st_shared_v4(place + at, 0u, 0u, 0u, 0u);
         }
     }
@@ -659,7 +687,14 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         const unsigned long long first = (unsigned long long)(blockIdx.x / args.cluster) * steps;
         mine.set(first + mx_run_begin(rank, args.cluster, steps), first + mx_run_begin(rank + 1u, args.cluster, steps), steps);
     } else {
-        mine.set(mx_run_begin(worker, workers, units), mx_run_begin(worker + 1u, workers, units), steps);
+        // (the device may know of fewer tiles than the launch provided for)
+        const unsigned long long enough = mx_workers(units, steps, kParts);
+        workers = enough < workers ? (uint32_t)enough : workers;
+        if (worker < workers) {
+            mine.set(mx_run_begin(worker, workers, units), mx_run_begin(worker + 1u, workers, units), steps);
+        } else {
+            mine.set(0ull, 0ull, steps);
+        }
     }
     const uint32_t run = mine.left;
     const uint32_t first_step = mine.from;
@@ -676,7 +711,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         return live;
     };
 
-    if (warp == kMxCopyWarp) {
+    if (warp == kCopyWarp) {
         if (elect_one()) {
             // (a pair's codes all count on the first block's barrier, which that block arms for both)
             const uint32_t bytes = kParts * (kMxRows + (stays ? 0u : x_rows)) * kMxStageBytes;
@@ -741,7 +776,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 mbar_wait(full(last % stages), (last / stages) & 1u, &abort_flag, args.status);
             }
         }
-    } else if (PAIR && warp == kMxMmaWarp && half != 0u) {
+    } else if (PAIR && warp == kMmaWarp && half != 0u) {
         // This block's scales are there: told to the first block, whose thread copies them to tensor memory.
         if (elect_one()) {
             const uint32_t signal = mapa_shared(bars, 0u);
@@ -760,7 +795,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 }
             }
         }
-    } else if (warp == kMxMmaWarp) {
+    } else if (warp == kMmaWarp) {
         if (elect_one()) {
             const uint32_t idesc0 = mx_idesc(kTileRows, args.ntok, 0u);
             const uint32_t idesc1 = mx_idesc(kTileRows, args.ntok, 1u);
@@ -863,12 +898,12 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 commit(summed(sums_ring.at));
             }
         }
-    } else if (warp >= kMxScaleWarp && warp < kMxCopyWarp) {
+    } else if (warp >= kScaleWarp && warp < kCopyWarp) {
         // Row t of either operand's tile, and row t + 128 of x.
         if (!stays || !early) {
             grid_dependency_wait();
         }
-        const uint32_t t = threadIdx.x - kMxScaleWarp * 32u;
+        const uint32_t t = threadIdx.x - kScaleWarp * 32u;
         const uint32_t cell = (t % 32u) * 16u + (t / 32u) * 4u;
         // The copies of as many stages as the ring has are on their way together, and count themselves on the stage's barrier:
         // the weights' scales come from memory.
@@ -909,27 +944,28 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             }
         }
         copy_async_wait_all();
-    } else if (warp < kMxStoreWarps) {
+    } else if (warp < kStoreWarps) {
         grid_dependency_wait();       // x, y, the row map and the scratch
         const uint32_t valid = live_rows();
         if (stays) {
             const uint32_t slots = run < args.slots ? run : args.slots;
             switch (args.x_type) {
             case 0u:
-                mx_quantize_x(args, static_cast<const float *>(args.x), place, slot_bytes, x_bars, first_step, slots, steps, valid);
+                mx_quantize_x<float, kStoreWarps>(args, static_cast<const float *>(args.x), place, slot_bytes, x_bars, first_step, slots, steps, valid);
                 break;
             case 1u:
-                mx_quantize_x(args, static_cast<const __half *>(args.x), place, slot_bytes, x_bars, first_step, slots, steps, valid);
+                mx_quantize_x<__half, kStoreWarps>(args, static_cast<const __half *>(args.x), place, slot_bytes, x_bars, first_step, slots, steps, valid);
                 break;
             default:
-                mx_quantize_x(args, static_cast<const __nv_bfloat16 *>(args.x), place, slot_bytes, x_bars, first_step, slots, steps,
+                mx_quantize_x<__nv_bfloat16, kStoreWarps>(args, static_cast<const __nv_bfloat16 *>(args.x), place, slot_bytes, x_bars, first_step, slots, steps,
                               valid);
                 break;
             }
         }
         const uint32_t stage = tail + warp * kMxEpilogueStage;
         const uint32_t quarter = (warp & 3u) * 32u;            // this warp's lanes of tensor memory, rows of w
-        const uint32_t c_first = (warp >> 2) * 16u;            // and its columns, rows of x: 16 of every 32
+        constexpr uint32_t kTurn = kStoreWarps * 4u;           // its columns, rows of x: 16 of each turn's
+        const uint32_t c_first = (warp >> 2) * 16u;
         const uint32_t lane_taddr = tmem + (quarter << 16);
         if (clusters) {
             __syncwarp();
@@ -974,7 +1010,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             const uint32_t columns = GATED ? width / 2u : width;
             if (clusters) {
                 // One piece per block: each column's sums go to the block of the cluster that adds them up.
-                for (uint32_t c0 = c_first; c0 < tile.rows; c0 += 32u) {
+                for (uint32_t c0 = c_first; c0 < tile.rows; c0 += kTurn) {
                     uint32_t v[16];
                     tmem_ld_32x16(sums + c0, v);
                     tmem_ld_wait();
@@ -998,7 +1034,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 if (here == 0u || !mbar_wait_counted(exchanged, 0u, &abort_flag, args.status)) {
                     break;
                 }
-                for (uint32_t c0 = c_first; c0 < here; c0 += 32u) {
+                for (uint32_t c0 = c_first; c0 < here; c0 += kTurn) {
                     uint32_t v[16] = {};
                     for (uint32_t r = 0; r < args.cluster; ++r) {
                         const uint32_t from = exchange + ((r * args.share + c0) * kMxRows + (quarter + lane) * 4u) * 4u;
@@ -1024,7 +1060,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             if (mine.from != 0u) {
                 // Another block owns the tile: its sums go to the scratch.
                 float *out = args.partial + blockIdx.x * args.tile_floats + quarter + lane;
-                for (uint32_t c0 = c_first; c0 < tile.rows; c0 += 32u) {
+                for (uint32_t c0 = c_first; c0 < tile.rows; c0 += kTurn) {
                     uint32_t v[16];
                     tmem_ld_32x16(sums + c0, v);
                     tmem_ld_wait();
@@ -1059,17 +1095,17 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             if (c_first >= tile.rows) {
                 release();
             }
-            for (uint32_t c0 = c_first; c0 < tile.rows; c0 += 32u) {
+            for (uint32_t c0 = c_first; c0 < tile.rows; c0 += kTurn) {
                 const uint32_t row_y = next_row;
-                next_row = row_of(c0 + 32u);
+                next_row = row_of(c0 + kTurn);
                 uint32_t v[16];
                 tmem_ld_32x16(sums + c0, v);
                 tmem_ld_wait();
-                if (c0 + 32u >= tile.rows) {
+                if (c0 + kTurn >= tile.rows) {
                     release();
                 }
                 if (others != 0u) {
-                    mx_add_partials(v, args.partial + (blockIdx.x + kBlocks) * args.tile_floats + (size_t)c0 * kMxRows + quarter + lane,
+                    mx_add_partials<FORM == kMxTwo ? 1u : 3u>(v, args.partial + (blockIdx.x + kBlocks) * args.tile_floats + (size_t)c0 * kMxRows + quarter + lane,
                                     kBlocks * args.tile_floats, others);
                 }
                 mx_store<YT, GATED>(args, stage, lane, first_col, columns, row_y, v);
@@ -1087,14 +1123,14 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     if (PAIR || clusters) {
         // No block leaves while another of the cluster may reach into it.
         __syncwarp();
-        if (clusters && warp >= kMxStoreWarps) {
+        if (clusters && warp >= kStoreWarps) {
             cluster_wait_acquire();
         }
         __syncwarp();
         cluster_arrive_relaxed();
         cluster_wait_acquire();
     }
-    if (warp == kMxMmaWarp) {
+    if (warp == kMmaWarp) {
         tc_fence_after_sync();
         if (PAIR) {
             pair_tmem_dealloc(tmem, args.tmem_columns);
@@ -1138,19 +1174,19 @@ static uint32_t up_to(uint32_t v, uint32_t multiple)
     return (v + multiple - 1u) / multiple * multiple;
 }
 
-template <typename YT, bool GATED, bool PAIR>
+template <typename YT, bool GATED, MxForm FORM>
 static cudaError_t launch_one(cudaStream_t stream, uint32_t grid, const CUtensorMap &map_w, const CUtensorMap &map_x,
                               const MxArgs &args, bool overlap)
 {
     static unsigned long long configured = 0ull;
-    const cudaError_t err = allow_shared_memory(mx4_product_kernel<YT, GATED, PAIR>, kMxSmem, &configured);
+    const cudaError_t err = allow_shared_memory(mx4_product_kernel<YT, GATED, FORM>, mx_smem(FORM), &configured, FORM == kMxTwo);
     if (err != cudaSuccess) {
         return err;
     }
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(grid, 1, 1);
-    config.blockDim = dim3(kMxThreads, 1, 1);
-    config.dynamicSmemBytes = kMxSmem;
+    config.blockDim = dim3(mx_threads(FORM), 1, 1);
+    config.dynamicSmemBytes = mx_smem(FORM);
     config.stream = stream;
     cudaLaunchAttribute attribute[2];
     unsigned int count = 0;
@@ -1159,130 +1195,155 @@ static cudaError_t launch_one(cudaStream_t stream, uint32_t grid, const CUtensor
         attribute[count].val.programmaticStreamSerializationAllowed = 1;
         ++count;
     }
-    if (PAIR || args.cluster > 1u) {
+    if (FORM == kMxPair || args.cluster > 1u) {
         attribute[count].id = cudaLaunchAttributeClusterDimension;
-        attribute[count].val.clusterDim.x = PAIR ? 2u : args.cluster;
+        attribute[count].val.clusterDim.x = FORM == kMxPair ? 2u : args.cluster;
         attribute[count].val.clusterDim.y = 1;
         attribute[count].val.clusterDim.z = 1;
         ++count;
     }
     config.attrs = attribute;
     config.numAttrs = count;
-    return cudaLaunchKernelEx(&config, mx4_product_kernel<YT, GATED, PAIR>, map_w, map_x, args);
+    return cudaLaunchKernelEx(&config, mx4_product_kernel<YT, GATED, FORM>, map_w, map_x, args);
+}
+
+template <typename YT, bool GATED>
+static cudaError_t launch_form(cudaStream_t stream, uint32_t grid, MxForm form, const CUtensorMap &map_w,
+                               const CUtensorMap &map_x, const MxArgs &args, bool overlap)
+{
+    switch (form) {
+    case kMxOne:
+        return launch_one<YT, GATED, kMxOne>(stream, grid, map_w, map_x, args, overlap);
+    case kMxTwo:
+        return launch_one<YT, GATED, kMxTwo>(stream, grid, map_w, map_x, args, overlap);
+    default:
+        return launch_one<YT, GATED, kMxPair>(stream, grid, map_w, map_x, args, overlap);
+    }
 }
 
 template <typename YT>
-static cudaError_t launch_typed(cudaStream_t stream, uint32_t grid, bool pair, const CUtensorMap &map_w,
+static cudaError_t launch_typed(cudaStream_t stream, uint32_t grid, MxForm form, const CUtensorMap &map_w,
                                 const CUtensorMap &map_x, const MxArgs &args, bool overlap)
 {
-    if (args.epilogue == kEpilogueSwiglu) {
-        return pair ? launch_one<YT, true, true>(stream, grid, map_w, map_x, args, overlap)
-                    : launch_one<YT, true, false>(stream, grid, map_w, map_x, args, overlap);
-    }
-    return pair ? launch_one<YT, false, true>(stream, grid, map_w, map_x, args, overlap)
-                : launch_one<YT, false, false>(stream, grid, map_w, map_x, args, overlap);
+    return args.epilogue == kEpilogueSwiglu ? launch_form<YT, true>(stream, grid, form, map_w, map_x, args, overlap)
+                                            : launch_form<YT, false>(stream, grid, form, map_w, map_x, args, overlap);
 }
 
-// How the steps of a product of `tiles` tiles, `steps` deep, are dealt to at most `sms` blocks: in clusters that share a tile
-// where there are few tiles (`clustered`: the caller knows how many, and they are one batch of rows of x), else in equal runs.
+static uint32_t steps_of(uint32_t k, MxForm form)
+{
+    return (k + mx_parts(form) * kMxStageK - 1u) / (mx_parts(form) * kMxStageK);
+}
+
+static uint32_t row_tiles_of(uint32_t n, MxForm form)
+{
+    const uint32_t rows = form == kMxPair ? 2u * kMxRows : kMxRows;
+    return (n + rows - 1u) / rows;
+}
+
+// How a product is multiplied: the form of the kernel, rows of x per tile, and how the steps of its tiles are dealt to blocks.
 struct MxPlan {
-    uint32_t cluster;              // 0: equal runs
+    MxForm form;
+    uint32_t ntok;
+    uint32_t cluster;              // blocks that share a tile; 0: equal runs of steps
     uint32_t grid;
-    uint32_t run;                  // steps of a block, at most
+    uint32_t slots;                // stages of x that a block of mx4_linear keeps, 0: x comes in MX4
 };
 
-static MxPlan plan_of(unsigned long long tiles, uint32_t steps, uint32_t sms, bool clustered)
+static void deal(MxPlan &plan, unsigned long long tiles, uint32_t steps, uint32_t workers)
+{
+    const unsigned long long enough = mx_workers(tiles * steps, steps, mx_parts(plan.form));
+    plan.cluster = 0u;
+    plan.grid = enough < workers ? (uint32_t)enough : workers;
+}
+
+static MxPlan plan_of(const Mx4Product &p, uint32_t sms, bool quantises)
 {
     MxPlan plan = {};
-    if (clustered) {
-        for (uint32_t c = kMxMaxCluster; c >= 2u; c >>= 1) {
-            if (tiles <= (c == 8u ? kMxClustersOf8 : c == 4u ? kMxClustersOf4 : kMxClusterTiles)
-                && steps >= (c == 2u ? c : c * kMxClusterSteps)) {
-                plan.cluster = c;
-                plan.grid = (uint32_t)tiles * c;
-                plan.run = (steps + c - 1u) / c;
-                return plan;
-            }
-        }
-        if (tiles <= sms) {
-            // a tile a block: nothing is cut
-            plan.grid = (uint32_t)tiles;
-            plan.run = steps;
+    const bool by_expert = p.offsets != nullptr;
+    const uint32_t typical = by_expert ? (p.m + p.experts - 1u) / p.experts : p.m;
+    auto tok_tiles = [&] {
+        return by_expert ? (unsigned long long)p.m / plan.ntok + (p.experts < p.m ? p.experts : p.m)
+                         : ((unsigned long long)p.m + plan.ntok - 1u) / plan.ntok;
+    };
+    // Many rows of x, and tiles for every pair: 256 rows of w by up to 192 of x (what two blocks multiply is a multiple of 32).
+    if (!quantises && typical >= kMxPairFrom) {
+        const uint32_t parts = (typical + kMxPairTok - 1u) / kMxPairTok;
+        if ((unsigned long long)parts * row_tiles_of(p.n, kMxPair) * p.experts >= sms / 2u) {
+            plan.form = kMxPair;
+            plan.ntok = up_to((typical + parts - 1u) / parts, 32u);
+            deal(plan, tok_tiles() * row_tiles_of(p.n, kMxPair), steps_of(p.k, kMxPair), sms / 2u);
+            plan.grid *= 2u;
             return plan;
         }
     }
-    const unsigned long long units = tiles * steps;
-    const unsigned long long blocks = (units + kMxFewSteps - 1u) / kMxFewSteps;
-    plan.grid = blocks < sms ? (uint32_t)blocks : sms;
-    plan.run = (uint32_t)((units + plan.grid - 1u) / plan.grid);
+    // Rows of x per tile: equal parts of at most 256, or of 128 where the tiles are few enough for clusters (whose exchange
+    // takes the shared memory of wider ones).  By expert, twice what one has on average, so that most need one tile and their
+    // weights are read once.
+    const uint32_t row_tiles = row_tiles_of(p.n, kMxOne);
+    const uint32_t steps = steps_of(p.k, kMxOne);
+    if (by_expert && typical <= kMxClusterTok / 2u) {
+        plan.ntok = up_to(2u * typical, 32u);
+    } else {
+        uint32_t parts = (typical + kMxMaxTok - 1u) / kMxMaxTok;
+        const uint32_t narrow = (p.m + kMxClusterTok - 1u) / kMxClusterTok;
+        if (!by_expert && (unsigned long long)narrow * row_tiles <= kMxClustersOf2) {
+            parts = narrow;
+        }
+        plan.ntok = up_to((typical + parts - 1u) / parts, 16u);
+    }
+    const unsigned long long tiles = tok_tiles() * row_tiles;
+    // Few tiles, and the host knows how many: clusters that share a tile, else a tile a block.
+    if (!by_expert && (p.m_dev == nullptr || tok_tiles() == 1ull) && plan.ntok <= kMxClusterTok) {
+        for (uint32_t c = 8u; c >= 2u; c >>= 1) {
+            if (tiles <= (c == 8u ? kMxClustersOf8 : c == 4u ? kMxClustersOf4 : kMxClustersOf2)
+                && steps >= (c == 2u ? 2u : c * kMxClusterSteps)) {
+                plan.form = c >= 4u && plan.ntok <= kMxTwoClusterTok ? kMxTwo : kMxOne;
+                plan.cluster = c;
+                plan.grid = (uint32_t)tiles * c;
+                return plan;
+            }
+        }
+        if (tiles <= sms || (!quantises && tiles <= 2u * sms && plan.ntok <= kMxTwoTok)) {
+            plan.form = tiles <= sms ? kMxOne : kMxTwo;
+            plan.grid = (uint32_t)tiles;
+            return plan;
+        }
+    }
+    plan.form = plan.ntok <= kMxTwoTok ? kMxTwo : kMxOne;
+    deal(plan, tiles, steps, plan.form == kMxTwo ? 2u * sms : sms);
     return plan;
 }
 
-static uint32_t steps_of(uint32_t k, bool pair = false)
+// The plan of mx4_linear for few rows: the stages of x that a block needs have to fit beside a ring of weights.
+static MxPlan linear_plan(const Mx4Product &p, uint32_t sms)
 {
-    return (k + mx_parts(pair) * kMxStageK - 1u) / (mx_parts(pair) * kMxStageK);
-}
-
-static uint32_t row_tiles_of(uint32_t n)
-{
-    return (n + kMxRows - 1u) / kMxRows;
-}
-
-// Rows of x per tile: equal parts of at most 256, or of 128 where the tiles are few enough for clusters (whose exchange
-// takes the shared memory of wider ones).  By expert, twice what one has on average, so that most need one tile and their
-// weights are read once.
-static uint32_t token_tile(const Mx4Product &p)
-{
-    const uint32_t typical = p.offsets != nullptr ? (p.m + p.experts - 1u) / p.experts : p.m;
-    if (p.offsets != nullptr && typical <= kMxClusterTok / 2u) {
-        return up_to(2u * typical, 32u);
+    MxPlan plan = plan_of(p, sms, true);
+    if (p.m > kMxFusedRows) {
+        return plan;
     }
-    uint32_t parts = (typical + kMxMaxTok - 1u) / kMxMaxTok;
-    if (p.offsets == nullptr) {
-        const uint32_t halves = (p.m + kMxClusterTok - 1u) / kMxClusterTok;
-        if (halves * (unsigned long long)row_tiles_of(p.n) <= kMxClusterTiles) {
-            parts = halves;
-        }
+    const uint32_t steps = steps_of(p.k, plan.form);
+    const unsigned long long units = (unsigned long long)row_tiles_of(p.n, plan.form) * steps;
+    const uint32_t bytes = plan.ntok * kMxStageBytes + 2u * kMxScaleBlock;
+    auto slots = [&] {
+        const uint32_t run = plan.cluster != 0u ? (steps + plan.cluster - 1u) / plan.cluster
+                                                : (uint32_t)((units + plan.grid - 1u) / plan.grid);
+        return run < steps ? run : steps;
+    };
+    const uint32_t all = slots();
+    if (all <= kMxMaxSlots && p.m * all <= kMxFusedWork && all * bytes <= mx_rings(plan.form) * 2u / 5u) {
+        plan.slots = all;
     }
-    return up_to((typical + parts - 1u) / parts, 16u);
-}
-
-// Pairs of blocks: 256 rows of w by up to 192 of x.
-static uint32_t pair_token_tile(const Mx4Product &p)
-{
-    const uint32_t typical = p.offsets != nullptr ? (p.m + p.experts - 1u) / p.experts : p.m;
-    const uint32_t parts = (typical + kMxPairTok - 1u) / kMxPairTok;
-    return up_to((typical + parts - 1u) / parts, 32u);
-}
-
-static bool pair_takes(const Mx4Product &p, uint32_t sms)
-{
-    if (p.x != nullptr) {
-        return false;
-    }
-    const uint32_t typical = p.offsets != nullptr ? (p.m + p.experts - 1u) / p.experts : p.m;
-    const unsigned long long tiles = (unsigned long long)((typical + kMxPairTok - 1u) / kMxPairTok)
-                                   * ((p.n + 2u * kMxRows - 1u) / (2u * kMxRows)) * p.experts;
-    return typical >= kMxPairFrom && tiles >= sms / 2u;
-}
-
-// Stages of x that a block of mx4_linear keeps, 0 if that many rows are quantised by a launch of their own.
-static uint32_t linear_slots(uint32_t n, uint32_t k, uint32_t m, uint32_t sms)
-{
-    if (m > kMxFusedRows) {
-        return 0u;
-    }
-    const uint32_t steps = steps_of(k);
-    const uint32_t run = plan_of(row_tiles_of(n), steps, sms, true).run;
-    const uint32_t slots = run < steps ? run : steps;
-    const uint32_t bytes = up_to(m, 16u) * kMxStageBytes + 2u * kMxScaleBlock;
-    return slots <= kMxMaxSlots && slots * bytes <= kMxRings / 2u && (m <= kMxFusedAnyway || m * slots <= kMxFusedStages)
-        ? slots : 0u;
+    return plan;
 }
 
 bool mx4_linear_quantizes(uint32_t n, uint32_t k, uint32_t m, unsigned int sm_count)
 {
-    return linear_slots(n, k, m, sm_count) != 0u;
+    Mx4Product p = {};
+    p.experts = 1u;
+    p.n = n;
+    p.k = k;
+    p.m = m;
+    return linear_plan(p, sm_count).slots != 0u;
 }
 
 cudaError_t launch_mx4_product(cudaStream_t stream, const UmmaScratch &scratch, unsigned int sm_count, unsigned int set,
@@ -1316,40 +1377,30 @@ cudaError_t launch_mx4_product(cudaStream_t stream, const UmmaScratch &scratch, 
     const uint32_t size = p.y_dtype == 0 ? 4u : 2u;
     args.wide = (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0u && (args.ldy * size) % 16u == 0u;
     const uint32_t blocks = sm_count < scratch.blocks ? sm_count : scratch.blocks;
-    const bool pair = pair_takes(p, blocks);
-    args.ntok = pair ? pair_token_tile(p) : token_tile(p);
+    const MxPlan plan = p.x != nullptr ? linear_plan(p, blocks) : plan_of(p, blocks, false);
+    const bool pair = plan.form == kMxPair;
+    const MxForm form = plan.form;
+    args.ntok = plan.ntok;
+    args.slots = plan.slots;
+    args.cluster = plan.cluster;
     if (p.x != nullptr) {
         args.x = p.x;
         args.x_type = (uint32_t)p.x_dtype;
         args.ldx = p.ldx;
         args.x_aligned = (reinterpret_cast<uintptr_t>(p.x) & 15u) == 0u && (p.ldx * (p.x_dtype == 0 ? 4u : 2u)) % 16u == 0u;
-        args.slots = linear_slots(p.n, p.k, p.m, blocks);
     }
     const uint32_t x_blocks = mx_scale_blocks(args.ntok);
     const uint32_t x_rows = pair ? args.ntok / 2u : args.ntok;
-    const uint32_t x_bytes = mx_parts(pair) * (x_rows * kMxStageBytes + 2u * x_blocks * kMxScaleBlock);
-    args.stage_bytes = mx_parts(pair) * (kMxRows * kMxStageBytes + 2u * kMxScaleBlock) + (args.slots != 0u ? 0u : x_bytes);
-    // Tiles at most (by expert and live batch the device knows how many).
-    const unsigned long long tok_tiles = p.offsets != nullptr ? p.m / args.ntok + (p.experts < p.m ? p.experts : p.m)
-                                                              : (p.m + args.ntok - 1u) / args.ntok;
-    MxPlan plan;
-    if (pair) {
-        const unsigned long long tiles = tok_tiles * ((p.n + 2u * kMxRows - 1u) / (2u * kMxRows));
-        plan = plan_of(tiles, steps_of(p.k, true), blocks / 2u, false);
-        plan.grid *= 2u;
-    } else {
-        plan = plan_of(tok_tiles * row_tiles_of(p.n), steps_of(p.k), blocks,
-                       p.offsets == nullptr && (p.m_dev == nullptr || tok_tiles == 1u) && args.ntok <= kMxClusterTok);
-    }
-    args.cluster = plan.cluster;
+    const uint32_t x_bytes = mx_parts(form) * (x_rows * kMxStageBytes + 2u * x_blocks * kMxScaleBlock);
+    args.stage_bytes = mx_parts(form) * (kMxRows * kMxStageBytes + 2u * kMxScaleBlock) + (args.slots != 0u ? 0u : x_bytes);
     const uint32_t tile_rows = p.m < args.ntok ? p.m : args.ntok;
     args.share = plan.cluster != 0u ? up_to((tile_rows + plan.cluster - 1u) / plan.cluster, 4u) : 0u;
     const uint32_t exchange = args.cluster * args.share * kMxRows * 4u;
-    const uint32_t fit = (kMxRings - exchange - args.slots * x_bytes) / args.stage_bytes;
+    const uint32_t fit = (mx_rings(form) - exchange - args.slots * x_bytes) / args.stage_bytes;
     args.stages = fit < kMxMaxStages ? fit : kMxMaxStages;
     // Tensor memory: two accumulators where they fit beside scales, and those of as many stages as then fit, two at least (a
     // single block copies a stage's scales without asking for the place: it has one for each).
-    const uint32_t stage_columns = mx_parts(pair) * 8u * (1u + x_blocks);
+    const uint32_t stage_columns = mx_parts(form) * 8u * (1u + x_blocks);
     const uint32_t least = pair ? 2u * stage_columns : args.stages * stage_columns;
     args.accumulators = 2u * args.ntok + least <= 512u ? 2u : 1u;
     const uint32_t places = (512u - args.accumulators * args.ntok) / stage_columns;
@@ -1366,11 +1417,11 @@ cudaError_t launch_mx4_product(cudaStream_t stream, const UmmaScratch &scratch, 
     }
     switch (p.y_dtype) {
     case 0:
-        return launch_typed<float>(stream, plan.grid, pair, map_w, map_x, args, p.overlap);
+        return launch_typed<float>(stream, plan.grid, form, map_w, map_x, args, p.overlap);
     case 1:
-        return launch_typed<__half>(stream, plan.grid, pair, map_w, map_x, args, p.overlap);
+        return launch_typed<__half>(stream, plan.grid, form, map_w, map_x, args, p.overlap);
     default:
-        return launch_typed<__nv_bfloat16>(stream, plan.grid, pair, map_w, map_x, args, p.overlap);
+        return launch_typed<__nv_bfloat16>(stream, plan.grid, form, map_w, map_x, args, p.overlap);
     }
 }
 

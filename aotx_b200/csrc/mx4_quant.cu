@@ -28,10 +28,10 @@ mx4_quantize_kernel(const T *x, uint32_t x_rows, unsigned long long ldx, uint32_
                     bool activations)
 {
     constexpr uint32_t kTogether = sizeof(T) == 4u ? 2u : kQuantChunks;
-    grid_dependency_wait();
     if (activations) {
-        grid_launch_dependents();
+        grid_launch_dependents();      // the product that this is part of: nothing is written here that it reads before its own wait
     }
+    grid_dependency_wait();
     uint32_t live = rows;
     if (rows_dev != nullptr) {
         const uint32_t on_device = *rows_dev;

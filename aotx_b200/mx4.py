@@ -220,8 +220,8 @@ class Mx4Calls:
         return y
 
     def mx4_linear(self, w, x, m_dev=None, y=None, y_dtype=None, epilogue=EPILOGUE_STORE, workspace=None):
-        """`mx4_matmul` of w with `mx4_quantize(x)`, the same y bit for bit; few rows are quantised by the kernel that
-        multiplies them."""
+        """`mx4_matmul` of w with `mx4_quantize(x)`, up to the order of the float sums; few rows are quantised by the kernel
+        that multiplies them."""
         code = _dtype_code(x.dtype)
         m, k, stride = self._mx4_rows_in(x)
         self._mx4_pair(w, k)

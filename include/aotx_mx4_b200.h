@@ -52,7 +52,7 @@ int aotx_mx4_matmul(aotx_q8_ctx *ctx, void *stream, const void *w_codes, const v
                     const void *x_codes, const void *x_scales, uint32_t m, const uint32_t *m_dev, void *y, int y_dtype,
                     int epilogue);
 
-/* aotx_mx4_quantize of x, then aotx_mx4_matmul: the same y, bit for bit.  Few rows are quantised by the kernel that
+/* aotx_mx4_quantize of x, then aotx_mx4_matmul: the same products, whose float sums may be formed in another order.  Few rows are quantised by the kernel that
  * multiplies them; otherwise `workspace` (16-byte aligned device memory of aotx_mx4_linear_workspace_bytes; 0 where none is
  * needed) holds x in MX4 between the two. */
 size_t aotx_mx4_linear_workspace_bytes(const aotx_q8_ctx *ctx, uint32_t n, uint32_t k, uint32_t m);

@@ -44,7 +44,7 @@ def random_codes(rows, k, seed, low, high):
 SHAPES = [(128, 64, 16), (16, 32, 1), (1, 32, 3), (130, 96, 5), (127, 256, 17), (300, 416, 33), (129, 1056, 100), (512, 512, 128),
           (260, 320, 129), (257, 288, 200), (200, 1024, 256), (140, 192, 257), (388, 544, 513), (64, 4096, 2), (2000, 2560, 300),
           (4100, 1312, 40), (2050, 1024, 20), (6144, 1024, 100), (4096, 2080, 256), (1030, 8192, 3), (8192, 512, 130),
-          (9000, 608, 16), (40000, 800, 9)]
+          (9000, 608, 16), (40000, 800, 9), (40000, 288, 60), (30000, 1056, 128)]
 # pairs of blocks: whole tiles, cut ones, edges of either operand
 PAIRS = [(9472, 256, 258), (9500, 96, 290), (10001, 544, 300), (9472, 1312, 448), (4800, 800, 1000), (20000, 2080, 260)]
 
@@ -120,27 +120,33 @@ def test_y_off_a_boundary_and_scale_nan(ctx):
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("n,k,m", [(130, 96, 1), (300, 416, 5), (200, 2080, 16), (4096, 512, 8), (140, 1056, 17), (200, 96, 33),
-                                   (260, 320, 100), (130, 64, 300)])
+                                   (260, 320, 100), (130, 64, 300), (4000, 4128, 2), (19000, 1056, 3), (40000, 2080, 4),
+                                   (40000, 288, 16), (20000, 1056, 3), (1000, 288, 16)])
 def test_linear_is_quantisation_and_product(ctx, n, k, m, kind):
+    """Against the sums of what mx4_quantize makes of the same rows."""
     torch = torch_mod()
-    w = tensor(*random_codes(n, k, n, -9, -3))
+    codes = random_codes(n, k, n, -9, -3)
+    w, w64 = tensor(*codes), _mx4.values(*codes)
     gen = torch.Generator().manual_seed(m)
     x = torch.randn((m, k + 8), generator=gen)
     x[m // 2, :32] = 0
     x = x.to(dtype(kind)).cuda()
     for view in (x[:, :k].contiguous(), x[:, 8:], x[:, 1:k + 1]):
         q = ctx.mx4_quantize(view)
-        assert torch.equal(ctx.mx4_linear(w, view), ctx.mx4_matmul(w, q))
+        x64 = _mx4.values(q.codes.cpu().numpy(), q.scales.cpu().numpy())
+        want, error = x64 @ w64.T, _mx4.sum_bound(w64, x64)
+        assert _mx4.close(ctx.mx4_linear(w, view).double().cpu().numpy(), want, error, "f32").all()
         for out in ("f16", "bf16"):
-            assert torch.equal(ctx.mx4_linear(w, view, y_dtype=dtype(out), epilogue=SWIGLU),
-                               ctx.mx4_matmul(w, q, y_dtype=dtype(out), epilogue=SWIGLU))
+            got = ctx.mx4_linear(w, view, y_dtype=dtype(out), epilogue=SWIGLU).double().cpu().numpy()
+            assert _mx4.close(got, _mx4.gated(want), _mx4.gated_bound(want, error, out), out).all()
         y = torch.ones((m, n), device="cuda")
         ctx.mx4_linear(w, view, y=y, epilogue=ADD)
-        assert torch.equal(y, 1 + ctx.mx4_matmul(w, q))
+        assert _mx4.close(y.double().cpu().numpy(), 1 + want, error + np.abs(want) * 2.0 ** -24, "f32").all()
         live = torch.tensor([m // 2], dtype=torch.int32, device="cuda")
         y = torch.full((m, n), GUARD, device="cuda")
         ctx.mx4_linear(w, view, y=y, m_dev=live)
-        assert torch.equal(y[:m // 2], ctx.mx4_matmul(w, q)[:m // 2]) and (y[m // 2:] == GUARD).all()
+        assert _mx4.close(y[:m // 2].double().cpu().numpy(), want[:m // 2], error[:m // 2], "f32").all()
+        assert (y[m // 2:] == GUARD).all()
 
 
 def test_linear_takes_not_a_number_into_its_row_only(ctx):
@@ -330,7 +336,7 @@ def test_captured_twice_and_on_another_stream(ctx, m):
         x.copy_(torch.randn((m, k), device="cuda").half())
         graphs[turn % 2].replay()
         torch.cuda.synchronize()
-        once = ctx.mx4_matmul(w, ctx.mx4_quantize(x))
+        once = ctx.mx4_linear(w, x)
         assert torch.equal(ys[turn % 2], once + once)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
