@@ -25,13 +25,16 @@ template <typename T>
 __global__ void __launch_bounds__(kQuantThreads)
 mx4_quantize_kernel(const T *x, uint32_t x_rows, unsigned long long ldx, uint32_t k, const uint32_t *rows_of, uint32_t rows,
                     const uint32_t *rows_dev, uint2 *__restrict__ codes, uint8_t *__restrict__ scales, bool aligned,
-                    bool activations)
+                    uint32_t start)
 {
     constexpr uint32_t kTogether = sizeof(T) == 4u ? 2u : kQuantChunks;
-    if (activations) {
-        grid_launch_dependents();      // the product that this is part of: nothing is written here that it reads before its own wait
+    if (start == kMx4StartAtOnce) {
+        grid_launch_dependents();
     }
     grid_dependency_wait();
+    if (start == kMx4StartBehindWait) {
+        grid_launch_dependents();
+    }
     uint32_t live = rows;
     if (rows_dev != nullptr) {
         const uint32_t on_device = *rows_dev;
@@ -79,8 +82,7 @@ mx4_quantize_kernel(const T *x, uint32_t x_rows, unsigned long long ldx, uint32_
             }
         }
     }
-    if (!activations) {
-        // Not before the stores: what is written here may be weights, which a product reads early (aotx_mx4_matmul).
+    if (start == kMx4StartBehindStores) {
         __syncthreads();
         grid_launch_dependents();
     }
@@ -193,12 +195,12 @@ static dim3 quant_grid(uint32_t rows, uint32_t rows_a_block, uint32_t k)
 
 cudaError_t launch_mx4_quantize(cudaStream_t stream, bool overlap, const void *x, int x_dtype, uint32_t x_rows,
                                 unsigned long long ldx, uint32_t k, const uint32_t *rows_of, uint32_t rows,
-                                const uint32_t *rows_dev, void *codes, void *scales, bool activations)
+                                const uint32_t *rows_dev, void *codes, void *scales, uint32_t start)
 {
     auto launch = [&](auto kernel, auto *typed) {
         const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15u) == 0u && (ldx * sizeof(*typed)) % 16u == 0u;
         return launch_kernel_early(overlap, kernel, quant_grid(rows, kQuantRows, k), kQuantThreads, 0, stream, typed, x_rows, ldx, k,
-                                   rows_of, rows, rows_dev, static_cast<uint2 *>(codes), static_cast<uint8_t *>(scales), aligned, activations);
+                                   rows_of, rows, rows_dev, static_cast<uint2 *>(codes), static_cast<uint8_t *>(scales), aligned, start);
     };
     switch (x_dtype) {
     case 0:

@@ -169,7 +169,7 @@ def order_of(ids, experts, live):
 
 
 @pytest.mark.parametrize("tokens,used,experts", [(1, 1, 1), (1, 8, 128), (8, 8, 128), (7, 3, 5), (77, 4, 20), (512, 8, 128),
-                                                 (300, 2, 256), (2048, 8, 64), (33, 1, 3)])
+                                                 (300, 2, 256), (2048, 8, 64), (33, 1, 3), (5000, 7, 200)])
 def test_order(ctx, tokens, used, experts):
     torch = torch_mod()
     rng = np.random.Generator(np.random.PCG64(tokens))
