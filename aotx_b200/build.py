@@ -22,7 +22,7 @@ SOURCES = ["q8_api.cu", "q8_simt.cu", "q8_dispatch.cu", "q8_stream.cu", "q8_deco
 MX4_SOURCES = ["mx4_api.cu", "mx4_quant.cu", "mx4_product.cu", "mx4_order.cu"]
 HEADERS = ["q8_common.cuh", "q8_ptx.cuh", "q8_warp_ptx.cuh", "q8_rows.cuh", "q8_schedule.cuh", "q8_decode_operands.cuh", "q8_store.cuh", "q8_simt_gemv.cuh", "q8_route.cuh", "q8_launch.h", "q8_tile.cuh", "q_blocks.cuh", os.path.join("..", "..", "include", "aotx_q8_b200.h"),
            os.path.join("..", "..", "include", "aotx_gguf_b200.h"), "q8_context.h"]
-MX4_HEADERS = ["mx4.h", "mx4_ptx.cuh", os.path.join("..", "..", "include", "aotx_mx4_b200.h")]
+MX4_HEADERS = ["mx4.h", "mx4_block.cuh", "mx4_ptx.cuh", os.path.join("..", "..", "include", "aotx_mx4_b200.h")]
 NVCC_FLAGS = ["-std=c++17", "-O3", "-lineinfo", "-gencode", "arch=compute_100a,code=sm_100a",
               "-Xcompiler", "-fPIC", "-Xptxas", "-v"]
 

@@ -10,7 +10,8 @@
 namespace {
 
 const uint32_t kMaxRows = 1u << 24;    // of x; (1 << 31) - 1 of w
-const uint32_t kMaxDepth = 1u << 26;
+const uint32_t kMaxDepth = 1u << 24;
+const uint64_t kMaxProducts = 1ull << 40;  // rows of x by an expert's rows of w: the kernel counts its tiles in 32 bits
 
 int fail(aotx_q8_ctx *ctx, cudaError_t err)
 {
@@ -254,7 +255,7 @@ extern "C" int aotx_mx4_matmul_grouped(aotx_q8_ctx *ctx, void *stream, const voi
                                        void *y, int y_dtype, int epilogue)
 {
     if (ctx == nullptr || !known(y_dtype) || !depth(k) || experts == 0u || experts > q8::kMx4MaxExperts
-        || (unsigned long long)experts * n > 0x7FFFFFFFull || rows > kMaxRows
+        || (unsigned long long)experts * n > 0x7FFFFFFFull || rows > kMaxRows || (uint64_t)rows * n > kMaxProducts
         || !epilogue_known(epilogue, n, y_dtype, false)) {
         return AOTX_Q8_ERR_ARGUMENT;
     }

@@ -14,6 +14,9 @@
  *           (anything but 255 does).  4-byte aligned.  (The four scales that 128 values of a row need lie together, and the
  *           words of successive rows do, whatever row a tile of the product starts at.)
  *
+ * Limits: k up to 2^24; rows of x up to 2^24 (quantisation and dequantisation: 2^31 - 1, as rows of w); grouped, rows of x
+ * times rows of an expert's matrix up to 2^40.
+ *
  * The reference has no counterpart: its block types (cuda/model/model.cuh:24-36) all are dequantised to binary16 before
  * they are multiplied.
  */
@@ -52,9 +55,10 @@ int aotx_mx4_matmul(aotx_q8_ctx *ctx, void *stream, const void *w_codes, const v
                     const void *x_codes, const void *x_scales, uint32_t m, const uint32_t *m_dev, void *y, int y_dtype,
                     int epilogue);
 
-/* aotx_mx4_quantize of x, then aotx_mx4_matmul: the same products, whose float sums may be formed in another order.  Few rows are quantised by the kernel that
- * multiplies them; otherwise `workspace` (16-byte aligned device memory of aotx_mx4_linear_workspace_bytes; 0 where none is
- * needed) holds x in MX4 between the two. */
+/* aotx_mx4_quantize of x, then aotx_mx4_matmul: the same products, whose float sums may be formed in another order.  Few rows
+ * are quantised by the kernel that multiplies them; otherwise `workspace` (16-byte aligned device memory of
+ * aotx_mx4_linear_workspace_bytes; 0 where none is needed) holds x in MX4 between the two.  (The weights may be read early
+ * here as there: before x is quantised.) */
 size_t aotx_mx4_linear_workspace_bytes(const aotx_q8_ctx *ctx, uint32_t n, uint32_t k, uint32_t m);
 int aotx_mx4_linear(aotx_q8_ctx *ctx, void *stream, const void *w_codes, const void *w_scales, uint32_t n, uint32_t k,
                     const void *x, int x_dtype, uint64_t ldx, uint32_t m, const uint32_t *m_dev, void *y, int y_dtype,
@@ -71,9 +75,9 @@ int aotx_mx4_moe_order(aotx_q8_ctx *ctx, void *stream, const uint32_t *ids, uint
 /* Products grouped by expert: rows offsets[e] .. offsets[e + 1] of x (`rows` rows, sorted by expert) times expert e's matrix,
  * rows e * n .. e * n + n of w (experts * n rows).  offsets: experts + 1 device words, ascending; an expert may have no
  * row.  Entries past `rows` count as `rows`, and a range that runs backwards as empty.  Row i of the result goes to row i of y or,
- * where y_rows_of is not null, to row y_rows_of[i]; y has y_rows rows, and a row past them is left out.  Rows of
- * x that no expert has, and their rows of y, are not touched.  epilogue: STORE or SWIGLU (n counts gate and up rows).
- * experts <= 256. */
+ * where y_rows_of is not null, to row y_rows_of[i]; y has y_rows rows, and a row past them is left out (a row that two
+ * entries name holds either's result, a value at a time).  Rows of x that no expert has, and their rows of y, are not
+ * touched.  epilogue: STORE or SWIGLU (n counts gate and up rows).  experts <= 256. */
 int aotx_mx4_matmul_grouped(aotx_q8_ctx *ctx, void *stream, const void *w_codes, const void *w_scales, uint32_t experts,
                             uint32_t n, uint32_t k, const void *x_codes, const void *x_scales, uint32_t rows,
                             const uint32_t *offsets, const uint32_t *y_rows_of, uint32_t y_rows, void *y, int y_dtype,

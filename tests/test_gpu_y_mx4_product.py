@@ -344,3 +344,60 @@ def test_captured_twice_and_on_another_stream(ctx, m):
         other = ctx.mx4_linear(w, x)
     side.synchronize()
     assert torch.equal(other, ctx.mx4_linear(w, x))
+
+
+def test_two_contexts_at_once(ctx):
+    """Products whose tiles are cut between blocks, on two contexts and two streams at the same time: blocks wait for blocks of
+    their own launch while the other launch holds some of the SMs."""
+    import aotx_b200
+    torch = torch_mod()
+    other = aotx_b200.Q8Context(0)
+    shapes = ((40000, 1056, 8), (20000, 2080, 300), (38000, 544, 130))
+    tensors = [(tensor(*random_codes(n, k, n, -9, -3)), tensor(*random_codes(m, k, m, -4, 3))) for n, k, m in shapes]
+    want = [ctx.mx4_matmul(w, x) for w, x in tensors]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    results = []
+    for turn in range(6):
+        for context, stream in zip((ctx, other), streams):
+            with torch.cuda.stream(stream):
+                w, x = tensors[(turn + (context is other)) % 3]
+                results.append(((turn + (context is other)) % 3, context.mx4_matmul(w, x)))
+    torch.cuda.synchronize()
+    for i, got in results:
+        assert torch.equal(got, want[i])
+    assert other.device_status() == 0
+    other.close()
+
+
+def test_tensors_past_four_gigabytes(ctx):
+    """Addresses of codes, of values and of results that pass 32 bits: the last rows against a tensor of those rows alone."""
+    import aotx_b200
+    torch = torch_mod()
+    n, k, m = 1100000, 8192, 3
+    w = aotx_b200.Mx4Tensor.empty(n, k, "cuda")
+    w.codes.random_(0, 256)
+    w.scales.random_(120, 124)
+    x = torch.randn((m, k), device="cuda").half()
+    last = slice(n - 300, n)
+    part = aotx_b200.Mx4Tensor(w.codes[last].contiguous(), w.scales[:, last].contiguous())
+    q = ctx.mx4_quantize(x)
+    w64 = _mx4.values(part.codes.cpu().numpy(), part.scales.cpu().numpy())
+    x64 = _mx4.values(q.codes.cpu().numpy(), q.scales.cpu().numpy())
+    want, error = x64 @ w64.T, _mx4.sum_bound(w64, x64)
+    assert _mx4.close(ctx.mx4_matmul(w, q)[:, last].double().cpu().numpy(), want, error, "f32").all()
+    assert _mx4.close(ctx.mx4_linear(w, x)[:, last].double().cpu().numpy(), want, error, "f32").all()
+    rows = 600000
+    values = ctx.mx4_dequant(w, first_row=n - rows, rows=rows)
+    assert torch.equal(values[-300:].double().cpu(), torch.from_numpy(w64).half().double())
+    back = ctx.mx4_quantize(values)
+    assert torch.equal(ctx.mx4_dequant(back, first_row=rows - 300, rows=300), values[-300:])
+    del w, values, back
+    torch.cuda.empty_cache()
+    # many rows of x: results past 4 GB
+    w = tensor(*random_codes(70000, 64, 1, -2, 2))
+    x = tensor(*random_codes(20000, 64, 2, -2, 2))
+    y = ctx.mx4_matmul(w, x)
+    rows64, cols64 = _mx4.values(x.codes[-5:].cpu().numpy(), x.scales[:, -5:].contiguous().cpu().numpy()), \
+        _mx4.values(w.codes[-200:].cpu().numpy(), w.scales[:, -200:].contiguous().cpu().numpy())
+    assert np.array_equal(y[-5:, -200:].cpu().numpy(), (rows64 @ cols64.T).astype(np.float32))

@@ -65,13 +65,14 @@ GOOD = {
 WRONG = [
     ("aotx_mx4_quantize", dict(x=0)), ("aotx_mx4_quantize", dict(x=P + 1)), ("aotx_mx4_quantize", dict(x=P + 2, x_dtype=F32)),
     ("aotx_mx4_quantize", dict(x_dtype=3)), ("aotx_mx4_quantize", dict(ldx=63)), ("aotx_mx4_quantize", dict(k=0)),
+    ("aotx_mx4_quantize", dict(k=(1 << 24) + 32, ldx=1 << 25)),
     ("aotx_mx4_quantize", dict(k=48, ldx=48)), ("aotx_mx4_quantize", dict(rows=5)), ("aotx_mx4_quantize", dict(codes=P + 8)),
     ("aotx_mx4_quantize", dict(codes=0)), ("aotx_mx4_quantize", dict(scales=P + 2)), ("aotx_mx4_quantize", dict(scales=0)),
     ("aotx_mx4_quantize", dict(rows_of=P + 2)), ("aotx_mx4_quantize", dict(rows_dev=P + 1)),
     ("aotx_mx4_dequant", dict(first_row=1)), ("aotx_mx4_dequant", dict(rows=5)), ("aotx_mx4_dequant", dict(out=0)),
     ("aotx_mx4_dequant", dict(out=P + 2, out_dtype=F32)), ("aotx_mx4_dequant", dict(out_dtype=-1)),
     ("aotx_mx4_dequant", dict(k=33)), ("aotx_mx4_dequant", dict(first_row=2 ** 32 - 2)),
-    ("aotx_mx4_matmul", dict(k=40)), ("aotx_mx4_matmul", dict(y_dtype=7)), ("aotx_mx4_matmul", dict(y=0)),
+    ("aotx_mx4_matmul", dict(k=40)), ("aotx_mx4_matmul", dict(k=1 << 25)), ("aotx_mx4_matmul", dict(y_dtype=7)), ("aotx_mx4_matmul", dict(y=0)),
     ("aotx_mx4_matmul", dict(y=P + 2)), ("aotx_mx4_matmul", dict(w_codes=P + 4)), ("aotx_mx4_matmul", dict(x_codes=0)),
     ("aotx_mx4_matmul", dict(x_scales=P + 1)), ("aotx_mx4_matmul", dict(epilogue=3)), ("aotx_mx4_matmul", dict(epilogue=-1)),
     ("aotx_mx4_matmul", dict(epilogue=ADD, y_dtype=F16)), ("aotx_mx4_matmul", dict(epilogue=SWIGLU, n=5)),
@@ -86,6 +87,7 @@ WRONG = [
     ("aotx_mx4_matmul_grouped", dict(offsets=P + 2)), ("aotx_mx4_matmul_grouped", dict(y_rows_of=P + 2)),
     ("aotx_mx4_matmul_grouped", dict(experts=256, n=1 << 24)), ("aotx_mx4_matmul_grouped", dict(y=0)),
     ("aotx_mx4_matmul_grouped", dict(epilogue=SWIGLU, n=3)),
+    ("aotx_mx4_matmul_grouped", dict(rows=1 << 24, n=(1 << 16) + 128)),
 ]
 
 
@@ -201,3 +203,48 @@ def test_plain_form_rounds_as_the_format_says():
     codes, scales = _mx4.quantize(edge)
     assert scales[0, :, 0].tolist() == [0, 252, 0]
     assert _mx4.values(codes, scales)[:, 0].tolist() == [0.0, 6 * 2.0 ** 125, 2.0 ** -126]
+
+
+CALLS = {"aotx_mx4_quantize": (None, 0, 0, 1, 4, 64, 64, 0, 4, 0, 0, 0),
+         "aotx_mx4_dequant": (None, 0, 0, 0, 4, 64, 0, 4, 0, 1),
+         "aotx_mx4_matmul": (None, 0, 0, 0, 4, 64, 0, 0, 4, 0, 0, 0, 0),
+         "aotx_mx4_linear": (None, 0, 0, 0, 4, 64, 0, 1, 64, 4, 0, 0, 0, 0, 0, 0),
+         "aotx_mx4_moe_order": (None, 0, 0, 4, 0, 2, 8, 0, 0, 0),
+         "aotx_mx4_matmul_grouped": (None, 0, 0, 0, 2, 4, 64, 0, 0, 4, 0, 0, 4, 0, 0, 0)}
+
+
+@pytest.mark.parametrize("name", sorted(CALLS))
+def test_the_package_calls_the_library_as_ctypes_does(lib, name):
+    call, good = library.native_call(lib, name), CALLS[name]
+    assert call(*good) == getattr(lib, name)(*good) != 0      # no context
+    for wrong in (good[:-1], good + (0,), (1.5,) + good[1:], ("x",) + good[1:]):
+        with pytest.raises(TypeError):
+            call(*wrong)
+    for i, kind in enumerate(getattr(lib, name).argtypes):
+        one = good[:i] + (None,) + good[i + 1:]
+        if kind is C.c_void_p:
+            assert call(*one) != 0
+        else:
+            with pytest.raises(TypeError):
+                call(*one)
+
+
+def test_every_argument_arrives_in_its_place():
+    for name in CALLS:
+        kinds = getattr(library.load_library(), name).argtypes
+        seen = []
+        answer = C.CFUNCTYPE(C.c_int, *kinds)(lambda *args: seen.append(args) or 7)
+        stub = type("Library", (), {name: answer})
+        wide = (C.c_void_p, C.c_uint64, C.c_size_t)
+        sent = tuple(0x7F1234567000 + i if kind in wide else 100 + i for i, kind in enumerate(kinds))
+        assert library.native_call(stub, name)(*sent) == 7
+        assert seen == [sent]
+
+
+def test_counted_stores_of_four_words_are_acquired_at_cluster_scope():
+    """(What tests/test_counted_stores.py holds of the stores of one word.)"""
+    with open(os.path.join(builder.CSRC, "mx4_product.cu")) as f:
+        code = re.sub(r"//[^\n]*", "", f.read())
+    counted = re.findall(r"store_counted_v4\([^;]*mapa_shared\((\w+), \w+\)\);", code)
+    assert counted == ["exchanged"] and code.count("store_counted_v4(") == 1
+    assert set(re.findall(r"(mbar_\w*(?:wait|test)\w*)\(\s*exchanged\b", code)) == {"mbar_wait_counted"}
