@@ -50,7 +50,7 @@ constexpr uint32_t kMxFewSteps = 8;
 constexpr uint32_t kMxPairTok = 192;        // rows of x per tile of a pair of blocks, at most: two accumulators beside the scales
 constexpr uint32_t kMxTwoTok = 64;          // rows of x per tile where two blocks share an SM, at most
 constexpr uint32_t kMxTwoClusterTok = 32;   // and where they are a cluster's
-constexpr uint32_t kMxPairFrom = 257;       // rows of x that pairs take, at least
+constexpr uint32_t kMxPairFrom = 65;        // rows of x that pairs take, at least
 // Tiles of a product that is multiplied by clusters, at most: as many clusters of each size as the GPU runs at the same time.
 constexpr uint32_t kMxClustersOf8 = 12;
 constexpr uint32_t kMxClustersOf4 = 32;
@@ -424,30 +424,57 @@ __device__ __forceinline__ float mx_gated(float gate, float up)
     return gate * rcp_approx(1.0f + ex2_approx(gate * -1.4426950408889634f)) * up;
 }
 
-// 16 rows of x (v: this lane's row of w for each) to y, rows `first` and up below `end`; `row_y`: lane i's is the row of y of row i.
-// They are turned round in the warp's own shared memory and written 16 bytes a lane.  GATED: neighbouring lanes hold gate
+// Where a storing warp's columns of a tile go in y, as one of its lanes needs it: `y` is at the lane's 16 bytes of row 0 (wide) or at
+// its column.
+template <typename YT>
+struct MxOut {
+    YT *y;
+    uint32_t ldy;
+    bool in;                       // the lane has columns of the tile
+    bool wide, adds;
+};
+
+template <typename YT, bool GATED>
+__device__ __forceinline__ MxOut<YT> mx_out(const MxArgs &args, uint32_t lane, uint32_t first_col, uint32_t columns)
+{
+    constexpr uint32_t kPiece = 16u / sizeof(YT);
+    constexpr uint32_t kLanesPerRow = (GATED ? 16u : 32u) / kPiece;
+    MxOut<YT> out;
+    out.ldy = args.ldy;
+    out.wide = args.wide != 0u;
+    out.adds = !GATED && sizeof(YT) == 4 && args.epilogue == kEpilogueAdd;
+    const uint32_t column = out.wide ? lane % kLanesPerRow * kPiece : lane;
+    out.in = column < columns;
+    out.y = static_cast<YT *>(args.y) + first_col + column;
+    return out;
+}
+
+// 16 rows of x (v: this lane's row of w for each) to y; lane i's row_y is the row of y of row i, 0xFFFFFFFF for none.  They are
+// turned round in the warp's own shared memory and written 16 bytes a lane.  GATED: neighbouring lanes hold gate
 // and up of a column (arithmetic of cuda/model/norm.cu:92-105); of two rows of x the even lane forms the first's value and
 // the odd lane the second's.
 template <typename YT, bool GATED>
-__device__ __forceinline__ void mx_store(const MxArgs &args, uint32_t stage, uint32_t lane, uint32_t first_col, uint32_t columns,
-                                         uint32_t row_y, const uint32_t (&v)[16])
+__device__ __forceinline__ void mx_store(const MxOut<YT> &out, uint32_t stage, uint32_t lane, uint32_t row_y, const uint32_t (&v)[16])
 {
-    constexpr uint32_t kColumns = GATED ? 16u : 32u;
-    constexpr uint32_t kRowBytes = kColumns * sizeof(YT);
-    constexpr uint32_t kPiece = 16u / sizeof(YT);
+    constexpr uint32_t kRowBytes = (GATED ? 16u : 32u) * sizeof(YT);
     constexpr uint32_t kLanesPerRow = kRowBytes / 16u;
     constexpr uint32_t kRowsPerStep = 32u / kLanesPerRow;
-    auto put = [&](uint32_t row, uint32_t column, float value) {
+    constexpr uint32_t kSteps = 16u / kRowsPerStep;
+    // (the rows that this lane writes are known before anything is waited for)
+    uint32_t row[kSteps];
+#pragma unroll
+    for (uint32_t step = 0; step < kSteps; ++step) {
+        row[step] = __shfl_sync(0xFFFFFFFFu, row_y, step * kRowsPerStep + lane / kLanesPerRow);
+    }
+    auto put = [&](uint32_t at_row, uint32_t column, float value) {
         if (sizeof(YT) == 4) {
-            st_shared_b32(stage + row * kRowBytes + column * 4u, __float_as_uint(value));
+            st_shared_b32(stage + at_row * kRowBytes + column * 4u, __float_as_uint(value));
         } else {
-            st_shared_b16(stage + row * kRowBytes + column * 2u, out_bits<YT>(value));
+            st_shared_b16(stage + at_row * kRowBytes + column * 2u, out_bits<YT>(value));
         }
     };
     __syncwarp();                  // the rows before these are out of it
     if (GATED) {
-        // (exchanges, then arithmetic, then stores: each of the three keeps its place in the program, and a value at a time
-        // they wait for each other, 600 cycles for the 16 rows instead of 250)
         const bool odd = (lane & 1u) != 0u;
         float got[8], value[8];
 #pragma unroll
@@ -470,25 +497,20 @@ __device__ __forceinline__ void mx_store(const MxArgs &args, uint32_t stage, uin
         }
     }
     __syncwarp();
-    const bool adds = !GATED && sizeof(YT) == 4 && args.epilogue == kEpilogueAdd;
-    if (args.wide != 0u) {
-        constexpr uint32_t kSteps = 16u / kRowsPerStep;
-        const uint32_t part = lane % kLanesPerRow;
+    if (out.wide) {
         uint4 piece[kSteps];
-        YT *at[kSteps];
 #pragma unroll
         for (uint32_t step = 0; step < kSteps; ++step) {
-            const uint32_t local = step * kRowsPerStep + lane / kLanesPerRow;
-            const uint32_t row = __shfl_sync(0xFFFFFFFFu, row_y, local);
-            ld_shared_v4(stage + local * kRowBytes + part * 16u, piece[step].x, piece[step].y, piece[step].z, piece[step].w);
-            at[step] = row != 0xFFFFFFFFu && part * kPiece < columns
-                ? static_cast<YT *>(args.y) + (size_t)row * args.ldy + first_col + part * kPiece : nullptr;
+            ld_shared_v4(stage + step * 512u + lane * 16u, piece[step].x, piece[step].y, piece[step].z, piece[step].w);
         }
-        if (adds) {
+        if (out.adds) {
             float4 before[kSteps];
 #pragma unroll
             for (uint32_t step = 0; step < kSteps; ++step) {
-                before[step] = at[step] != nullptr ? *reinterpret_cast<const float4 *>(at[step]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                before[step] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (out.in && row[step] != 0xFFFFFFFFu) {
+                    before[step] = *reinterpret_cast<const float4 *>(out.y + (size_t)row[step] * out.ldy);
+                }
             }
 #pragma unroll
             for (uint32_t step = 0; step < kSteps; ++step) {
@@ -500,22 +522,22 @@ __device__ __forceinline__ void mx_store(const MxArgs &args, uint32_t stage, uin
         }
 #pragma unroll
         for (uint32_t step = 0; step < kSteps; ++step) {
-            if (at[step] != nullptr) {
-                *reinterpret_cast<uint4 *>(at[step]) = piece[step];
+            if (out.in && row[step] != 0xFFFFFFFFu) {
+                *reinterpret_cast<uint4 *>(out.y + (size_t)row[step] * out.ldy) = piece[step];
             }
         }
     } else {
         // rows of y off the boundary: a value a lane
 #pragma unroll 4
         for (uint32_t i = 0; i < 16u; ++i) {
-            const uint32_t row = __shfl_sync(0xFFFFFFFFu, row_y, i);
-            if (row == 0xFFFFFFFFu || lane >= columns) {
+            const uint32_t to = __shfl_sync(0xFFFFFFFFu, row_y, i);
+            if (to == 0xFFFFFFFFu || !out.in) {
                 continue;
             }
-            YT *at = static_cast<YT *>(args.y) + (size_t)row * args.ldy + first_col + lane;
+            YT *at = out.y + (size_t)to * out.ldy;
             if (sizeof(YT) == 4) {
                 const float value = ld_shared_f32(stage + i * kRowBytes + lane * 4u);
-                *reinterpret_cast<float *>(at) = adds ? *reinterpret_cast<float *>(at) + value : value;
+                *reinterpret_cast<float *>(at) = out.adds ? *reinterpret_cast<float *>(at) + value : value;
             } else {
                 *reinterpret_cast<unsigned short *>(at) = ld_shared_u16(stage + i * kRowBytes + lane * 2u);
             }
@@ -982,7 +1004,6 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 uint32_t row_y = 0xFFFFFFFFu;
                 if (lane < 16u && row_x < last_row) {
                     row_y = args.y_rows_of != nullptr ? args.y_rows_of[row_x] : row_x;
-                    row_y = row_y < args.y_rows ? row_y : 0xFFFFFFFFu;
                 }
                 return row_y;
             };
@@ -1007,7 +1028,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             const uint32_t j0 = tile.row0 + half * kMxRows + quarter;
             const uint32_t width = args.n > j0 ? (args.n - j0 < 32u ? args.n - j0 : 32u) : 0u;
             const uint32_t first_col = GATED ? j0 / 2u : j0;
-            const uint32_t columns = GATED ? width / 2u : width;
+            const MxOut<YT> out = mx_out<YT, GATED>(args, lane, first_col, GATED ? width / 2u : width);
             if (clusters) {
                 // One piece per block: each column's sums go to the block of the cluster that adds them up.
                 for (uint32_t c0 = c_first; c0 < tile.rows; c0 += kTurn) {
@@ -1053,20 +1074,20 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     }
                     const uint32_t row_x = tile.first + rank * args.share + c0 + lane;
                     const bool stores = lane < 16u && c0 + lane < here && row_x < last_row;
-                    mx_store<YT, GATED>(args, stage, lane, first_col, columns, stores ? row_x : 0xFFFFFFFFu, v);
+                    mx_store<YT, GATED>(out, stage, lane, stores ? row_x : 0xFFFFFFFFu, v);
                 }
                 break;
             }
             if (mine.from != 0u) {
                 // Another block owns the tile: its sums go to the scratch.
-                float *out = args.partial + blockIdx.x * args.tile_floats + quarter + lane;
+                float *left = args.partial + blockIdx.x * args.tile_floats + quarter + lane;
                 for (uint32_t c0 = c_first; c0 < tile.rows; c0 += kTurn) {
                     uint32_t v[16];
                     tmem_ld_32x16(sums + c0, v);
                     tmem_ld_wait();
 #pragma unroll
                     for (uint32_t i = 0; i < 16u; ++i) {
-                        __stcg(out + (size_t)(c0 + i) * kMxRows, __uint_as_float(v[i]));
+                        __stcg(left + (size_t)(c0 + i) * kMxRows, __uint_as_float(v[i]));
                     }
                 }
                 release();
@@ -1096,7 +1117,8 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 release();
             }
             for (uint32_t c0 = c_first; c0 < tile.rows; c0 += kTurn) {
-                const uint32_t row_y = next_row;
+                // (looked at here only: the load has had the last rows' time)
+                const uint32_t row_y = next_row < args.y_rows ? next_row : 0xFFFFFFFFu;
                 next_row = row_of(c0 + kTurn);
                 uint32_t v[16];
                 tmem_ld_32x16(sums + c0, v);
@@ -1108,7 +1130,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     mx_add_partials<FORM == kMxTwo ? 1u : 3u>(v, args.partial + (blockIdx.x + kBlocks) * args.tile_floats + (size_t)c0 * kMxRows + quarter + lane,
                                     kBlocks * args.tile_floats, others);
                 }
-                mx_store<YT, GATED>(args, stage, lane, first_col, columns, row_y, v);
+                mx_store<YT, GATED>(out, stage, lane, row_y, v);
             }
             __syncwarp();
             for (uint32_t o = lane; o < others; o += 32u) {
@@ -1268,9 +1290,11 @@ static MxPlan plan_of(const Mx4Product &p, uint32_t sms, bool quantises)
     // Many rows of x, and tiles for every pair: 256 rows of w by up to 192 of x (what two blocks multiply is a multiple of 32).
     if (!quantises && typical >= kMxPairFrom) {
         const uint32_t parts = (typical + kMxPairTok - 1u) / kMxPairTok;
-        if ((unsigned long long)parts * row_tiles_of(p.n, kMxPair) * p.experts >= sms / 2u) {
+        const uint32_t ntok = up_to((typical + parts - 1u) / parts, 32u);
+        if ((unsigned long long)parts * row_tiles_of(p.n, kMxPair) * p.experts >= sms / 2u
+            && (by_expert || parts == 1u || (parts * ntok - typical) * 6u <= typical)) {
             plan.form = kMxPair;
-            plan.ntok = up_to((typical + parts - 1u) / parts, 32u);
+            plan.ntok = ntok;
             deal(plan, tok_tiles() * row_tiles_of(p.n, kMxPair), steps_of(p.k, kMxPair), sms / 2u);
             plan.grid *= 2u;
             return plan;
@@ -1282,7 +1306,7 @@ static MxPlan plan_of(const Mx4Product &p, uint32_t sms, bool quantises)
     const uint32_t row_tiles = row_tiles_of(p.n, kMxOne);
     const uint32_t steps = steps_of(p.k, kMxOne);
     if (by_expert && typical <= kMxClusterTok / 2u) {
-        plan.ntok = up_to(2u * typical, 32u);
+        plan.ntok = up_to(typical > 32u ? typical : 2u * typical < 32u ? 2u * typical : 32u, 16u);
     } else {
         uint32_t parts = (typical + kMxMaxTok - 1u) / kMxMaxTok;
         const uint32_t narrow = (p.m + kMxClusterTok - 1u) / kMxClusterTok;
@@ -1295,9 +1319,9 @@ static MxPlan plan_of(const Mx4Product &p, uint32_t sms, bool quantises)
     // Few tiles, and the host knows how many: clusters that share a tile, else a tile a block.
     if (!by_expert && (p.m_dev == nullptr || tok_tiles() == 1ull) && plan.ntok <= kMxClusterTok) {
         for (uint32_t c = 8u; c >= 2u; c >>= 1) {
-            if (tiles <= (c == 8u ? kMxClustersOf8 : c == 4u ? kMxClustersOf4 : kMxClustersOf2)
-                && steps >= (c == 2u ? 2u : c * kMxClusterSteps)) {
-                plan.form = c >= 4u && plan.ntok <= kMxTwoClusterTok ? kMxTwo : kMxOne;
+            const uint32_t runs = c == 8u ? kMxClustersOf8 : c == 4u ? kMxClustersOf4 : kMxClustersOf2;
+            if (tiles <= (plan.ntok <= kMxTwoClusterTok ? 2u * runs : runs) && steps >= (c == 2u ? 2u : c * kMxClusterSteps)) {
+                plan.form = plan.ntok <= kMxTwoClusterTok ? kMxTwo : kMxOne;
                 plan.cluster = c;
                 plan.grid = (uint32_t)tiles * c;
                 return plan;
