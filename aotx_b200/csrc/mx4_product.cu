@@ -1287,8 +1287,11 @@ static MxPlan plan_of(const Mx4Product &p, uint32_t sms, bool quantises)
         return by_expert ? (unsigned long long)p.m / plan.ntok + (p.experts < p.m ? p.experts : p.m)
                          : ((unsigned long long)p.m + plan.ntok - 1u) / plan.ntok;
     };
-    // Many rows of x, and tiles for every pair: 256 rows of w by up to 192 of x (what two blocks multiply is a multiple of 32).
-    if (!quantises && typical >= kMxPairFrom) {
+    // Many rows of x, more tiles than blocks and tiles for every pair: 256 rows of w by up to 192 of x (what two blocks multiply is a
+    // multiple of 32).
+    const uint32_t row_tiles = row_tiles_of(p.n, kMxOne);
+    const bool one_each = !by_expert && (unsigned long long)((p.m + kMxMaxTok - 1u) / kMxMaxTok) * row_tiles <= sms;
+    if (!quantises && !one_each && typical >= kMxPairFrom) {
         const uint32_t parts = (typical + kMxPairTok - 1u) / kMxPairTok;
         const uint32_t ntok = up_to((typical + parts - 1u) / parts, 32u);
         if ((unsigned long long)parts * row_tiles_of(p.n, kMxPair) * p.experts >= sms / 2u
@@ -1303,22 +1306,29 @@ static MxPlan plan_of(const Mx4Product &p, uint32_t sms, bool quantises)
     // Rows of x per tile: equal parts of at most 256, or of 128 where the tiles are few enough for clusters (whose exchange
     // takes the shared memory of wider ones).  By expert, twice what one has on average, so that most need one tile and their
     // weights are read once.
-    const uint32_t row_tiles = row_tiles_of(p.n, kMxOne);
     const uint32_t steps = steps_of(p.k, kMxOne);
     if (by_expert && typical <= kMxClusterTok / 2u) {
         plan.ntok = up_to(typical > 32u ? typical : 2u * typical < 32u ? 2u * typical : 32u, 16u);
     } else {
         uint32_t parts = (typical + kMxMaxTok - 1u) / kMxMaxTok;
-        const uint32_t narrow = (p.m + kMxClusterTok - 1u) / kMxClusterTok;
-        if (!by_expert && (unsigned long long)narrow * row_tiles <= kMxClustersOf2) {
-            parts = narrow;
+        if (!by_expert) {
+            const uint32_t most = (p.m + kMxTwoClusterTok - 1u) / kMxTwoClusterTok;
+            const uint32_t room = sms / row_tiles < most ? sms / row_tiles : most;
+            parts = room > parts ? room : parts;
+            for (uint32_t tok = kMxTwoClusterTok; tok <= kMxClusterTok; tok *= 2u) {
+                const uint32_t narrow = (p.m + tok - 1u) / tok;
+                if ((unsigned long long)narrow * row_tiles <= kMxClustersOf2) {
+                    parts = narrow;
+                    break;
+                }
+            }
         }
         plan.ntok = up_to((typical + parts - 1u) / parts, 16u);
     }
     const unsigned long long tiles = tok_tiles() * row_tiles;
     // Few tiles, and the host knows how many: clusters that share a tile, else a tile a block.
-    if (!by_expert && (p.m_dev == nullptr || tok_tiles() == 1ull) && plan.ntok <= kMxClusterTok) {
-        for (uint32_t c = 8u; c >= 2u; c >>= 1) {
+    if (!by_expert && (p.m_dev == nullptr || tok_tiles() == 1ull)) {
+        for (uint32_t c = 8u; c >= 2u && plan.ntok <= kMxClusterTok; c >>= 1) {
             const uint32_t runs = c == 8u ? kMxClustersOf8 : c == 4u ? kMxClustersOf4 : kMxClustersOf2;
             if (tiles <= (plan.ntok <= kMxTwoClusterTok ? 2u * runs : runs) && steps >= (c == 2u ? 2u : c * kMxClusterSteps)) {
                 plan.form = plan.ntok <= kMxTwoClusterTok ? kMxTwo : kMxOne;
