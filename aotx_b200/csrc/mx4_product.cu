@@ -545,32 +545,23 @@ __device__ __forceinline__ void mx_store(const MxOut<YT> &out, uint32_t stage, u
     }
 }
 
-// What `others` blocks left of one piece (16 rows of x by 32 rows of w, a slot every `stride` floats), added in their order;
-// the values of TOGETHER blocks are on their way at a time.
-template <uint32_t TOGETHER>
-__device__ __forceinline__ void mx_add_partials(uint32_t (&v)[16], const float *slots, unsigned long long stride, uint32_t others)
+// What another block left of 16 rows of x by this lane's row of w: four rows of x side by side, [row of x / 4][row of w][row of x % 4].
+__device__ __forceinline__ void mx_fetch_partial(float4 (&part)[4], const float4 *slot)
 {
-#pragma unroll 1
-    for (uint32_t o = 0; o < others; o += TOGETHER) {
-        float more[TOGETHER][16];
 #pragma unroll
-        for (uint32_t j = 0; j < TOGETHER; ++j) {
-            if (o + j < others) {
+    for (uint32_t i = 0; i < 4u; ++i) {
+        part[i] = __ldcg(slot + i * kMxRows);
+    }
+}
+
+__device__ __forceinline__ void mx_add_partial(uint32_t (&v)[16], const float4 (&part)[4])
+{
 #pragma unroll
-                for (uint32_t i = 0; i < 16u; ++i) {
-                    more[j][i] = __ldcg(slots + (o + j) * stride + i * kMxRows);
-                }
-            }
-        }
-#pragma unroll
-        for (uint32_t j = 0; j < TOGETHER; ++j) {
-            if (o + j < others) {
-#pragma unroll
-                for (uint32_t i = 0; i < 16u; ++i) {
-                    v[i] = __float_as_uint(__uint_as_float(v[i]) + more[j][i]);
-                }
-            }
-        }
+    for (uint32_t i = 0; i < 4u; ++i) {
+        v[4u * i] = __float_as_uint(__uint_as_float(v[4u * i]) + part[i].x);
+        v[4u * i + 1u] = __float_as_uint(__uint_as_float(v[4u * i + 1u]) + part[i].y);
+        v[4u * i + 2u] = __float_as_uint(__uint_as_float(v[4u * i + 2u]) + part[i].z);
+        v[4u * i + 3u] = __float_as_uint(__uint_as_float(v[4u * i + 3u]) + part[i].w);
     }
 }
 
@@ -1008,6 +999,31 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 return row_y;
             };
             uint32_t next_row = row_of(c_first);
+            // The blocks behind this one that hold the rest of its depth; the first one's sums come while this one's are waited for and
+            // stored (a block to an SM: two have no registers for that).
+            constexpr bool kAhead = FORM != kMxTwo;
+            auto slot_of = [&](uint32_t o) {
+                return reinterpret_cast<const float4 *>(args.partial + (blockIdx.x + (1u + o) * kBlocks) * args.tile_floats) + quarter + lane;
+            };
+            float4 ahead[4];
+            uint32_t others = 0u;
+            if (!clusters && mine.from == 0u && mine.to < steps) {
+                const unsigned long long tile_end = (unsigned long long)(mine.tile + 1u) * steps;
+                while (mx_run_begin(worker + others + 1u, workers, units) < tile_end) {
+                    ++others;
+                }
+                bool there = true;
+                for (uint32_t o = lane; o < others; o += 32u) {
+                    there = there && mx_wait_flag(args.flags + (blockIdx.x + (1u + o) * kBlocks) * kFlagWords + warp, &abort_flag, args.status);
+                }
+                if (!__all_sync(0xFFFFFFFFu, there)) {
+                    break;
+                }
+                __syncwarp();
+                if (kAhead) {
+                    mx_fetch_partial(ahead, slot_of(0u) + c_first / 4u * kMxRows);
+                }
+            }
             if (!mbar_wait_hot(summed(ring.at), ring.parity, &abort_flag, args.status)) {
                 break;
             }
@@ -1080,14 +1096,16 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             }
             if (mine.from != 0u) {
                 // Another block owns the tile: its sums go to the scratch.
-                float *left = args.partial + blockIdx.x * args.tile_floats + quarter + lane;
+                float4 *left = reinterpret_cast<float4 *>(args.partial + blockIdx.x * args.tile_floats) + quarter + lane;
                 for (uint32_t c0 = c_first; c0 < tile.rows; c0 += kTurn) {
                     uint32_t v[16];
                     tmem_ld_32x16(sums + c0, v);
                     tmem_ld_wait();
 #pragma unroll
-                    for (uint32_t i = 0; i < 16u; ++i) {
-                        __stcg(left + (size_t)(c0 + i) * kMxRows, __uint_as_float(v[i]));
+                    for (uint32_t i = 0; i < 4u; ++i) {
+                        __stcg(left + (c0 / 4u + i) * kMxRows,
+                               make_float4(__uint_as_float(v[4u * i]), __uint_as_float(v[4u * i + 1u]),
+                                           __uint_as_float(v[4u * i + 2u]), __uint_as_float(v[4u * i + 3u])));
                     }
                 }
                 release();
@@ -1096,22 +1114,6 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     st_release_gpu(args.flags + blockIdx.x * kFlagWords + warp, 1u);
                 }
                 continue;
-            }
-            // The blocks behind this one that hold the rest of its depth.
-            uint32_t others = 0u;
-            if (mine.to < steps) {
-                const unsigned long long tile_end = (unsigned long long)(mine.tile + 1u) * steps;
-                while (mx_run_begin(worker + others + 1u, workers, units) < tile_end) {
-                    ++others;
-                }
-                bool there = true;
-                for (uint32_t o = lane; o < others; o += 32u) {
-                    there = there && mx_wait_flag(args.flags + (blockIdx.x + (1u + o) * kBlocks) * kFlagWords + warp, &abort_flag, args.status);
-                }
-                if (!__all_sync(0xFFFFFFFFu, there)) {
-                    break;
-                }
-                __syncwarp();
             }
             if (c_first >= tile.rows) {
                 release();
@@ -1127,8 +1129,18 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     release();
                 }
                 if (others != 0u) {
-                    mx_add_partials<FORM == kMxTwo ? 1u : 3u>(v, args.partial + (blockIdx.x + kBlocks) * args.tile_floats + (size_t)c0 * kMxRows + quarter + lane,
-                                    kBlocks * args.tile_floats, others);
+                    if (kAhead) {
+                        mx_add_partial(v, ahead);
+                    }
+#pragma unroll 1
+                    for (uint32_t o = kAhead ? 1u : 0u; o < others; ++o) {
+                        float4 more[4];
+                        mx_fetch_partial(more, slot_of(o) + c0 / 4u * kMxRows);
+                        mx_add_partial(v, more);
+                    }
+                    if (kAhead && c0 + kTurn < tile.rows) {
+                        mx_fetch_partial(ahead, slot_of(0u) + (c0 + kTurn) / 4u * kMxRows);
+                    }
                 }
                 mx_store<YT, GATED>(out, stage, lane, row_y, v);
             }
