@@ -43,6 +43,7 @@ constexpr uint32_t kMxMaxTok = 256;         // rows of x per tile, at most
 constexpr uint32_t kMxStageK = 256;         // values of a row per part of a stage: 128 bytes, a row of the swizzle
 constexpr uint32_t kMxStageBytes = kMxStageK / 2;
 constexpr uint32_t kMxMaxStages = 12;
+constexpr uint32_t kMxMaxScales = 16;       // stages whose scales are on their way
 constexpr uint32_t kMxMaxSlots = 9;         // stages of x that stay
 constexpr uint32_t kMxScaleBlock = 512;     // scales of 128 rows and 128 values
 constexpr uint32_t kMxEpilogueStage = 16u * 32u * 4u;  // per storing warp
@@ -63,7 +64,7 @@ constexpr uint32_t kMxClusterTok = 128;     // and rows of x per tile
 // (16 stages), 1 row, 11.4 against 10.0.
 constexpr uint32_t kMxFusedRows = 16;
 constexpr uint32_t kMxFusedWork = 32;       // rows times stages
-constexpr uint32_t kMxBars = 2 * kMxMaxStages + 5 + kMxMaxSlots;
+constexpr uint32_t kMxBars = 2 * kMxMaxStages + 5 + kMxMaxSlots + 2 * kMxMaxScales;
 __host__ __device__ constexpr uint32_t mx_smem(MxForm form)
 {
     return (form == kMxTwo ? 109u : 223u) * 1024u;
@@ -90,7 +91,8 @@ struct MxArgs {
     unsigned int epilogue;
     unsigned int *status;
     uint32_t ntok;                 // rows of x per tile, a multiple of 16
-    uint32_t stages, stage_bytes;
+    uint32_t stages, stage_bytes;  // of codes
+    uint32_t scale_slots, scale_bytes;
     uint32_t tmem_columns, accumulators;
     uint32_t scale_places;         // stages whose scales are in tensor memory at a time
     uint32_t weights_late;
@@ -604,20 +606,27 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const uint32_t worker = PAIR ? blockIdx.x / 2u : blockIdx.x;
     uint32_t workers = PAIR ? gridDim.x / 2u : gridDim.x;
     const uint32_t x_rows = PAIR ? args.ntok / 2u : args.ntok;     // of a tile, in this block's shared memory
-    // a stage: codes of w, scales of w, codes of x, scales of x; x that stays has places of its own behind the ring
-    const uint32_t w_scales_at = kParts * kMxRows * kMxStageBytes;
-    const uint32_t x_codes_at = w_scales_at + 2u * kParts * kMxScaleBlock;
-    const uint32_t x_scales_at = x_codes_at + kParts * x_rows * kMxStageBytes;
-    const uint32_t place = base + stages * args.stage_bytes;
+    // A stage: codes of w, codes of x; its scales, of w and of x, lie behind all stages.  They come by other copies than the codes and
+    // take longer: of a pair, which has room for few stages, they have a ring and barriers of their own and more of them are on their
+    // way (28672 x 4096, 2048 rows, 116.9 -> 113.0 us; a single block loses by it, 4096 x 4096, 1 row, 6.3 -> 6.5 us: another wait a
+    // stage).  x that stays has places behind both.
+    constexpr bool kApart = PAIR;
+    const uint32_t x_codes_at = kParts * kMxRows * kMxStageBytes;
+    const uint32_t scales = base + stages * args.stage_bytes;
+    const uint32_t scale_slots = args.scale_slots;
+    const uint32_t x_scales_at = 2u * kParts * kMxScaleBlock;
+    const uint32_t place = scales + scale_slots * args.scale_bytes;
     const uint32_t slot_bytes = args.ntok * kMxStageBytes + 2u * x_blocks * kMxScaleBlock;
     const uint32_t tail = base + mx_rings(FORM);
     const uint32_t bars = tail + kStoreWarps * kMxEpilogueStage;
-    auto full = [&](uint32_t s) { return bars + s * 8u; };           // codes and scales are there
+    auto full = [&](uint32_t s) { return bars + s * 8u; };           // codes are there, and scales that are not apart
     auto empty = [&](uint32_t s) { return bars + (kMxMaxStages + s) * 8u; };
     auto summed = [&](uint32_t b) { return bars + (2u * kMxMaxStages + b) * 8u; };
     auto taken = [&](uint32_t b) { return bars + (2u * kMxMaxStages + 2u + b) * 8u; };
     const uint32_t exchanged = bars + (2u * kMxMaxStages + 4u) * 8u;
     const uint32_t x_bars = bars + (2u * kMxMaxStages + 5u) * 8u;
+    auto scaled = [&](uint32_t s) { return kApart ? bars + (kMxBars - 2u * kMxMaxScales + s) * 8u : full(s); };
+    auto used = [&](uint32_t s) { return kApart ? bars + (kMxBars - kMxMaxScales + s) * 8u : empty(s); };
     // a cluster's exchange: per block of it this block's columns, [block][four columns][row of w][column] floats, at the end of the rings
     const uint32_t exchange = tail - (clusters ? args.cluster * args.share * kMxRows * 4u : 0u);
     const uint32_t rank = clusters ? blockIdx.x % args.cluster : 0u;
@@ -635,12 +644,12 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     if (threadIdx.x < kMxBars) {
         const uint32_t i = threadIdx.x;
         uint32_t count = kStoreWarps;                          // taken, and the stages of x that stay
-        if (i < kMxMaxStages) {
-            // the codes and the scales; of a pair the first block's counts the second block's scales as well, and the second
-            // block's counts its scales alone
-            count = PAIR ? (half == 0u ? 2u + 128u : 128u) : 1u + 128u;
-        } else if (i < 2u * kMxMaxStages + 2u || i == 2u * kMxMaxStages + 4u) {
-            count = 1u;                                          // empty, summed, exchanged
+        if (!kApart && i < kMxMaxStages) {
+            count = 1u + 128u;
+        } else if (i < 2u * kMxMaxStages + 2u || i == 2u * kMxMaxStages + 4u || i >= kMxBars - kMxMaxScales) {
+            count = 1u;                                          // full, empty, summed, exchanged, used
+        } else if (i >= kMxBars - 2u * kMxMaxScales) {
+            count = half == 0u ? 128u + 1u : 128u;               // the second block of a pair tells the first of its scales
         } else if (PAIR && i < 2u * kMxMaxStages + 4u) {
             count = 2u * kStoreWarps;
         }
@@ -792,12 +801,12 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     } else if (PAIR && warp == kMmaWarp && half != 0u) {
         // This block's scales are there: told to the first block, whose thread copies them to tensor memory.
         if (elect_one()) {
-            const uint32_t signal = mapa_shared(bars, 0u);
+            const uint32_t signal = mapa_shared(scaled(0u), 0u);
             MxRing ring;
             bool ok = true;
             while (ok && mine.next()) {
-                for (uint32_t step = mine.from; step < mine.to; ++step, ring.next(stages)) {
-                    if (!mbar_wait_hot(full(ring.at), ring.parity, &abort_flag, args.status)) {
+                for (uint32_t step = mine.from; step < mine.to; ++step, ring.next(scale_slots)) {
+                    if (!mbar_wait_hot(scaled(ring.at), ring.parity, &abort_flag, args.status)) {
                         ok = false;
                         break;
                     }
@@ -839,7 +848,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             const uint64_t codes_desc = umma_desc_sw128(0u);
             const uint64_t scale_desc = mx_scale_desc(0u);
             uint32_t it = 0, piece = 0;
-            MxRing ring, slot, sums_ring, scale_place, behind;
+            MxRing ring, slot, sums_ring, scale_place, scale_ring, behind;
             bool ok = true;
             bool ready = false, unused = false, empty_sums = false;
             for (; ok && mine.next(); ++piece, sums_ring.next(args.accumulators)) {
@@ -851,7 +860,8 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 for (uint32_t step = mine.from; step < mine.to; ++step, ++it, slot.next(args.slots),
                               scale_place.next(args.scale_places)) {
                     if (!ready && ((stays && it < args.slots && !mbar_wait_hot(x_bars + slot.at * 8u, 0u, &abort_flag, args.status))
-                                   || !mbar_wait_hot(full(ring.at), ring.parity, &abort_flag, args.status))) {
+                                   || !mbar_wait_hot(full(ring.at), ring.parity, &abort_flag, args.status)
+                                   || (kApart && !mbar_wait_hot(scaled(scale_ring.at), scale_ring.parity, &abort_flag, args.status)))) {
                         ok = false;
                         break;
                     }
@@ -866,8 +876,12 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     // The next stage is asked for now: the answer comes while this one's instructions are issued (a wait takes 200
                     // cycles even where nothing is missing, as much as these).
                     const uint32_t now = ring.at;
+                    const uint32_t now_scales = kApart ? scale_ring.at : now;
                     ring.next(stages);
-                    ready = (!stays || it + 1u >= args.slots) && mbar_test(full(ring.at), ring.parity) != 0u;
+                    scale_ring.next(scale_slots);
+                    ready = (!stays || it + 1u >= args.slots)
+                        && (!kApart || mbar_test(scaled(scale_ring.at), scale_ring.parity) != 0u)
+                        && mbar_test(full(ring.at), ring.parity) != 0u;
                     unused = PAIR && mbar_test(empty(behind.at), behind.parity) != 0u;
                     if (step + 1u == mine.to) {
                         MxRing after = sums_ring;
@@ -880,8 +894,9 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     const uint32_t x_at = stays ? place + slot.at * slot_bytes : at + x_codes_at;
                     const uint32_t w_scales = scales_at + scale_place.at * columns;
                     const uint32_t x_scales = w_scales + kParts * 8u;
-                    const uint64_t w_from = scale_desc | ((at + w_scales_at) >> 4);
-                    const uint64_t x_from = scale_desc | ((x_at + kParts * x_rows * kMxStageBytes) >> 4);
+                    const uint32_t scales_from = scales + now_scales * args.scale_bytes;
+                    const uint64_t w_from = scale_desc | (scales_from >> 4);
+                    const uint64_t x_from = scale_desc | ((stays ? x_at + x_rows * kMxStageBytes : scales_from + x_scales_at) >> 4);
                     // (a block of scales: 128 values of 128 rows)
 #pragma unroll
                     for (uint32_t c = 0; c < 2u * kParts; ++c) {
@@ -907,6 +922,9 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                         }
                     }
                     commit(empty(now));
+                    if (kApart) {
+                        commit(used(now_scales));
+                    }
                 }
                 commit(summed(sums_ring.at));
             }
@@ -918,8 +936,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         }
         const uint32_t t = threadIdx.x - kScaleWarp * 32u;
         const uint32_t cell = (t % 32u) * 16u + (t / 32u) * 4u;
-        // The copies of as many stages as the ring has are on their way together, and count themselves on the stage's barrier:
-        // the weights' scales come from memory.
+        // The copies of as many stages as the ring has are on their way together, and count themselves on the ring's barriers.
         uint32_t it = 0;
         MxRing ring;
         bool ok = true;
@@ -933,16 +950,16 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             const uint32_t *w_from = args.w_scales + (w_in ? (size_t)(2u * kParts * mine.from) * args.w_rows + w_row : 0u);
             const uint32_t *x_from = stays ? nullptr
                 : args.x_scales + (x_in ? (size_t)(2u * kParts * mine.from) * args.x_rows + tile.first + t : 0u);
-            for (uint32_t step = mine.from; step < mine.to; ++step, ++it, ring.next(stages)) {
-                if (it >= stages && !mbar_wait_hot(empty(ring.at), ring.parity ^ 1u, &abort_flag, args.status)) {
+            for (uint32_t step = mine.from; step < mine.to; ++step, ++it, ring.next(scale_slots)) {
+                if (it >= scale_slots && !mbar_wait_hot(used(ring.at), ring.parity ^ 1u, &abort_flag, args.status)) {
                     ok = false;
                     break;
                 }
-                const uint32_t at = base + ring.at * args.stage_bytes + cell;
+                const uint32_t at = scales + ring.at * args.scale_bytes + cell;
 #pragma unroll
                 for (uint32_t c = 0; c < 2u * kParts; ++c) {
                     const bool in = 2u * kParts * step + c < args.chunks;
-                    copy_async_4(at + w_scales_at + c * kMxScaleBlock, w_from, w_in && in ? 4u : 0u);
+                    copy_async_4(at + c * kMxScaleBlock, w_from, w_in && in ? 4u : 0u);
                     w_from += w_in && in ? args.w_rows : 0u;
                     if (!stays) {
                         copy_async_4(at + x_scales_at + c * x_blocks * kMxScaleBlock, x_from, x_in && in ? 4u : 0u);
@@ -953,7 +970,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                         x_from += x_in && in ? args.x_rows : 0u;
                     }
                 }
-                copy_async_arrive(full(ring.at));
+                copy_async_arrive(scaled(ring.at));
             }
         }
         copy_async_wait_all();
@@ -1438,12 +1455,16 @@ cudaError_t launch_mx4_product(cudaStream_t stream, const UmmaScratch &scratch, 
     const uint32_t x_blocks = mx_scale_blocks(args.ntok);
     const uint32_t x_rows = pair ? args.ntok / 2u : args.ntok;
     const uint32_t x_bytes = mx_parts(form) * (x_rows * kMxStageBytes + 2u * x_blocks * kMxScaleBlock);
-    args.stage_bytes = mx_parts(form) * (kMxRows * kMxStageBytes + 2u * kMxScaleBlock) + (args.slots != 0u ? 0u : x_bytes);
+    args.stage_bytes = mx_parts(form) * (kMxRows + (args.slots != 0u ? 0u : x_rows)) * kMxStageBytes;
+    args.scale_bytes = mx_parts(form) * 2u * (1u + (args.slots != 0u ? 0u : x_blocks)) * kMxScaleBlock;
     const uint32_t tile_rows = p.m < args.ntok ? p.m : args.ntok;
     args.share = plan.cluster != 0u ? up_to((tile_rows + plan.cluster - 1u) / plan.cluster, 4u) : 0u;
     const uint32_t exchange = args.cluster * args.share * kMxRows * 4u;
-    const uint32_t fit = (mx_rings(form) - exchange - args.slots * x_bytes) / args.stage_bytes;
+    const uint32_t room = mx_rings(form) - exchange - args.slots * x_bytes;
+    const uint32_t fit = room / (args.stage_bytes + args.scale_bytes);
     args.stages = fit < kMxMaxStages ? fit : kMxMaxStages;
+    const uint32_t scales = pair ? (room - args.stages * args.stage_bytes) / args.scale_bytes : args.stages;
+    args.scale_slots = scales < kMxMaxScales ? scales : kMxMaxScales;
     // Tensor memory: two accumulators where they fit beside scales, and those of as many stages as then fit, two at least (a
     // single block copies a stage's scales without asking for the place: it has one for each).
     const uint32_t stage_columns = mx_parts(form) * 8u * (1u + x_blocks);
