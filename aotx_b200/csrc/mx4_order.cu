@@ -25,8 +25,8 @@ __device__ __forceinline__ void order_load(const uint32_t *ids, uint32_t first, 
     }
 }
 
-// The lanes with the same expert (what a match gives, which takes 350 cycles of the scheduler; a ballot for each of the number's bits
-// 40): e is an expert or 0xFFFFFFFF.
+// The lanes with the same expert (what a match gives, which takes 350 cycles of the scheduler; a ballot for each of the number's
+// bits 40): e is an expert or 0xFFFFFFFF.
 __device__ __forceinline__ uint32_t order_same(uint32_t e, uint32_t bits)
 {
     uint32_t same = __ballot_sync(0xFFFFFFFFu, e != 0xFFFFFFFFu);
@@ -39,11 +39,11 @@ __device__ __forceinline__ uint32_t order_same(uint32_t e, uint32_t bits)
     return same;
 }
 
-// One block; latency bounds it, and the way of scattered words through one SM: so the order is made in shared memory where it fits and
-// goes out in rows (512 tokens of 8 of 128 experts 7.6 us without, ORDER_US with).  Each warp takes a run of the pairs and counts them by expert; then warp by warp of eight
-// experts, a lane for each of the 32 warps, running totals over the warps; running totals over the experts give each warp
-// its first place per expert; then it places its pairs, lanes in order within a step (lanes with the same expert find each
-// other with a match).
+// One block; latency bounds it, and the way of scattered words through one SM: so the order is made in shared memory where it
+// fits and goes out in rows (512 tokens with 8 of 128 experts 6.7 us, without 7.6; 8 tokens 3.4 us).  Each warp takes a run of
+// the pairs and counts them by expert; then warp by warp of eight experts, a lane for each of the 32 warps, running totals over the
+// warps; running totals over the experts give each warp its first place per expert; then it places its pairs, lanes in order
+// within a step (lanes with the same expert find each other by ballots).
 __global__ void __launch_bounds__(kOrderThreads)
 mx4_order_kernel(const uint32_t *ids, uint32_t tokens_max, const uint32_t *tokens_dev, uint32_t used, uint32_t experts,
                  uint32_t *__restrict__ order, uint32_t *__restrict__ token_of, uint32_t *__restrict__ offsets, bool staged)

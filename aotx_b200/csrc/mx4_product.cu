@@ -1,22 +1,36 @@
 // Products of MX4 tensors: y[i][j] = sum_c x[i][c] * w[j][c], plain or grouped by expert.
 //
 // Both operands go to the tensor core as they lie in memory (tcgen05.mma kind::mxf4: E2M1 codes, a power of two per 32
-// values of either operand, float sums).  A block takes 128 rows of w, the MMA's rows, by up to 256 rows of x, its columns:
+// values of either operand, float sums).  A tile is 128 rows of w, the MMA's rows, by up to 256 rows of x, its columns; a step
+// is 256 values of its depth:
 //
-//   * Codes come by bulk tensor copies, 256 values (128 bytes) of each row a stage, in the 128-byte swizzle.
+//   * Codes come by bulk tensor copies, 128 bytes of each row a step, in the 128-byte swizzle.
 //   * Scales come by four warps, a word of four scales (128 values) at a time.  The MMA wants them in tensor memory, row r
 //     of the operand in lane r % 32 of column r / 32, the same in each quarter of the lanes: a block of 512 bytes in
 //     shared memory, 16 bytes per lane, is laid down so by one tcgen05.cp.  The words of successive rows are neighbours in
 //     memory, so rows may start anywhere, as the rows of an expert do.
 //   * One thread issues the copies of the scales and the MMAs behind them (they run in that order).  Each stage has its own
 //     columns of tensor memory for scales, so that nothing is overwritten before its MMAs are done.
-//   * Eight warps store: the sums of 16 rows of x are turned round in shared memory, 16 bytes a lane.
-//   * The grid is at most one block per SM, and the steps of all tiles (a tile by one stage) are dealt to it in equal runs, so
-//     copies go on from tile to tile and every SM streams to the end.  A tile that is cut between blocks belongs to the one
-//     with its first step: the others leave their sums in the context's scratch and raise a flag per warp (a block does so
-//     once, with its first tile, before it waits for anyone), and the owner adds them in the order of the blocks.
+//   * Four or eight warps store: the sums of 16 rows of x are turned round in shared memory, 16 bytes a lane.
 //   * Few rows of x in 16 or 32 bits (mx4_linear) are quantised by the storing warps, which have nothing else to do at first,
 //     straight into the shared memory that the MMA reads, every stage that the block needs once.
+//
+// Few rows of x are bound by w's bytes, and what a launch costs by itself; many by the way of the codes from L2 to shared memory (with
+// all MMAs but a step's first left out, 28672 x 4096 by 2048 rows takes 8 % less).  The forms of the kernel and the ways of dealing
+// the steps of all tiles to blocks follow from that:
+//
+//   * Few tiles: a cluster of 2, 4 or 8 blocks shares one.  Each has a part of its depth; each column's sums go through distributed
+//     shared memory to the block that adds them and stores it.  (1024 x 4096 by 8 rows 4.5 us, a block a tile 7.1 us; 8192 x 4096 7.6
+//     and 8.4.)
+//   * At most a tile a block: blocks have one each.  Rows of x are cut into as many parts as fill the SMs so (8192 x 4096 by 256 rows
+//     10.1 us, 16.8 in one part; 18432 x 4096 by 200 rows 13.0, in equal runs 19.8).
+//   * Else equal runs of steps, so copies go on from tile to tile and every SM streams to the end.  A tile that is cut between
+//     blocks belongs to the one with its first step: the others leave their sums in the context's scratch and raise a flag per warp (a
+//     block does so once, with its first tile, before it waits for anyone), and the owner adds them in the order of the
+//     blocks.
+//   * Two blocks to an SM for few rows of x: one's stores overlap the other's copies.
+//   * A pair of blocks on neighbouring SMs for many: 256 rows of w, each block with its 128 and half of x's rows, so that each code is
+//     read into shared memory half as often.
 #include <cuda.h>
 
 #include "mx4.h"
@@ -47,17 +61,29 @@ constexpr uint32_t kMxMaxScales = 16;       // stages whose scales are on their 
 constexpr uint32_t kMxMaxSlots = 9;         // stages of x that stay
 constexpr uint32_t kMxScaleBlock = 512;     // scales of 128 rows and 128 values
 constexpr uint32_t kMxEpilogueStage = 16u * 32u * 4u;  // per storing warp
+// A run is cut from a tile only if it has as many steps (by expert 4, 8 or 16 differ by less than 2 %).
 constexpr uint32_t kMxFewSteps = 8;
-constexpr uint32_t kMxPairTok = 192;        // rows of x per tile of a pair of blocks, at most: two accumulators beside the scales
-constexpr uint32_t kMxTwoTok = 64;          // rows of x per tile where two blocks share an SM, at most
-constexpr uint32_t kMxTwoClusterTok = 32;   // and where they are a cluster's
-constexpr uint32_t kMxPairFrom = 65;        // rows of x that pairs take, at least
-// Tiles of a product that is multiplied by clusters, at most: as many clusters of each size as the GPU runs at the same time.
+// Rows of x per tile of a pair of blocks, at most: two accumulators beside the scales.  (28672 x 4096 by 300 rows 30.3 us, with 128
+// 34.4; by 2048 rows 118 and 132.)
+constexpr uint32_t kMxPairTok = 192;
+// Rows of x that pairs take, at least.  (19456 x 2560 by 96 rows 10.5 us, single blocks 11.7; 28672 x 4096 by 192 rows 21.6 and 23.7, by
+// 2048 rows 118 and 144; by 48 rows 15.7 and 14.0.  128 experts of 1536 x 2048 with 96 rows each 55 and 64, with 32 the same.)
+constexpr uint32_t kMxPairFrom = 65;
+// Rows of x per tile where two blocks share an SM, at most.  (28672 x 4096 by 8 rows 13.4 us, a block to an SM 14.5; by 64 rows 15.0 and
+// 15.9; 65536 x 4096 by 96 rows 34.3 and 31.7; 128 experts of 1536 x 2048, 64 pairs, 19.6 and 21.8.)
+constexpr uint32_t kMxTwoTok = 64;
+// And where they are a cluster's.  (18432 x 4096 by 1 row 10.7 us, a block to an SM 12.0; by 64 rows 13.3 and 11.1.)
+constexpr uint32_t kMxTwoClusterTok = 32;
+// Tiles of a product that is multiplied by clusters, at most: as many clusters of each size as the GPU runs at the same time, twice as
+// many where two blocks share an SM.  (More wait for the first to end: 4096 x 8192 by 1 row, 32 tiles, by eights 8.5 us, by fours
+// 7.9; 12288 x 4096, 96 tiles, by pairs with a block to an SM 15.4, with two 8.6.)
 constexpr uint32_t kMxClustersOf8 = 12;
 constexpr uint32_t kMxClustersOf4 = 32;
 constexpr uint32_t kMxClustersOf2 = 72;
-constexpr uint32_t kMxClusterSteps = 4;     // steps of a block of a larger cluster, at least
-constexpr uint32_t kMxClusterTok = 128;     // and rows of x per tile
+constexpr uint32_t kMxClusterSteps = 4;     // steps of a block of a larger cluster, at least (2 gain nothing)
+// And rows of x per tile, at most.  Narrower tiles come first where there are clusters for all: less to exchange (512 x 2048 by 128 rows
+// in one part 7.3 us, in two 5.5, in four 4.8).
+constexpr uint32_t kMxClusterTok = 128;
 // What the kernel quantises of x itself: few rows, and few stages of them.  Every block turns the stages that it needs by itself; a launch
 // of its own costs a microsecond more than the product alone.  4096 x 4096 (4 stages a block), 1 row, 6.3 us against 7.3, 8 rows 6.8 against
 // 7.4, 16 rows 9.2 against 7.6; 20000 x 4096 (9 stages), 2 rows, 12.0 against 12.9, 8 rows 14.2 against 13.1; 12288 x 4096
@@ -111,8 +137,8 @@ struct MxArgs {
 };
 
 // Parts of a stage.  A wait, a commit and what else the thread that issues the MMAs does for a stage take it as long as four MMAs of
-// 208 columns: pairs of blocks have two parts to a stage (28672 x 4096, 2048 rows, 125 -> PAIR_US us).  A single block has one, so
-// that few steps can be dealt evenly.
+// 208 columns: pairs of blocks have two parts to a stage (28672 x 4096 by 2048 rows 118 us, with one 129).  A single block has one,
+// so that few steps can be dealt evenly.
 __host__ __device__ constexpr uint32_t mx_parts(MxForm form)
 {
     return form == kMxPair ? 2u : 1u;
@@ -416,7 +442,8 @@ __device__ __forceinline__ void mx_quantize_x(const MxArgs &args, const T *x, ui
 }
 
 // silu(gate) * up.  For a float y as the Q8_0 products form it; for 16 bits by the approximate exponential and reciprocal, which are
-// off by 2^-18 of the result at most for gates from -14 on (2^-15 at -100), against 2^-11 and 2^-8 of the rounding: 6 instructions instead of 20, 16 rows 900 -> GATED_CYCLES cycles.
+// off by 2^-18 of the result at most for gates from -14 on (2^-15 at -100), against 2^-11 and 2^-8 of the rounding: 6 instructions instead
+// of 20 (28672 x 4096 by 2048 rows 119 us, with the exact unit 137; by 8 rows 13.9 and 14.0).
 template <typename YT>
 __device__ __forceinline__ float mx_gated(float gate, float up)
 {
@@ -981,14 +1008,16 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             const uint32_t slots = run < args.slots ? run : args.slots;
             switch (args.x_type) {
             case 0u:
-                mx_quantize_x<float, kStoreWarps>(args, static_cast<const float *>(args.x), place, slot_bytes, x_bars, first_step, slots, steps, valid);
+                mx_quantize_x<float, kStoreWarps>(args, static_cast<const float *>(args.x), place, slot_bytes, x_bars, first_step,
+                    slots, steps, valid);
                 break;
             case 1u:
-                mx_quantize_x<__half, kStoreWarps>(args, static_cast<const __half *>(args.x), place, slot_bytes, x_bars, first_step, slots, steps, valid);
+                mx_quantize_x<__half, kStoreWarps>(args, static_cast<const __half *>(args.x), place, slot_bytes, x_bars, first_step,
+                    slots, steps, valid);
                 break;
             default:
-                mx_quantize_x<__nv_bfloat16, kStoreWarps>(args, static_cast<const __nv_bfloat16 *>(args.x), place, slot_bytes, x_bars, first_step, slots, steps,
-                              valid);
+                mx_quantize_x<__nv_bfloat16, kStoreWarps>(args, static_cast<const __nv_bfloat16 *>(args.x), place, slot_bytes, x_bars, first_step,
+                    slots, steps, valid);
                 break;
             }
         }
@@ -1316,8 +1345,9 @@ static MxPlan plan_of(const Mx4Product &p, uint32_t sms, bool quantises)
         return by_expert ? (unsigned long long)p.m / plan.ntok + (p.experts < p.m ? p.experts : p.m)
                          : ((unsigned long long)p.m + plan.ntok - 1u) / plan.ntok;
     };
-    // Many rows of x, more tiles than blocks and tiles for every pair: 256 rows of w by up to 192 of x (what two blocks multiply is a
-    // multiple of 32).
+    // Many rows of x, more tiles than blocks (18432 x 4096 by 256 rows: a tile a block 14.2 us, pairs 20.4) and tiles for every pair:
+    // 256 rows of w by up to 192 of x.  What two blocks multiply is a multiple of 32 rows of x: not where it would be a sixth more than
+    // there are (28672 x 4096 by 208 rows 26.4 us, single blocks 25.0).
     const uint32_t row_tiles = row_tiles_of(p.n, kMxOne);
     const bool one_each = !by_expert && (unsigned long long)((p.m + kMxMaxTok - 1u) / kMxMaxTok) * row_tiles <= sms;
     if (!quantises && !one_each && typical >= kMxPairFrom) {
@@ -1332,9 +1362,9 @@ static MxPlan plan_of(const Mx4Product &p, uint32_t sms, bool quantises)
             return plan;
         }
     }
-    // Rows of x per tile: equal parts of at most 256, or of 128 where the tiles are few enough for clusters (whose exchange
-    // takes the shared memory of wider ones).  By expert, twice what one has on average, so that most need one tile and their
-    // weights are read once.
+    // Rows of x per tile: equal parts of at most 256, more of them while there is an SM for each tile, or few enough for clusters.  By
+    // expert what one has on average, twice that for few: a wider tile reads weights less often and is stored by fewer blocks (128
+    // experts of 2048 x 768 with 32 rows each, by 32 rows 32.7 us, by 64 34.7; of 1536 x 2048 with 16 each, by 16 43.8, by 32 41.8).
     const uint32_t steps = steps_of(p.k, kMxOne);
     if (by_expert && typical <= kMxClusterTok / 2u) {
         plan.ntok = up_to(typical > 32u ? typical : 2u * typical < 32u ? 2u * typical : 32u, 16u);

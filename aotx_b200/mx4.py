@@ -214,7 +214,8 @@ class Mx4Calls:
         w_codes, w_scales = w._at
         x_codes, x_scales = x._at
         result = self._mx4_matmul_call(self._address, self._stream(), w_codes, w_scales, w.rows, w.k, x_codes, x_scales, x.rows,
-                                       None if m_dev is None else self._mx4_words("m_dev", m_dev, 1), y.data_ptr(), _dtype_code(y.dtype), epilogue)
+                                       None if m_dev is None else self._mx4_words("m_dev", m_dev, 1), y.data_ptr(),
+                                       _dtype_code(y.dtype), epilogue)
         if result != 0:
             self._check(result)
         return y
@@ -239,8 +240,8 @@ class Mx4Calls:
                 raise self._mx4_elsewhere(workspace)
         w_codes, w_scales = w._at
         result = self._mx4_linear_call(self._address, self._stream(), w_codes, w_scales, w.rows, k, x.data_ptr(), code, stride,
-                                       m, None if m_dev is None else self._mx4_words("m_dev", m_dev, 1), y.data_ptr(), _dtype_code(y.dtype), epilogue,
-                                       _pointer(workspace), size)
+                                       m, None if m_dev is None else self._mx4_words("m_dev", m_dev, 1), y.data_ptr(),
+                                       _dtype_code(y.dtype), epilogue, _pointer(workspace), size)
         if result != 0:
             self._check(result)
         return y
