@@ -84,10 +84,10 @@ constexpr uint32_t kMxClusterSteps = 4;     // steps of a block of a larger clus
 // And rows of x per tile, at most.  Narrower tiles come first where there are clusters for all: less to exchange (512 x 2048 by 128 rows
 // in one part 7.3 us, in two 5.5, in four 4.8).
 constexpr uint32_t kMxClusterTok = 128;
-// What the kernel quantises of x itself: few rows, and few stages of them.  Every block turns the stages that it needs by itself; a launch
-// of its own costs a microsecond more than the product alone.  4096 x 4096 (4 stages a block), 1 row, 6.3 us against 7.3, 8 rows 6.8 against
-// 7.4, 16 rows 9.2 against 7.6; 20000 x 4096 (9 stages), 2 rows, 12.0 against 12.9, 8 rows 14.2 against 13.1; 12288 x 4096
-// (16 stages), 1 row, 11.4 against 10.0.
+// What the kernel quantises of x itself: few rows, and few stages of them.  Every block turns the stages that it needs by itself; a
+// launch of its own costs a microsecond more than the product alone.  4096 x 4096 (4 stages a block), 1 row, 6.4 us against 7.3 apart, 8
+// rows 6.9 against 7.4, 16 rows 9.2 against 7.5; 12288 x 4096 (8 stages), 4 rows, 8.8 against 9.3, 8 rows 10.6 against 9.3; 20000 x 4096
+// (9 stages), 2 rows, 12.4 against 12.9, 8 rows 14.1 against 12.9.
 constexpr uint32_t kMxFusedRows = 16;
 constexpr uint32_t kMxFusedWork = 32;       // rows times stages
 constexpr uint32_t kMxBars = 2 * kMxMaxStages + 5 + kMxMaxSlots + 2 * kMxMaxScales;
