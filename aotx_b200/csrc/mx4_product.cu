@@ -1385,9 +1385,10 @@ static MxPlan plan_of(const Mx4Product &p, uint32_t sms, bool quantises)
         plan.ntok = up_to((typical + parts - 1u) / parts, 16u);
     }
     const unsigned long long tiles = tok_tiles() * row_tiles;
-    // Few tiles, and the host knows how many: clusters that share a tile, else a tile a block.
-    if (!by_expert && (p.m_dev == nullptr || tok_tiles() == 1ull)) {
-        for (uint32_t c = 8u; c >= 2u && plan.ntok <= kMxClusterTok; c >>= 1) {
+    // Few tiles: clusters that share one, if the host knows how many there are, else a tile a block (fewer, if the device finds fewer).
+    if (!by_expert) {
+        const bool known = p.m_dev == nullptr || tok_tiles() == 1ull;
+        for (uint32_t c = 8u; c >= 2u && known && plan.ntok <= kMxClusterTok; c >>= 1) {
             const uint32_t runs = c == 8u ? kMxClustersOf8 : c == 4u ? kMxClustersOf4 : kMxClustersOf2;
             if (tiles <= (plan.ntok <= kMxTwoClusterTok ? 2u * runs : runs) && steps >= (c == 2u ? 2u : c * kMxClusterSteps)) {
                 plan.form = plan.ntok <= kMxTwoClusterTok ? kMxTwo : kMxOne;

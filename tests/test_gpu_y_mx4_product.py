@@ -401,3 +401,34 @@ def test_tensors_past_four_gigabytes(ctx):
     rows64, cols64 = _mx4.values(x.codes[-5:].cpu().numpy(), x.scales[:, -5:].contiguous().cpu().numpy()), \
         _mx4.values(w.codes[-200:].cpu().numpy(), w.scales[:, -200:].contiguous().cpu().numpy())
     assert np.array_equal(y[-5:, -200:].cpu().numpy(), (rows64 @ cols64.T).astype(np.float32))
+
+
+# clusters whose blocks share an SM; x in as many parts as there are SMs or clusters for; a tile a block, up to 256 wide; pairs of blocks
+# for one part of x, whole and cut
+DEALT = [(12288, 320, 16), (18432, 512, 1), (6100, 4128, 8), (2500, 8192, 20), (512, 640, 512), (2048, 1056, 250), (5120, 288, 200),
+         (8192, 288, 512), (12160, 544, 250), (18432, 288, 256), (19456, 800, 96), (19001, 352, 65), (20000, 1312, 128),
+         (10240, 1056, 400)]
+
+
+@pytest.mark.parametrize("n,k,m", DEALT)
+def test_exact_sums_however_the_tiles_are_dealt(ctx, n, k, m):
+    test_exact_sums(ctx, n, k, m)
+
+
+@pytest.mark.parametrize("n,k,m,live", [(2560, 8192, 2048, 100), (2560, 8192, 2048, 0), (2560, 8192, 2048, 1999), (2560, 8192, 1500, 100),
+                                        (6144, 512, 200, 70), (6144, 512, 200, 200), (6144, 512, 200, 130)])
+def test_fewer_tiles_than_the_launch_provides_for(ctx, n, k, m, live):
+    """The device finds fewer tiles than the host dealt: several blocks share one, and more than one leaves its sums to the owner.
+    (Exact, as in test_exact_sums.)"""
+    torch = torch_mod()
+    w, x = random_codes(n, k, n + k, -2, 2), random_codes(m, k, m + k + 1, -2, 2)
+    want = _mx4.values(*x)[:live] @ _mx4.values(*w).T
+    y = torch.full((m, n), GUARD, device="cuda")
+    ctx.mx4_matmul(tensor(*w), tensor(*x), m_dev=torch.tensor([live], dtype=torch.int32, device="cuda"), y=y)
+    assert np.array_equal(y[:live].cpu().numpy(), want.astype(np.float32))
+    assert (y[live:] == GUARD).all()
+
+
+@pytest.mark.parametrize("counts,n,k", [([3, 2], 128, 8192), ([1], 384, 8192), ([70] * 8, 2560, 544), ([0, 200, 96, 65, 1, 97, 0, 33], 2600, 1056)])
+def test_grouped_however_the_tiles_are_dealt(ctx, counts, n, k):
+    grouped(ctx, counts, n, k)
