@@ -80,10 +80,17 @@ constexpr uint32_t kMxTwoClusterTok = 32;
 constexpr uint32_t kMxClustersOf8 = 12;
 constexpr uint32_t kMxClustersOf4 = 32;
 constexpr uint32_t kMxClustersOf2 = 72;
-constexpr uint32_t kMxClusterSteps = 4;     // steps of a block of a larger cluster, at least (2 gain nothing)
+// Steps of a block of a larger cluster, at least (2 or 3: the same; with 6, 1024 x 4096 by 1 row takes 6.8 us, not 4.9).
+constexpr uint32_t kMxClusterSteps = 4;
+// Steps of a tile that a cluster of two shares, at least: up to kMxTwoClusterTok rows of x per tile, and more.  (Time by clusters and with
+// a block a tile: 8192 x 1024 by 8 rows 4.7 and 4.2 us, x 2048, in 16 bits, 1 row 5.9 and 6.1; x 1024 by 64 rows 6.6 and 4.7, x 2560 7.6 and
+// 6.6, x 4096 8.7 both.)
+constexpr uint32_t kMxClusterSteps2 = 7;
+constexpr uint32_t kMxClusterSteps2Wide = 14;
 // And rows of x per tile, at most.  Narrower tiles come first where there are clusters for all: less to exchange (512 x 2048 by 128 rows
-// in one part 7.3 us, in two 5.5, in four 4.8).
-constexpr uint32_t kMxClusterTok = 128;
+// in one part 7.3 us, in two 5.5, in four 4.8; 6144 x 4096 by 100 rows in one part by clusters 9.4, in three, a block each, 8.8; 8192 x 2048
+// by 128 rows 9.5 and 6.7; but 6144 x 8192 by 100 rows 13.0 and 14.0).
+constexpr uint32_t kMxClusterTok = 64;
 // What the kernel quantises of x itself: few rows, and few stages of them.  Every block turns the stages that it needs by itself; a
 // launch of its own costs a microsecond more than the product alone.  4096 x 4096 (4 stages a block), 1 row, 6.4 us against 7.3 apart, 8
 // rows 6.9 against 7.4, 16 rows 9.2 against 7.5; 12288 x 4096 (8 stages), 4 rows, 8.8 against 9.3, 8 rows 10.6 against 9.3; 20000 x 4096
@@ -1371,7 +1378,7 @@ static MxPlan plan_of(const Mx4Product &p, uint32_t sms, bool quantises)
     } else {
         uint32_t parts = (typical + kMxMaxTok - 1u) / kMxMaxTok;
         if (!by_expert) {
-            const uint32_t most = (p.m + kMxTwoClusterTok - 1u) / kMxTwoClusterTok;
+            const uint32_t most = (p.m + kMxClusterTok - 1u) / kMxClusterTok;
             const uint32_t room = sms / row_tiles < most ? sms / row_tiles : most;
             parts = room > parts ? room : parts;
             for (uint32_t tok = kMxTwoClusterTok; tok <= kMxClusterTok; tok *= 2u) {
@@ -1389,8 +1396,10 @@ static MxPlan plan_of(const Mx4Product &p, uint32_t sms, bool quantises)
     if (!by_expert) {
         const bool known = p.m_dev == nullptr || tok_tiles() == 1ull;
         for (uint32_t c = 8u; c >= 2u && known && plan.ntok <= kMxClusterTok; c >>= 1) {
+            const uint32_t least = c != 2u ? c * kMxClusterSteps
+                : plan.ntok <= kMxTwoClusterTok ? kMxClusterSteps2 : kMxClusterSteps2Wide;
             const uint32_t runs = c == 8u ? kMxClustersOf8 : c == 4u ? kMxClustersOf4 : kMxClustersOf2;
-            if (tiles <= (plan.ntok <= kMxTwoClusterTok ? 2u * runs : runs) && steps >= (c == 2u ? 2u : c * kMxClusterSteps)) {
+            if (tiles <= (plan.ntok <= kMxTwoClusterTok ? 2u * runs : runs) && steps >= least) {
                 plan.form = plan.ntok <= kMxTwoClusterTok ? kMxTwo : kMxOne;
                 plan.cluster = c;
                 plan.grid = (uint32_t)tiles * c;
