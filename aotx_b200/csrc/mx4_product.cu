@@ -61,16 +61,20 @@ constexpr uint32_t kMxMaxScales = 16;       // stages whose scales are on their 
 constexpr uint32_t kMxMaxSlots = 9;         // stages of x that stay
 constexpr uint32_t kMxScaleBlock = 512;     // scales of 128 rows and 128 values
 constexpr uint32_t kMxEpilogueStage = 16u * 32u * 4u;  // per storing warp
+// Tiles are dealt whole where what the blocks then lose, waiting for those with one more, is no more than this depth on average; a cut costs
+// as much.  (36864 x 2048 by 300 rows 17.6 us, with tiles cut 21.8; 19456 x 2560 15.5 and 16.6; 128 experts of 2048 x 768, 4096 pairs,
+// 28.7 and 32.9.  By 4096 instead: 28672 x 8192 by 128 rows 28.9, not 27.2; by 2048: 14336 x 4096 by 512 rows 22.7, not 21.5.)
+constexpr uint32_t kMxCutDepth = 3000;
 // A run is cut from a tile only if it has as many steps (by expert 4, 8 or 16 differ by less than 2 %).
 constexpr uint32_t kMxFewSteps = 8;
 // Rows of x per tile of a pair of blocks, at most: two accumulators beside the scales.  (28672 x 4096 by 300 rows 30.3 us, with 128
 // 34.4; by 2048 rows 118 and 132.)
 constexpr uint32_t kMxPairTok = 192;
-// Rows of x that pairs take, at least.  (19456 x 2560 by 96 rows 10.5 us, single blocks 11.7; 28672 x 4096 by 192 rows 21.6 and 23.7, by
-// 2048 rows 118 and 144; by 48 rows 15.7 and 14.0.  128 experts of 1536 x 2048 with 96 rows each 55 and 64, with 32 the same.)
+// Rows of x that pairs take, at least.  (40960 x 2048 by 72 rows 12.1 us, single blocks 13.3, by 128 rows 13.3 and 14.9; 28672 x 4096 by
+// 128 rows 16.9 and 17.2, by 2048 rows 118 and 144; by 48 rows 15.7 and 14.0.  128 experts of 1536 x 2048 with 96 rows each 55 and 64.)
 constexpr uint32_t kMxPairFrom = 65;
 // Rows of x per tile where two blocks share an SM, at most.  (28672 x 4096 by 8 rows 13.4 us, a block to an SM 14.5; by 64 rows 15.0 and
-// 15.9; 65536 x 4096 by 96 rows 34.3 and 31.7; 128 experts of 1536 x 2048, 64 pairs, 19.6 and 21.8.)
+// 15.7; 20480 x 2048 by 48 rows 7.5 and 9.4; but 40960 x 4096 by 64 rows, cut, 23.5 and 21.0, and 65536 x 4096 by 96 rows 34.3 and 31.7.)
 constexpr uint32_t kMxTwoTok = 64;
 // And where they are a cluster's.  (18432 x 4096 by 1 row 10.7 us, a block to an SM 12.0; by 64 rows 13.3 and 11.1.)
 constexpr uint32_t kMxTwoClusterTok = 32;
@@ -311,6 +315,14 @@ __host__ __device__ __forceinline__ unsigned long long mx_workers(unsigned long 
     const uint32_t few = steps < kMxFewSteps / parts ? steps : kMxFewSteps / parts;
     const unsigned long long workers = units / few;
     return workers != 0ull ? workers : 1ull;
+}
+
+// Are `tiles` tiles of depth k dealt whole to `blocks` blocks?  Where what then waits for the block with the most of them is less than
+// cutting tiles costs.
+__device__ __forceinline__ bool mx_whole(uint32_t tiles, uint32_t blocks, uint32_t k)
+{
+    const unsigned long long each = (tiles + blocks - 1u) / blocks;
+    return (each * blocks - tiles) * k <= (unsigned long long)kMxCutDepth * blocks;
 }
 
 // The pieces of a run: a tile and the steps [from, to) of its depth.
@@ -737,17 +749,19 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         tiles = tok_tiles * row_tiles;
     }
     const bool early = !waited && args.weights_late == 0u;
-    const unsigned long long units = (unsigned long long)tiles * steps;
+    const bool whole = !stays && mx_whole(tiles, workers, args.k);
+    const unsigned long long units = whole ? tiles : (unsigned long long)tiles * steps;
     MxPieces mine;
     if (clusters) {
         const unsigned long long first = (unsigned long long)(blockIdx.x / args.cluster) * steps;
         mine.set(first + mx_run_begin(rank, args.cluster, steps), first + mx_run_begin(rank + 1u, args.cluster, steps), steps);
     } else {
         // (the device may know of fewer tiles than the launch provided for)
-        const unsigned long long enough = mx_workers(units, steps, kParts);
+        const unsigned long long enough = whole ? units : mx_workers(units, steps, kParts);
+        const uint32_t unit = whole ? steps : 1u;
         workers = enough < workers ? (uint32_t)enough : workers;
         if (worker < workers) {
-            mine.set(mx_run_begin(worker, workers, units), mx_run_begin(worker + 1u, workers, units), steps);
+            mine.set(mx_run_begin(worker, workers, units) * unit, mx_run_begin(worker + 1u, workers, units) * unit, steps);
         } else {
             mine.set(0ull, 0ull, steps);
         }
@@ -1370,11 +1384,12 @@ static MxPlan plan_of(const Mx4Product &p, uint32_t sms, bool quantises)
         }
     }
     // Rows of x per tile: equal parts of at most 256, more of them while there is an SM for each tile, or few enough for clusters.  By
-    // expert what one has on average, twice that for few: a wider tile reads weights less often and is stored by fewer blocks (128
-    // experts of 2048 x 768 with 32 rows each, by 32 rows 32.7 us, by 64 34.7; of 1536 x 2048 with 16 each, by 16 43.8, by 32 41.8).
+    // expert half as many again as one has on average, so that most need one tile (128 experts of 1536 x 2048 with 32 rows each, by 48
+    // rows 41.8 us, by 32 44.9, by 64 43.5; with 16 rows each, by 32 38.9, by 16 41.0).
     const uint32_t steps = steps_of(p.k, kMxOne);
-    if (by_expert && typical <= kMxClusterTok / 2u) {
-        plan.ntok = up_to(typical > 32u ? typical : 2u * typical < 32u ? 2u * typical : 32u, 16u);
+    if (by_expert && typical <= kMxTwoTok) {
+        const uint32_t ample = typical + typical / 2u;
+        plan.ntok = up_to(ample < kMxTwoTok ? ample : kMxTwoTok, 16u);
     } else {
         uint32_t parts = (typical + kMxMaxTok - 1u) / kMxMaxTok;
         if (!by_expert) {
