@@ -61,8 +61,8 @@ constexpr uint32_t kMxMaxScales = 16;       // stages whose scales are on their 
 constexpr uint32_t kMxMaxSlots = 9;         // stages of x that stay
 constexpr uint32_t kMxScaleBlock = 512;     // scales of 128 rows and 128 values
 constexpr uint32_t kMxEpilogueStage = 16u * 32u * 4u;  // per storing warp
-// Tiles are dealt whole where what the blocks then lose, waiting for those with one more, is no more than this depth on average; a cut costs
-// as much.  (36864 x 2048 by 300 rows 17.6 us, with tiles cut 21.8; 19456 x 2560 15.5 and 16.6; 128 experts of 2048 x 768, 4096 pairs,
+// Tiles are dealt whole where what the blocks then lose, waiting for those with one more, is no more than this depth on average; cutting
+// costs as much.  (36864 x 2048 by 300 rows 17.6 us, with tiles cut 21.8; 19456 x 2560 15.5 and 16.6; 128 experts of 2048 x 768, 4096 pairs,
 // 28.7 and 32.9.  By 4096 instead: 28672 x 8192 by 128 rows 28.9, not 27.2; by 2048: 14336 x 4096 by 512 rows 22.7, not 21.5.)
 constexpr uint32_t kMxCutDepth = 3000;
 // A run is cut from a tile only if it has as many steps (by expert 4, 8 or 16 differ by less than 2 %).
@@ -245,13 +245,12 @@ struct MxTiles {
     uint32_t expert = 0, begin = 0, end = 0;     // of tiles of the expert that the last one belonged to
     uint32_t tok_tiles = 0;
     uint32_t row_tile = 0, tok_tile = 0;         // the next one
-    bool known = false;
+    uint32_t following = 0xFFFFFFFFu;            // its index
 
     __device__ __forceinline__ MxTile next(const MxArgs &args, const MxGroups &groups, uint32_t tile_rows, uint32_t index,
                                            uint32_t all_tok_tiles, uint32_t live)
     {
-        if (!known) {
-            known = true;
+        if (index != following) {
             uint32_t in = index;
             tok_tiles = all_tok_tiles;
             end = 0xFFFFFFFFu;
@@ -284,6 +283,7 @@ struct MxTiles {
             row_tile = 0u;
             tok_tile = 0u;
         }
+        following = index + 1u;
         const uint32_t first = args.offsets != nullptr ? groups.first[expert] : 0u;
         const uint32_t rows = args.offsets != nullptr ? groups.rows[expert] : live;
         const uint32_t skip = tok_tile * args.ntok;
@@ -317,17 +317,10 @@ __host__ __device__ __forceinline__ unsigned long long mx_workers(unsigned long 
     return workers != 0ull ? workers : 1ull;
 }
 
-// Are `tiles` tiles of depth k dealt whole to `blocks` blocks?  Where what then waits for the block with the most of them is less than
-// cutting tiles costs.
-__device__ __forceinline__ bool mx_whole(uint32_t tiles, uint32_t blocks, uint32_t k)
-{
-    const unsigned long long each = (tiles + blocks - 1u) / blocks;
-    return (each * blocks - tiles) * k <= (unsigned long long)kMxCutDepth * blocks;
-}
-
-// The pieces of a run: a tile and the steps [from, to) of its depth.
+// The pieces of a run, and of whole tiles behind it: a tile and the steps [from, to) of its depth.
 struct MxPieces {
     uint32_t left;                 // steps of the run that no piece has had
+    uint32_t then_tile, then_left; // and of the tiles behind it
     uint32_t steps;
     uint32_t tile, from, to;
     bool begun;
@@ -336,16 +329,30 @@ struct MxPieces {
     {
         left = (uint32_t)(end - unit);
         steps = depth;
-        tile = (uint32_t)(unit / depth);
+        tile = unit != 0ull ? (uint32_t)(unit / depth) : 0u;
         from = (uint32_t)(unit - (unsigned long long)tile * depth);
         to = from;
         begun = false;
+        then_left = 0u;
+    }
+
+    __device__ __forceinline__ void then(uint32_t first, uint32_t tiles)
+    {
+        then_tile = first;
+        then_left = tiles * steps;
     }
 
     __device__ __forceinline__ bool next()
     {
         if (left == 0u) {
-            return false;
+            if (then_left == 0u) {
+                return false;
+            }
+            left = then_left;
+            then_left = 0u;
+            tile = then_tile;
+            from = 0u;
+            begun = false;
         }
         if (begun) {
             ++tile;
@@ -749,22 +756,29 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         tiles = tok_tiles * row_tiles;
     }
     const bool early = !waited && args.weights_late == 0u;
-    const bool whole = !stays && mx_whole(tiles, workers, args.k);
-    const unsigned long long units = whole ? tiles : (unsigned long long)tiles * steps;
+    // Each block has `each` whole tiles; those left over go whole to the first blocks, where what the others then lose is less than
+    // cutting tiles costs, or are cut: dealt in runs of steps, which come before a block's whole tiles, so that what cutting adds to
+    // the stores is behind their copies.  (x that stays is quantised for one run: all tiles are cut then.)
+    const uint32_t each = stays ? 0u : tiles / workers;
+    const uint32_t over = tiles - each * workers;
+    const bool whole = !stays && (over == 0u || (unsigned long long)(workers - over) * args.k <= (unsigned long long)kMxCutDepth * workers);
+    const unsigned long long units = whole ? 0ull : (unsigned long long)over * steps;
     MxPieces mine;
+    mine.set(0ull, 0ull, steps);
     if (clusters) {
         const unsigned long long first = (unsigned long long)(blockIdx.x / args.cluster) * steps;
         mine.set(first + mx_run_begin(rank, args.cluster, steps), first + mx_run_begin(rank + 1u, args.cluster, steps), steps);
+    } else if (whole) {
+        mine.then(worker * each + (worker < over ? worker : over), each + (worker < over ? 1u : 0u));
     } else {
         // (the device may know of fewer tiles than the launch provided for)
-        const unsigned long long enough = whole ? units : mx_workers(units, steps, kParts);
-        const uint32_t unit = whole ? steps : 1u;
-        workers = enough < workers ? (uint32_t)enough : workers;
+        const uint32_t cutters = workers;
+        const unsigned long long enough = mx_workers(units, steps, kParts);
+        workers = enough < cutters ? (uint32_t)enough : cutters;
         if (worker < workers) {
-            mine.set(mx_run_begin(worker, workers, units) * unit, mx_run_begin(worker + 1u, workers, units) * unit, steps);
-        } else {
-            mine.set(0ull, 0ull, steps);
+            mine.set(mx_run_begin(worker, workers, units), mx_run_begin(worker + 1u, workers, units), steps);
         }
+        mine.then(over + worker * each, each);
     }
     const uint32_t run = mine.left;
     const uint32_t first_step = mine.from;

@@ -432,3 +432,22 @@ def test_fewer_tiles_than_the_launch_provides_for(ctx, n, k, m, live):
 @pytest.mark.parametrize("counts,n,k", [([3, 2], 128, 8192), ([1], 384, 8192), ([70] * 8, 2560, 544), ([0, 200, 96, 65, 1, 97, 0, 33], 2600, 1056)])
 def test_grouped_however_the_tiles_are_dealt(ctx, counts, n, k):
     grouped(ctx, counts, n, k)
+
+
+@pytest.mark.parametrize("n,k,m,live", [(20480, 4128, 70, None), (20000, 4128, 300, None), (40000, 4128, 9, None), (20480, 4128, 384, 100),
+                                        (38500, 3232, 40, 33)])
+def test_a_few_cut_tiles_before_whole_ones(ctx, n, k, m, live):
+    """Deep tiles, a few more than every block has one of: these few are cut.  (Exact, as in test_exact_sums; the sums in 64 bits are
+    formed on the device, from values that test_gpu_y_mx4_quantize.py checks.)"""
+    torch = torch_mod()
+    w, x = tensor(*random_codes(n, k, n + k, -2, 2)), tensor(*random_codes(m, k, m + k + 1, -2, 2))
+    rows = m if live is None else live
+    x64 = ctx.mx4_dequant(x, dtype=torch.float32).double()[:rows]
+    w64 = ctx.mx4_dequant(w, dtype=torch.float32).double()
+    assert (x64.abs() @ w64.abs().T).max() < 2.0 ** 18
+    y = torch.full((m, n), GUARD, device="cuda")
+    for _ in range(2):
+        y.fill_(GUARD)
+        ctx.mx4_matmul(w, x, y=y, m_dev=None if live is None else torch.tensor([live], dtype=torch.int32, device="cuda"))
+        assert torch.equal(y[:rows], (x64 @ w64.T).float())
+        assert (y[rows:] == GUARD).all()
