@@ -23,11 +23,12 @@
 //     shared memory to the block that adds them and stores it.  (1024 x 4096 by 8 rows 4.5 us, a block a tile 7.1 us; 8192 x 4096 7.6
 //     and 8.4.)
 //   * At most a tile a block: blocks have one each.  Rows of x are cut into as many parts as fill the SMs so (8192 x 4096 by 256 rows
-//     10.1 us, 16.8 in one part; 18432 x 4096 by 200 rows 13.0, in equal runs 19.8).
-//   * Else equal runs of steps, so copies go on from tile to tile and every SM streams to the end.  A tile that is cut between
-//     blocks belongs to the one with its first step: the others leave their sums in the context's scratch and raise a flag per warp (a
+//     10.1 us, in one part and equal runs 16.8; 18432 x 4096 by 200 rows 13.0, in equal runs 19.8).
+//   * Else blocks have the same number of whole tiles, one behind the other, so copies go on from tile to tile.  What is left over goes
+//     to some of them, or is dealt to all as equal runs of steps, before their whole tiles.  A tile that is cut between blocks
+//     belongs to the one with its first step: the others leave their sums in the context's scratch and raise a flag per warp (a
 //     block does so once, with its first tile, before it waits for anyone), and the owner adds them in the order of the
-//     blocks.
+//     blocks.  (14336 x 8192 by 300 rows 25.0 us; with the cuts behind the whole tiles, where nothing hides their stores, 27.8.)
 //   * Two blocks to an SM for few rows of x: one's stores overlap the other's copies.
 //   * A pair of blocks on neighbouring SMs for many: 256 rows of w, each block with its 128 and half of x's rows, so that each code is
 //     read into shared memory half as often.
@@ -65,7 +66,8 @@ constexpr uint32_t kMxEpilogueStage = 16u * 32u * 4u;  // per storing warp
 // costs as much.  (36864 x 2048 by 300 rows 17.6 us, with tiles cut 21.8; 19456 x 2560 15.5 and 16.6; 128 experts of 2048 x 768, 4096 pairs,
 // 28.7 and 32.9.  By 4096 instead: 28672 x 8192 by 128 rows 28.9, not 27.2; by 2048: 14336 x 4096 by 512 rows 22.7, not 21.5.)
 constexpr uint32_t kMxCutDepth = 3000;
-// A run is cut from a tile only if it has as many steps (by expert 4, 8 or 16 differ by less than 2 %).
+// A run is cut from a tile only if it has as many steps.  (With 4, 28672 x 4096 by 300 rows takes 31.1 us, not 28.3, and 20480 x 8192 by 128
+// rows 31.0, not 22.5; with 12, 40960 x 4096 by 8 rows 20.6, not 18.8.)
 constexpr uint32_t kMxFewSteps = 8;
 // Rows of x per tile of a pair of blocks, at most: two accumulators beside the scales.  (28672 x 4096 by 300 rows 30.3 us, with 128
 // 34.4; by 2048 rows 118 and 132.)
