@@ -82,7 +82,7 @@ constexpr uint32_t kMxTwoTok = 64;
 constexpr uint32_t kMxTwoClusterTok = 32;
 // Tiles of a product that is multiplied by clusters, at most: as many clusters of each size as the GPU runs at the same time, twice as
 // many where two blocks share an SM.  (More wait for the first to end: 4096 x 8192 by 1 row, 32 tiles, by eights 8.5 us, by fours
-// 7.9; 12288 x 4096, 96 tiles, by pairs with a block to an SM 15.4, with two 8.6.)
+// 7.9; 12288 x 4096, 96 tiles, by twos with a block to an SM 15.4, with two blocks 8.6.)
 constexpr uint32_t kMxClustersOf8 = 12;
 constexpr uint32_t kMxClustersOf4 = 32;
 constexpr uint32_t kMxClustersOf2 = 72;
