@@ -6,8 +6,11 @@
 
 namespace q8 {
 
-constexpr uint32_t kOrderThreads = 1024;
-constexpr uint32_t kOrderWarps = kOrderThreads / 32u;
+// Warps: 32, or 8 for few pairs, which are started and synchronised sooner (64 pairs 2.3 us, 512 2.9; with 32 warps, and lanes for warps in
+// the running totals, 3.3 and 3.8).
+constexpr uint32_t kOrderWarps = 32;
+constexpr uint32_t kOrderFewWarps = 8;
+constexpr uint32_t kOrderFewPairs = 1024;
 constexpr uint32_t kOrderAhead = 4;          // selections per lane whose loads are issued together
 constexpr uint32_t kOrderStaged = 32768;     // pairs whose order is made in shared memory, at most
 
@@ -40,18 +43,19 @@ __device__ __forceinline__ uint32_t order_same(uint32_t e, uint32_t bits)
 }
 
 // One block; latency bounds it, and the way of scattered words through one SM: so the order is made in shared memory where it
-// fits and goes out in rows (512 tokens with 8 of 128 experts 6.7 us, without 7.6; 8 tokens 3.4 us).  Each warp takes a run of
-// the pairs and counts them by expert; then warp by warp of eight experts, a lane for each of the 32 warps, running totals over the
-// warps; running totals over the experts give each warp its first place per expert; then it places its pairs, lanes in order
-// within a step (lanes with the same expert find each other by ballots).
-__global__ void __launch_bounds__(kOrderThreads)
+// fits and goes out in rows (512 tokens with 8 of 128 experts 6.0 us, straight to memory 0.9 more).  Each warp takes a run of
+// the pairs and counts them by expert; running totals over the warps, a thread for each expert, and then over the experts give
+// each warp its first place per expert; then it places its pairs, lanes in order within a step (lanes with the same expert find each
+// other by ballots).
+template <uint32_t WARPS>
+__global__ void __launch_bounds__(WARPS * 32u)
 mx4_order_kernel(const uint32_t *ids, uint32_t tokens_max, const uint32_t *tokens_dev, uint32_t used, uint32_t experts,
                  uint32_t *__restrict__ order, uint32_t *__restrict__ token_of, uint32_t *__restrict__ offsets, bool staged)
 {
     extern __shared__ uint32_t sorted[];
     // (an odd distance of rows: a column's words lie in different banks)
-    __shared__ uint32_t place[kOrderWarps][kMx4MaxExperts + 1u];
-    __shared__ uint32_t count[kMx4MaxExperts];
+    __shared__ uint32_t place[WARPS][kMx4MaxExperts + 1u];
+    __shared__ uint32_t sums[kMx4MaxExperts / 32u];
     __shared__ uint32_t begin_of[kMx4MaxExperts];
     __shared__ uint32_t placed;
     const uint32_t warp = threadIdx.x >> 5;
@@ -69,7 +73,7 @@ mx4_order_kernel(const uint32_t *ids, uint32_t tokens_max, const uint32_t *token
     }
     const uint32_t all = tokens_max * used;
     const uint32_t pairs = tokens * used;
-    const uint32_t per_warp = ((pairs + kOrderWarps - 1u) / kOrderWarps + 31u) / 32u * 32u;
+    const uint32_t per_warp = ((pairs + WARPS - 1u) / WARPS + 31u) / 32u * 32u;
     const uint32_t begin = warp * per_warp < pairs ? warp * per_warp : pairs;
     const uint32_t end = begin + per_warp < pairs ? begin + per_warp : pairs;
     const uint32_t bits = 32u - (uint32_t)__clz((int)(experts - 1u));
@@ -84,55 +88,41 @@ mx4_order_kernel(const uint32_t *ids, uint32_t tokens_max, const uint32_t *token
         }
     }
     __syncthreads();
-    // eight experts a warp, lane w their pairs of warp w
-    {
-        uint32_t mine[8], through[8];
+    // a thread an expert: running totals over the warps, then over the experts
+    static_assert(WARPS * 32u >= kMx4MaxExperts, "a thread for each expert");
+    const uint32_t mine = threadIdx.x;
+    uint32_t total = 0u, through = 0u;
+    if (mine < kMx4MaxExperts) {
+        uint32_t here[WARPS];
 #pragma unroll
-        for (uint32_t i = 0; i < 8u; ++i) {
-            mine[i] = place[lane][warp * 8u + i];
-            through[i] = mine[i];
+        for (uint32_t w = 0; w < WARPS; ++w) {
+            here[w] = place[w][mine];
         }
 #pragma unroll
-        for (uint32_t step = 1u; step < 32u; step <<= 1) {
-#pragma unroll
-            for (uint32_t i = 0; i < 8u; ++i) {
-                const uint32_t below = __shfl_up_sync(0xFFFFFFFFu, through[i], step);
-                through[i] += lane >= step ? below : 0u;
-            }
+        for (uint32_t w = 0; w < WARPS; ++w) {
+            place[w][mine] = total;
+            total += here[w];
         }
-#pragma unroll
-        for (uint32_t i = 0; i < 8u; ++i) {
-            place[lane][warp * 8u + i] = through[i] - mine[i];
-            if (lane == 31u) {
-                count[warp * 8u + i] = through[i];
-            }
-        }
-    }
-    __syncthreads();
-    if (warp == 0u) {
-        // eight experts a lane
-        uint32_t sum[8], total = 0u;
-#pragma unroll
-        for (uint32_t i = 0; i < 8u; ++i) {
-            sum[i] = total;
-            total += count[lane * 8u + i];
-        }
-        uint32_t through = total;
+        through = total;
 #pragma unroll
         for (uint32_t step = 1u; step < 32u; step <<= 1) {
             const uint32_t below = __shfl_up_sync(0xFFFFFFFFu, through, step);
             through += lane >= step ? below : 0u;
         }
-#pragma unroll
-        for (uint32_t i = 0; i < 8u; ++i) {
-            const uint32_t ex = lane * 8u + i;
-            const uint32_t at = through - total + sum[i];
-            begin_of[ex] = at;
-            if (ex <= experts) {
-                offsets[ex] = at;
-            }
-        }
         if (lane == 31u) {
+            sums[warp] = through;
+        }
+    }
+    __syncthreads();
+    if (mine < kMx4MaxExperts) {
+        for (uint32_t w = 0; w < warp; ++w) {
+            through += sums[w];
+        }
+        begin_of[mine] = through - total;
+        if (mine <= experts) {
+            offsets[mine] = through - total;
+        }
+        if (mine == kMx4MaxExperts - 1u) {
             placed = through;
             if (experts == kMx4MaxExperts) {
                 offsets[kMx4MaxExperts] = through;
@@ -174,7 +164,7 @@ mx4_order_kernel(const uint32_t *ids, uint32_t tokens_max, const uint32_t *token
     }
     if (staged) {
         __syncthreads();
-        for (uint32_t at = threadIdx.x; at < placed; at += kOrderThreads) {
+        for (uint32_t at = threadIdx.x; at < placed; at += WARPS * 32u) {
             const uint32_t p = sorted[at];
             order[at] = p;
             if (token_of != nullptr) {
@@ -182,7 +172,7 @@ mx4_order_kernel(const uint32_t *ids, uint32_t tokens_max, const uint32_t *token
             }
         }
     }
-    for (uint32_t at = placed + threadIdx.x; at < all; at += kOrderThreads) {
+    for (uint32_t at = placed + threadIdx.x; at < all; at += WARPS * 32u) {
         order[at] = 0xFFFFFFFFu;
         if (token_of != nullptr) {
             token_of[at] = 0xFFFFFFFFu;
@@ -194,14 +184,19 @@ cudaError_t launch_mx4_order(cudaStream_t stream, bool overlap, const uint32_t *
                              const uint32_t *tokens_dev, uint32_t used, uint32_t experts, uint32_t *order, uint32_t *token_of,
                              uint32_t *offsets)
 {
+    auto launch = [&](auto kernel, uint32_t warps, bool staged) {
+        return launch_kernel_early(overlap, kernel, dim3(1), warps * 32u, staged ? tokens * used * 4u : 0u, stream, ids, tokens, tokens_dev,
+                                   used, experts, order, token_of, offsets, staged);
+    };
+    if (tokens * used <= kOrderFewPairs) {
+        return launch(mx4_order_kernel<kOrderFewWarps>, kOrderFewWarps, true);
+    }
     static unsigned long long configured = 0ull;
-    const cudaError_t err = allow_shared_memory(mx4_order_kernel, kOrderStaged * 4u, &configured);
+    const cudaError_t err = allow_shared_memory(mx4_order_kernel<kOrderWarps>, kOrderStaged * 4u, &configured);
     if (err != cudaSuccess) {
         return err;
     }
-    const bool staged = tokens * used <= kOrderStaged;
-    return launch_kernel_early(overlap, mx4_order_kernel, dim3(1), kOrderThreads, staged ? tokens * used * 4u : 0u, stream, ids, tokens,
-                               tokens_dev, used, experts, order, token_of, offsets, staged);
+    return launch(mx4_order_kernel<kOrderWarps>, kOrderWarps, tokens * used <= kOrderStaged);
 }
 
 } // namespace q8

@@ -451,3 +451,17 @@ def test_a_few_cut_tiles_before_whole_ones(ctx, n, k, m, live):
         ctx.mx4_matmul(w, x, y=y, m_dev=None if live is None else torch.tensor([live], dtype=torch.int32, device="cuda"))
         assert torch.equal(y[:rows], (x64 @ w64.T).float())
         assert (y[rows:] == GUARD).all()
+
+
+@pytest.mark.parametrize("tokens,used,experts", [(128, 8, 128), (129, 8, 256), (1, 1, 256), (1024, 1, 2), (1025, 1, 33)])
+def test_order_at_the_border_of_its_two_forms(ctx, tokens, used, experts):
+    test_order(ctx, tokens, used, experts)
+
+
+def test_order_of_no_tokens(ctx):
+    torch = torch_mod()
+    order, token_of, offsets = ctx.moe_order(torch.empty((0, 4), dtype=torch.int32, device="cuda"), 7)
+    assert order.numel() == 0 and token_of.numel() == 0 and offsets.tolist() == [0] * 8
+    live = torch.zeros(1, dtype=torch.int32, device="cuda")
+    order, token_of, offsets = ctx.moe_order(torch.zeros((400, 4), dtype=torch.int32, device="cuda"), 7, tokens_dev=live)
+    assert (order == -1).all() and (token_of == -1).all() and offsets.tolist() == [0] * 8
