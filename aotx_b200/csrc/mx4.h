@@ -16,14 +16,11 @@ __host__ __device__ inline uint32_t mx4_chunks(uint32_t k)
     return (k + 127u) / 128u;   // words of four scales in a row
 }
 
-// When the launch behind a quantisation may start: a product reads its weights before its own wait (unless they are what the latest
-// quantisation of the context writes).
-constexpr uint32_t kMx4StartBehindStores = 0u;   // what is written may be weights, even of a product on another context
-constexpr uint32_t kMx4StartBehindWait = 1u;     // rows of x by their numbers, which are activations
-constexpr uint32_t kMx4StartAtOnce = 2u;         // the product that the quantisation is part of
+// `own_product`: the launch behind is the product that the quantisation is part of, and may start at once.  Else nothing behind the
+// quantisation starts before it has ended.
 cudaError_t launch_mx4_quantize(cudaStream_t stream, bool overlap, const void *x, int x_dtype, uint32_t x_rows,
                                 unsigned long long ldx, uint32_t k, const uint32_t *rows_of, uint32_t rows,
-                                const uint32_t *rows_dev, void *codes, void *scales, uint32_t start);
+                                const uint32_t *rows_dev, void *codes, void *scales, bool own_product);
 cudaError_t launch_mx4_dequant(cudaStream_t stream, bool overlap, const void *codes, const void *scales,
                                uint32_t total_rows, uint32_t k, uint32_t first_row, uint32_t rows, void *out, int out_dtype);
 

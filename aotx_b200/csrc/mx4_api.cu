@@ -120,8 +120,7 @@ extern "C" int aotx_mx4_quantize(aotx_q8_ctx *ctx, void *stream, const void *x, 
     ctx->written[1] = static_cast<const unsigned char *>(scales);
     ctx->written_bytes[1] = scale_bytes(rows, k);
     return code_of(ctx, q8::launch_mx4_quantize((cudaStream_t)stream, ctx->overlap != 0, x, x_dtype, x_rows, ldx, k, rows_of,
-                                                rows, rows_dev, codes, scales,
-                                                rows_of != nullptr ? q8::kMx4StartBehindWait : q8::kMx4StartBehindStores));
+                                                rows, rows_dev, codes, scales, false));
 }
 
 extern "C" int aotx_mx4_dequant(aotx_q8_ctx *ctx, void *stream, const void *codes, const void *scales, uint32_t total_rows,
@@ -209,7 +208,7 @@ extern "C" int aotx_mx4_linear(aotx_q8_ctx *ctx, void *stream, const void *w_cod
         unsigned char *scales = codes + (code_bytes(m, k) + 255u) / 256u * 256u;
         const OnDevice on(ctx);
         const cudaError_t err = q8::launch_mx4_quantize((cudaStream_t)stream, ctx->overlap != 0, x, x_dtype, m, ldx, k, nullptr, m,
-                                                        m_dev, codes, scales, q8::kMx4StartAtOnce);
+                                                        m_dev, codes, scales, true);
         return err != cudaSuccess ? fail(ctx, err)
              : aotx_mx4_matmul(ctx, stream, w_codes, w_scales, n, k, codes, scales, m, m_dev, y, y_dtype, epilogue);
     }

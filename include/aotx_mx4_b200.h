@@ -36,7 +36,10 @@ extern "C" {
  *
  * The scale of a block is 2^(floor(log2 a) - 2), a the block's largest magnitude, and no smaller than 2^-127 (a block of
  * zeros has that scale); values are divided by it, rounded to the nearest code, ties to the even one, and saturate at 6.
- * A block with an infinity or a NaN gets scale 255 and codes 0: all of it is NaN. */
+ * A block with an infinity or a NaN gets scale 255 and codes 0: all of it is NaN.
+ *
+ * What is written may be the weights of the product behind it, on this context or another: no launch behind the quantisation starts
+ * before it has ended. */
 int aotx_mx4_quantize(aotx_q8_ctx *ctx, void *stream, const void *x, int x_dtype, uint32_t x_rows, uint64_t ldx, uint32_t k,
                       const uint32_t *rows_of, uint32_t rows, const uint32_t *rows_dev, void *codes, void *scales);
 
@@ -49,8 +52,8 @@ int aotx_mx4_dequant(aotx_q8_ctx *ctx, void *stream, const void *codes, const vo
  * becomes of a sum (`epilogue`: store, add into a float y, gated unit over interleaved rows of w), y's shape and type and the
  * live batch m_dev are as in aotx_q8_matmul_fused; x has m rows, however many of them live.
  *
- * The weights may be read while the operation before the product on the stream is still running (aotx_q8_set_overlap),
- * unless it is a quantisation on this context that writes them. */
+ * The weights may be read while the operation before the product on the stream is still running (aotx_q8_set_overlap): nothing but
+ * aotx_mx4_quantize may write them just before it. */
 int aotx_mx4_matmul(aotx_q8_ctx *ctx, void *stream, const void *w_codes, const void *w_scales, uint32_t n, uint32_t k,
                     const void *x_codes, const void *x_scales, uint32_t m, const uint32_t *m_dev, void *y, int y_dtype,
                     int epilogue);
