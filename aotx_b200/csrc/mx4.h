@@ -41,7 +41,6 @@ struct Mx4Product {
     int y_dtype;
     unsigned int epilogue;
     bool overlap;
-    bool weights_late;         // the operation before this one writes them
     // x in 16 or 32 bits instead of MX4 (null: x_codes and x_scales), where mx4_linear_quantizes
     const void *x;
     int x_dtype;

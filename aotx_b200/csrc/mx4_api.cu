@@ -68,19 +68,6 @@ struct OnDevice {
     }
 };
 
-// Does the latest quantisation of this context write any of these bytes?
-bool fresh(const aotx_q8_ctx *ctx, const void *from, size_t bytes)
-{
-    const uintptr_t begin = reinterpret_cast<uintptr_t>(from);
-    for (int i = 0; i < 2; ++i) {
-        const uintptr_t other = reinterpret_cast<uintptr_t>(ctx->written[i]);
-        if (begin < other + ctx->written_bytes[i] && other < begin + bytes) {
-            return true;
-        }
-    }
-    return false;
-}
-
 size_t code_bytes(uint64_t rows, uint32_t k)
 {
     return (size_t)rows * (k / 2u);
@@ -115,10 +102,6 @@ extern "C" int aotx_mx4_quantize(aotx_q8_ctx *ctx, void *stream, const void *x, 
         return AOTX_Q8_ERR_ARGUMENT;
     }
     const OnDevice on(ctx);
-    ctx->written[0] = static_cast<const unsigned char *>(codes);
-    ctx->written_bytes[0] = code_bytes(rows, k);
-    ctx->written[1] = static_cast<const unsigned char *>(scales);
-    ctx->written_bytes[1] = scale_bytes(rows, k);
     return code_of(ctx, q8::launch_mx4_quantize((cudaStream_t)stream, ctx->overlap != 0, x, x_dtype, x_rows, ldx, k, rows_of,
                                                 rows, rows_dev, codes, scales, false));
 }
@@ -172,7 +155,6 @@ extern "C" int aotx_mx4_matmul(aotx_q8_ctx *ctx, void *stream, const void *w_cod
     p.y_dtype = y_dtype;
     p.epilogue = (unsigned int)epilogue;
     p.overlap = ctx->overlap != 0;
-    p.weights_late = fresh(ctx, w_codes, code_bytes(n, k)) || fresh(ctx, w_scales, scale_bytes(n, k));
     return code_of(ctx, q8::launch_mx4_product((cudaStream_t)stream, ctx->scratch, ctx->sm_count, ctx->launches++, p));
 }
 
@@ -226,7 +208,6 @@ extern "C" int aotx_mx4_linear(aotx_q8_ctx *ctx, void *stream, const void *w_cod
     p.y_dtype = y_dtype;
     p.epilogue = (unsigned int)epilogue;
     p.overlap = ctx->overlap != 0;
-    p.weights_late = fresh(ctx, w_codes, code_bytes(n, k)) || fresh(ctx, w_scales, scale_bytes(n, k));
     p.x = x;
     p.x_dtype = x_dtype;
     p.ldx = ldx;
@@ -282,7 +263,5 @@ extern "C" int aotx_mx4_matmul_grouped(aotx_q8_ctx *ctx, void *stream, const voi
     p.y_dtype = y_dtype;
     p.epilogue = (unsigned int)epilogue;
     p.overlap = ctx->overlap != 0;
-    const uint64_t w_rows = (uint64_t)experts * n;
-    p.weights_late = fresh(ctx, w_codes, code_bytes(w_rows, k)) || fresh(ctx, w_scales, scale_bytes(w_rows, k));
     return code_of(ctx, q8::launch_mx4_product((cudaStream_t)stream, ctx->scratch, ctx->sm_count, ctx->launches++, p));
 }

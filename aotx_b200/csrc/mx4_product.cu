@@ -134,7 +134,6 @@ struct MxArgs {
     uint32_t scale_slots, scale_bytes;
     uint32_t tmem_columns, accumulators;
     uint32_t scale_places;         // stages whose scales are in tensor memory at a time
-    uint32_t weights_late;
     uint32_t wide;                 // rows of y lie on 16-byte boundaries
     // x in 16 or 32 bits, quantised here: its stages stay in `slots` places behind the ring
     const void *x;
@@ -757,7 +756,7 @@ mx4_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         tok_tiles = (live + args.ntok - 1u) / args.ntok;
         tiles = tok_tiles * row_tiles;
     }
-    const bool early = !waited && args.weights_late == 0u;
+    const bool early = !waited;            // weights may come before that
     // Each block has `each` whole tiles; those left over go whole to the first blocks, where what the others then lose is less than
     // cutting tiles costs, or are cut: dealt in runs of steps, which come before a block's whole tiles, so that what cutting adds to
     // the stores is behind their copies.  (x that stays is quantised for one run: all tiles are cut then.)
@@ -1504,7 +1503,6 @@ cudaError_t launch_mx4_product(cudaStream_t stream, const UmmaScratch &scratch, 
     args.ldy = p.epilogue == kEpilogueSwiglu ? p.n / 2u : p.n;
     args.epilogue = p.epilogue;
     args.status = scratch.status;
-    args.weights_late = p.weights_late ? 1u : 0u;
     args.partial = scratch.partial + (unsigned long long)(set & 1u) * scratch.blocks * scratch.tile_floats;
     args.flags = scratch.flags + (unsigned long long)(set & 1u) * scratch.blocks * kFlagWords;
     args.tile_floats = scratch.tile_floats;

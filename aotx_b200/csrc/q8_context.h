@@ -11,8 +11,4 @@ struct aotx_q8_ctx {
     int overlap;
     unsigned int launches;
     q8::UmmaScratch scratch;
-    // The bytes that the latest mx4_quantize of this context wrote: a product whose weights they are waits for them
-    // (other products may read their weights before the work before them has ended).
-    const unsigned char *written[2];
-    size_t written_bytes[2];
 };

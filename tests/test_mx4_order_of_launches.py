@@ -92,3 +92,39 @@ def test_the_product_of_a_linear_call_starts_beside_its_own_quantisation(emu, ct
     assert emu.aotx_mx4_linear(ctx, None, w.codes.ctypes.data, w.scales.ctypes.data, 8, 64, x.x.ctypes.data, F16, 64, 40, None,
                                y.ctypes.data, F32, 0, work.ctypes.data, size) == 0
     assert emu.mx4_emu_released() > 0
+
+
+def launched(emu):
+    """The description that the last product was launched by."""
+    room = C.create_string_buffer(4096)
+    size = emu.mx4_emu_product(room, 4096)
+    return room.raw[:size]
+
+
+@pytest.mark.parametrize("call", ["matmul", "linear", "grouped"])
+def test_a_product_is_launched_alike_whatever_was_quantised_before(emu, ctx, call):
+    """A model's weights are laid out once, its last matrix last: no later product of that matrix is slower for it."""
+    w, x, other = Rows(8, 64, 1), Rows(4, 64, 2), Rows(8, 64, 3)
+    y = memory(4 * 8 * 4)
+    offsets = np.array([0, 4], np.int32)
+
+    def multiply():
+        if call == "matmul":
+            code = emu.aotx_mx4_matmul(ctx, None, w.codes.ctypes.data, w.scales.ctypes.data, 8, 64, x.codes.ctypes.data,
+                                       x.scales.ctypes.data, 4, None, y.ctypes.data, F32, 0)
+        elif call == "linear":
+            code = emu.aotx_mx4_linear(ctx, None, w.codes.ctypes.data, w.scales.ctypes.data, 8, 64, x.x.ctypes.data, F16, 64, 4,
+                                       None, y.ctypes.data, F32, 0, None, 0)
+        else:
+            code = emu.aotx_mx4_matmul_grouped(ctx, None, w.codes.ctypes.data, w.scales.ctypes.data, 1, 8, 64,
+                                               x.codes.ctypes.data, x.scales.ctypes.data, 4, offsets.ctypes.data, None, 4,
+                                               y.ctypes.data, F32, 0)
+        assert code == 0
+        return launched(emu)
+
+    x.quantize(emu, ctx)
+    other.quantize(emu, ctx)
+    before = multiply()
+    w.quantize(emu, ctx)
+    assert any(before) and multiply() == before
+    assert multiply() == before
