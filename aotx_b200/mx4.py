@@ -295,9 +295,10 @@ class Mx4Calls:
 
     def mx4_moe_ffn(self, w_gate_up, w_down, experts, x, prob, ids, tokens_dev=None, out=None, out_dtype=None):
         """The routed feed-forward step of `moe_ffn_fused` on MX4 weights (gate and up rows of an expert interleaved): the
-        pairs in the experts' order, their rows of x quantised, gate and up by expert with the gated unit, its binary16
-        result quantised, the down product by expert, and the rank-ordered weighted sum.  x is any type that
-        `mx4_quantize` takes; prob [tokens][experts] float32 and ids [tokens][used] as `moe_route` leaves them."""
+        pairs in the experts' order, their rows of x quantised, gate and up by expert with the gated unit, its
+        result (in x's type, which has to hold it: binary16 up to 65504) quantised, the down product by expert, and the
+        rank-ordered weighted sum.  x is any type that `mx4_quantize` takes; prob [tokens][experts] float32 and ids
+        [tokens][used] as `moe_route` leaves them."""
         torch = _torch()
         if x.dim() != 2 or ids.dim() != 2 or ids.shape[0] != x.shape[0] or tuple(prob.shape) != (x.shape[0], experts):
             raise ValueError("x [tokens][hidden], ids [tokens][used], prob [tokens][experts]")
@@ -315,7 +316,7 @@ class Mx4Calls:
             raise ValueError("out is [%d][%d] without gaps" % (tokens, hidden))
         order, token_of, offsets = self.moe_order(ids, experts, tokens_dev=tokens_dev)
         feed = self.mx4_quantize(x, rows=token_of)
-        act = self.mx4_matmul_grouped(w_gate_up, experts, feed, offsets, y_dtype=torch.float16, epilogue=EPILOGUE_SWIGLU)
+        act = self.mx4_matmul_grouped(w_gate_up, experts, feed, offsets, y_dtype=x.dtype, epilogue=EPILOGUE_SWIGLU)
         # (rows that no pair has hold what they held; no expert reads them)
         proj = self.mx4_matmul_grouped(w_down, experts, self.mx4_quantize(act), offsets, y_rows=order, y_dtype=torch.float32)
         return self.moe_combine(proj.view(tokens, used, hidden), prob, ids, tokens_dev=tokens_dev, out=out, out_dtype=out_dtype)
