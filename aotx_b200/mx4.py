@@ -25,25 +25,34 @@ def _torch():
 class Mx4Tensor:
     """`rows` rows of k values: codes uint8 [rows][k / 2] (value 2i in the low four bits of byte i), scales uint8
     [ceil(k / 128)][rows][4] (byte b of (c, r): values 128c + 32b .. of row r, 2^(byte - 127); 255 is NaN; 0 past k)."""
-    __slots__ = ("rows", "k", "device", "_codes", "_scales", "_bytes", "_at")
+    __slots__ = ("rows", "k", "device", "_codes", "_scales", "_bytes", "_behind", "_at", "_count")
 
     def __init__(self, codes, scales):
+        self.rows = None
+        self._bytes = None
+        self._codes, self._scales = codes, scales
+        self._hold()
+
+    def _hold(self):
+        """Looks the two tensors over, and again when they have moved or changed their size."""
         torch = _torch()
+        codes, scales = self._codes, self._scales
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() != 2:
             raise ValueError("codes and scales are uint8, codes [rows][k / 2]")
-        self.rows, self.k = codes.shape[0], 2 * codes.shape[1]
-        if self.k == 0 or self.k % 32 != 0 or tuple(scales.shape) != ((self.k + 127) // 128, self.rows, 4):
+        rows, k = codes.shape[0], 2 * codes.shape[1]
+        if k == 0 or k % 32 != 0 or tuple(scales.shape) != ((k + 127) // 128, rows, 4):
             raise ValueError("k is a multiple of 32 and scales are [ceil(k / 128)][rows][4]")
         if not codes.is_contiguous() or not scales.is_contiguous() or codes.device != scales.device:
             raise ValueError("codes and scales lie without gaps on one device")
-        self.device = codes.device
-        self._codes, self._scales = codes, scales
-        self._bytes = None
+        if self.rows is not None and (rows != self.rows or k != self.k or codes.device != self.device):
+            raise ValueError("codes and scales are no longer %d rows of %d values on %s" % (self.rows, self.k, self.device))
+        self.rows, self.k, self.device = rows, k, codes.device
         self._at = (codes.data_ptr(), scales.data_ptr())
+        self._count = (codes.numel(), scales.numel())
 
     @classmethod
     def empty(cls, rows, k, device):
-        """Both arrays in one allocation; their tensors are made when they are asked for."""
+        """Both arrays in one allocation."""
         if k <= 0 or k % 32 != 0 or rows < 0:
             raise ValueError("k is a multiple of 32")
         return cls._make(rows, k, device)
@@ -54,25 +63,35 @@ class Mx4Tensor:
         t = cls.__new__(cls)
         t.rows, t.k = rows, k
         # (a row of codes is a multiple of 16 bytes, so the scales behind them lie on such a boundary too)
-        codes = rows * (k // 2)
+        t._behind = codes = rows * (k // 2)
         t._bytes = held = torch.empty(codes + (k + 127) // 128 * rows * 4, dtype=torch.uint8, device=device)
         t.device = held.device
-        t._codes = t._scales = None
-        at = held.data_ptr()
-        t._at = (at, at + codes)
         return t
 
     @property
     def codes(self):
-        if self._codes is None:
-            self._codes = self._bytes[:self.rows * (self.k // 2)].view(self.rows, self.k // 2)
-        return self._codes
+        if self._bytes is None:
+            return self._codes
+        return self._bytes[:self._behind].view(self.rows, self.k // 2)
 
     @property
     def scales(self):
-        if self._scales is None:
-            self._scales = self._bytes[self.rows * (self.k // 2):].view((self.k + 127) // 128, self.rows, 4)
-        return self._scales
+        if self._bytes is None:
+            return self._scales
+        return self._bytes[self._behind:].view((self.k + 127) // 128, self.rows, 4)
+
+    def _addresses(self):
+        """Where codes and scales are now: a tensor's storage can be put elsewhere under it (`resize_`, `.data = ...`)."""
+        held = self._bytes
+        if held is not None:
+            at = held.data_ptr()
+            return at, at + self._behind
+        codes, scales, at, count = self._codes, self._scales, self._at, self._count
+        if (codes.data_ptr() != at[0] or scales.data_ptr() != at[1] or codes.numel() != count[0]
+                or scales.numel() != count[1]):
+            self._hold()
+            at = self._at
+        return at
 
 
 def _pointer(t):
@@ -172,7 +191,7 @@ class Mx4Calls:
             raise ValueError("out has %d rows of %d values" % (out.rows, out.k))
         elif out.device != self.device:
             raise self._mx4_elsewhere(out)
-        codes, scales = out._at
+        codes, scales = out._addresses()
         result = self._mx4_quantize_call(
             self._address, self._stream(), x.data_ptr(), code, have, stride, k,
             None if rows is None else self._mx4_words("rows", rows), count,
@@ -199,7 +218,7 @@ class Mx4Calls:
                 raise ValueError("out is [%d][%d] without gaps" % (rows, t.k))
             if out.device != self.device:
                 raise self._mx4_elsewhere(out)
-        codes, scales = t._at
+        codes, scales = t._addresses()
         result = self._mx4_dequant_call(self._address, self._stream(), codes, scales, t.rows, t.k, first_row, rows,
                                         out.data_ptr(), code)
         if result != 0:
@@ -211,8 +230,8 @@ class Mx4Calls:
         """y[m][n] = x . w^T for two MX4 tensors; `m_dev`, `y` and `epilogue` as in `matmul_fused`."""
         self._mx4_pair(w, x.k, x)
         y = self._mx4_result(y, x.rows, self._mx4_width(w.rows, epilogue), y_dtype, epilogue)
-        w_codes, w_scales = w._at
-        x_codes, x_scales = x._at
+        w_codes, w_scales = w._addresses()
+        x_codes, x_scales = x._addresses()
         result = self._mx4_matmul_call(self._address, self._stream(), w_codes, w_scales, w.rows, w.k, x_codes, x_scales, x.rows,
                                        None if m_dev is None else self._mx4_words("m_dev", m_dev, 1), y.data_ptr(),
                                        _dtype_code(y.dtype), epilogue)
@@ -238,7 +257,7 @@ class Mx4Calls:
                 raise ValueError("the workspace has gaps")
             if workspace.device != self.device:
                 raise self._mx4_elsewhere(workspace)
-        w_codes, w_scales = w._at
+        w_codes, w_scales = w._addresses()
         result = self._mx4_linear_call(self._address, self._stream(), w_codes, w_scales, w.rows, k, x.data_ptr(), code, stride,
                                        m, None if m_dev is None else self._mx4_words("m_dev", m_dev, 1), y.data_ptr(),
                                        _dtype_code(y.dtype), epilogue, _pointer(workspace), size)
@@ -283,8 +302,8 @@ class Mx4Calls:
             raise ValueError("y is [rows][%d]" % width)
         rows = x.rows if y is None or y_rows is None else y.shape[0]
         y = self._mx4_result(y, rows, width, y_dtype, epilogue)
-        w_codes, w_scales = w._at
-        x_codes, x_scales = x._at
+        w_codes, w_scales = w._addresses()
+        x_codes, x_scales = x._addresses()
         result = self._mx4_grouped_call(self._address, self._stream(), w_codes, w_scales, experts, n, w.k, x_codes, x_scales,
                                         x.rows, self._mx4_words("offsets", offsets, experts + 1),
                                         self._mx4_words("y_rows", y_rows, x.rows), rows, y.data_ptr(), _dtype_code(y.dtype),
