@@ -8,47 +8,43 @@ same call or, `mx4_linear`, on their way into a product.
 Every method enqueues on the current CUDA stream of PyTorch for the context's device and returns without synchronising.  Like
 the rest of the context's methods they are for one thread at a time; tensors used on several streams are ordered by the caller.
 """
-EPILOGUE_STORE, EPILOGUE_ADD, EPILOGUE_SWIGLU = 0, 1, 2
+EPILOGUE_STORE, EPILOGUE_ADD, EPILOGUE_SWIGLU = EPILOGUES = 0, 1, 2
 
 
 _module = None
+_words = ()
 
 
 def _torch():
-    global _module
+    global _module, _words
     if _module is None:
         import torch
+        _words = (torch.int32, torch.uint32)
         _module = torch
     return _module
 
 
 class Mx4Tensor:
     """`rows` rows of k values: codes uint8 [rows][k / 2] (value 2i in the low four bits of byte i), scales uint8
-    [ceil(k / 128)][rows][4] (byte b of (c, r): values 128c + 32b .. of row r, 2^(byte - 127); 255 is NaN; 0 past k)."""
-    __slots__ = ("rows", "k", "device", "_codes", "_scales", "_bytes", "_behind", "_at", "_count")
+    [ceil(k / 128)][rows][4] (byte b of (c, r): values 128c + 32b .. of row r, 2^(byte - 127); 255 is NaN; 0 past k).
+
+    It shares the storage of the two tensors that it is made of, as a view does: what is written there later is read, storage
+    that grows under it is followed."""
+    __slots__ = ("rows", "k", "device", "_codes", "_scales", "_bytes", "_behind")
 
     def __init__(self, codes, scales):
-        self.rows = None
-        self._bytes = None
-        self._codes, self._scales = codes, scales
-        self._hold()
-
-    def _hold(self):
-        """Looks the two tensors over, and again when they have moved or changed their size."""
         torch = _torch()
-        codes, scales = self._codes, self._scales
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() != 2:
             raise ValueError("codes and scales are uint8, codes [rows][k / 2]")
-        rows, k = codes.shape[0], 2 * codes.shape[1]
-        if k == 0 or k % 32 != 0 or tuple(scales.shape) != ((k + 127) // 128, rows, 4):
+        self.rows, self.k = codes.shape[0], 2 * codes.shape[1]
+        if self.k == 0 or self.k % 32 != 0 or tuple(scales.shape) != ((self.k + 127) // 128, self.rows, 4):
             raise ValueError("k is a multiple of 32 and scales are [ceil(k / 128)][rows][4]")
         if not codes.is_contiguous() or not scales.is_contiguous() or codes.device != scales.device:
             raise ValueError("codes and scales lie without gaps on one device")
-        if self.rows is not None and (rows != self.rows or k != self.k or codes.device != self.device):
-            raise ValueError("codes and scales are no longer %d rows of %d values on %s" % (self.rows, self.k, self.device))
-        self.rows, self.k, self.device = rows, k, codes.device
-        self._at = (codes.data_ptr(), scales.data_ptr())
-        self._count = (codes.numel(), scales.numel())
+        self.device = codes.device
+        # (views of its own: neither another storage for the caller's tensors (`.data = ...`) nor another shape changes what it reads)
+        self._codes, self._scales = codes.detach(), scales.detach()
+        self._bytes = None
 
     @classmethod
     def empty(cls, rows, k, device):
@@ -71,27 +67,22 @@ class Mx4Tensor:
     @property
     def codes(self):
         if self._bytes is None:
-            return self._codes
+            return self._codes.detach()
         return self._bytes[:self._behind].view(self.rows, self.k // 2)
 
     @property
     def scales(self):
         if self._bytes is None:
-            return self._scales
+            return self._scales.detach()
         return self._bytes[self._behind:].view((self.k + 127) // 128, self.rows, 4)
 
     def _addresses(self):
-        """Where codes and scales are now: a tensor's storage can be put elsewhere under it (`resize_`, `.data = ...`)."""
+        """Where codes and scales are now: `resize_` of a tensor with the same storage may have put it elsewhere."""
         held = self._bytes
-        if held is not None:
-            at = held.data_ptr()
-            return at, at + self._behind
-        codes, scales, at, count = self._codes, self._scales, self._at, self._count
-        if (codes.data_ptr() != at[0] or scales.data_ptr() != at[1] or codes.numel() != count[0]
-                or scales.numel() != count[1]):
-            self._hold()
-            at = self._at
-        return at
+        if held is None:
+            return self._codes.data_ptr(), self._scales.data_ptr()
+        at = held.data_ptr()
+        return at, at + self._behind
 
 
 def _pointer(t):
@@ -122,8 +113,7 @@ class Mx4Calls:
         """The address of a device array of 32-bit whole numbers, or none."""
         if t is None:
             return None
-        torch = _torch()
-        if (t.dtype != torch.int32 and t.dtype != torch.uint32) or not t.is_contiguous():
+        if t.dtype not in _words or not t.is_contiguous():
             raise ValueError("%s is int32 or uint32 without gaps" % what)
         if count is not None and t.numel() != count:
             raise ValueError("%s has %d entries, not %d" % (what, t.numel(), count))
@@ -147,14 +137,14 @@ class Mx4Calls:
         return rows, k, max(apart, k)
 
     def _mx4_result(self, y, rows, width, y_dtype, epilogue):
-        if epilogue != EPILOGUE_STORE and epilogue != EPILOGUE_ADD and epilogue != EPILOGUE_SWIGLU:
+        if epilogue not in EPILOGUES:
             raise ValueError("unknown epilogue")
         if y is None:
             if epilogue == EPILOGUE_ADD:
                 raise ValueError("EPILOGUE_ADD adds into a y that the caller gives")
-            torch = _torch()
+            torch = _module or _torch()
             return torch.empty(rows, width, dtype=y_dtype or torch.float32, device=self.device)
-        if tuple(y.shape) != (rows, width) or not y.is_contiguous() or (y_dtype is not None and y.dtype != y_dtype):
+        if y.shape != (rows, width) or not y.is_contiguous() or (y_dtype is not None and y.dtype != y_dtype):
             raise ValueError("y is [%d][%d] without gaps" % (rows, width))
         if y.device != self.device:
             raise self._mx4_elsewhere(y)
@@ -170,10 +160,15 @@ class Mx4Calls:
     def _mx4_pair(self, w, k, x=None):
         if w.k != k:
             raise ValueError("rows of %d and of %d values" % (w.k, k))
-        if w.device != self.device:
-            raise self._mx4_elsewhere(w)
-        if x is not None and x.device != self.device:
-            raise self._mx4_elsewhere(x)
+        # (one object for one device, so that the next call need not compare them)
+        if w.device is not self.device:
+            if w.device != self.device:
+                raise self._mx4_elsewhere(w)
+            w.device = self.device
+        if x is not None and x.device is not self.device:
+            if x.device != self.device:
+                raise self._mx4_elsewhere(x)
+            x.device = self.device
 
     # -- quantisation -----------------------------------------------------------------------------------------------
     def mx4_quantize(self, x, rows=None, rows_dev=None, out=None):
