@@ -9,6 +9,8 @@ Every method enqueues on the current CUDA stream of PyTorch for the context's de
 the rest of the context's methods they are for one thread at a time; tensors used on several streams are ordered by the caller.
 """
 EPILOGUE_STORE, EPILOGUE_ADD, EPILOGUE_SWIGLU = EPILOGUES = 0, 1, 2
+# The library's limits.  (It takes 32-bit numbers, and what is larger would be cut on the way: it is refused before.)
+MAX_DEPTH, MAX_ROWS, MAX_EXPERTS = 1 << 24, (1 << 31) - 1, 256
 
 
 _module = None
@@ -41,6 +43,8 @@ class Mx4Tensor:
             raise ValueError("k is a multiple of 32 and scales are [ceil(k / 128)][rows][4]")
         if not codes.is_contiguous() or not scales.is_contiguous() or codes.device != scales.device:
             raise ValueError("codes and scales lie without gaps on one device")
+        if self.k > MAX_DEPTH or self.rows > MAX_ROWS:
+            raise ValueError("%d rows of %d values" % (self.rows, self.k))
         self.device = codes.device
         # (views of its own: neither another storage for the caller's tensors (`.data = ...`) nor another shape changes what it reads)
         self._codes, self._scales = codes.detach(), scales.detach()
@@ -55,6 +59,8 @@ class Mx4Tensor:
 
     @classmethod
     def _make(cls, rows, k, device):
+        if k > MAX_DEPTH or rows > MAX_ROWS:
+            raise ValueError("%d rows of %d values" % (rows, k))
         torch = _torch()
         t = cls.__new__(cls)
         t.rows, t.k = rows, k
@@ -268,12 +274,12 @@ class Mx4Calls:
         shape = ids.shape
         if len(shape) != 2 or shape[1] == 0:
             raise ValueError("ids is [tokens][used]")
-        if experts <= 0:
-            raise ValueError("no experts")
         tokens, used = shape
+        pairs = tokens * used
+        if experts <= 0 or experts > MAX_EXPERTS or pairs > MAX_ROWS:
+            raise ValueError("%d selections of %d experts" % (pairs, experts))
         at = self._mx4_words("ids", ids)
         # (one allocation and one split: slices of it take 0.7 us more, three allocations 0.3)
-        pairs = tokens * used
         words = torch.empty(2 * pairs + experts + 1, dtype=torch.int32, device=self.device)
         order, token_of, offsets = words.split_with_sizes((pairs, pairs, experts + 1))
         base = words.data_ptr()
@@ -287,7 +293,7 @@ class Mx4Calls:
         """Rows offsets[e] .. offsets[e + 1] of x times expert e's rows of w (w.rows / experts each).  `y_rows`: int32, the row
         of y for each row of x (one outside y is left out).  Rows that no expert has are not written."""
         self._mx4_pair(w, x.k, x)
-        if experts <= 0 or w.rows % experts != 0:
+        if experts <= 0 or experts > MAX_EXPERTS or w.rows % experts != 0:
             raise ValueError("%d rows of w for %d experts" % (w.rows, experts))
         if epilogue == EPILOGUE_ADD:
             raise ValueError("grouped products store or apply the gated unit")
@@ -296,6 +302,8 @@ class Mx4Calls:
         if y is not None and y.dim() != 2:
             raise ValueError("y is [rows][%d]" % width)
         rows = x.rows if y is None or y_rows is None else y.shape[0]
+        if rows >= 1 << 32:
+            raise ValueError("%d rows of y" % rows)
         y = self._mx4_result(y, rows, width, y_dtype, epilogue)
         w_codes, w_scales = w._addresses()
         x_codes, x_scales = x._addresses()

@@ -100,3 +100,42 @@ def test_released_storage_is_passed_on_as_a_null_pointer():
     x.codes.untyped_storage().resize_(0)
     c.mx4_matmul(w, x)
     assert passed(c)[1][0] == 0
+
+
+class OnMeta(Recorded):
+    """Tensors of any size, with nothing in them."""
+    device = torch.device("meta")
+
+
+def blank(*shape, dtype=torch.int32):
+    return torch.empty(shape, dtype=dtype, device="meta")
+
+
+def test_sizes_past_the_limits_are_refused_and_not_cut_to_32_bits():
+    """(The native calls take numbers modulo their width: 2^32 + 64 values would have been 64.)"""
+    c = OnMeta()
+    wide, far = (1 << 32) + 64, (1 << 32) + 5
+    calls = [
+        lambda: c.mx4_quantize(blank(1, wide, dtype=torch.float16)),
+        lambda: c.mx4_quantize(blank(2, 64, dtype=torch.float16), rows=blank(far)),
+        lambda: c.mx4_quantize(blank(2, 64, dtype=torch.float16), rows=blank(1 << 31)),
+        lambda: Mx4Tensor.empty(1, wide, "meta"), lambda: Mx4Tensor.empty(1, (1 << 24) + 32, "meta"),
+        lambda: Mx4Tensor.empty(far, 32, "meta"), lambda: Mx4Tensor.empty(1 << 31, 32, "meta"),
+        lambda: Mx4Tensor(blank(far, 16, dtype=torch.uint8), blank(1, far, 4, dtype=torch.uint8)),
+        lambda: Mx4Tensor(blank(1, wide // 2, dtype=torch.uint8), blank((wide + 127) // 128, 1, 4, dtype=torch.uint8)),
+        lambda: c.moe_order(blank(far, 1), 8), lambda: c.moe_order(blank(1 << 30, 2), 8),
+        lambda: c.moe_order(blank(4, 2), (1 << 32) + 8), lambda: c.moe_order(blank(4, 2), 257),
+        lambda: c.mx4_matmul_grouped(Mx4Tensor.empty(0, 64, "meta"), far, Mx4Tensor.empty(4, 64, "meta"), blank(far + 1)),
+        lambda: c.mx4_matmul_grouped(Mx4Tensor.empty(4, 64, "meta"), 2, Mx4Tensor.empty(4, 64, "meta"), blank(3), y_rows=blank(4),
+                                     y=blank(far, 2, dtype=torch.float32)),
+    ]
+    for i, call in enumerate(calls):
+        with pytest.raises(ValueError):
+            call()
+            raise AssertionError("call %d went through" % i)
+    assert c.calls == []
+    # the limits themselves
+    c.mx4_quantize(blank(1, 1 << 24, dtype=torch.float16))
+    c.mx4_quantize(blank(2, 64, dtype=torch.float16), rows=blank((1 << 31) - 1))
+    c.moe_order(blank((1 << 31) - 1, 1), 256)
+    assert len(c.calls) == 3
