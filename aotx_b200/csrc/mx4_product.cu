@@ -469,8 +469,9 @@ __device__ __forceinline__ void mx_quantize_x(const MxArgs &args, const T *x, ui
 }
 
 // silu(gate) * up.  For a float y as the Q8_0 products form it; for 16 bits by the approximate exponential and reciprocal, which are
-// off by 2^-18 of the result at most for gates from -14 on (2^-15 at -100), against 2^-11 and 2^-8 of the rounding: 6 instructions instead
-// of 20 (28672 x 4096 by 2048 rows 119 us, with the exact unit 137; by 8 rows 13.9 and 14.0).
+// off by 2^-18 of the result at most for gates from -14 on, and by 2^-16 down to -88, against 2^-11 and 2^-8 of the rounding: 6
+// instructions instead of 20 (28672 x 4096 by 2048 rows 119 us, with the exact unit 137; by 8 rows 13.9 and 14.0).  Below -88.73 the
+// exponential is infinite and the result a zero with its sign, in either form, as gate / (1 + expf(-gate)) is in floats.
 template <typename YT>
 __device__ __forceinline__ float mx_gated(float gate, float up)
 {
