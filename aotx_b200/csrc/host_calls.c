@@ -147,6 +147,17 @@ static PyObject *call_mx4_linear(PyObject *self, PyObject *const *args, Py_ssize
     return PyLong_FromLong(code);
 }
 
+static PyObject *call_mx4_linear_workspace_bytes(PyObject *self, PyObject *const *args, Py_ssize_t count)
+{
+    uint64_t v[5];
+    (void)self;
+    if (!take(args, count, "ppnnn", v)) {
+        return NULL;
+    }
+    return PyLong_FromSize_t(((__typeof__(&aotx_mx4_linear_workspace_bytes))PTR(0))(PTR(1), (uint32_t)v[2], (uint32_t)v[3],
+                                                                                   (uint32_t)v[4]));
+}
+
 static PyObject *call_mx4_moe_order(PyObject *self, PyObject *const *args, Py_ssize_t count)
 {
     uint64_t v[11];
@@ -189,6 +200,8 @@ static PyMethodDef methods[] = {
     {"aotx_mx4_dequant", (PyCFunction)(void (*)(void))call_mx4_dequant, METH_FASTCALL, "address, then aotx_mx4_dequant's arguments"},
     {"aotx_mx4_matmul", (PyCFunction)(void (*)(void))call_mx4_matmul, METH_FASTCALL, "address, then aotx_mx4_matmul's arguments"},
     {"aotx_mx4_linear", (PyCFunction)(void (*)(void))call_mx4_linear, METH_FASTCALL, "address, then aotx_mx4_linear's arguments"},
+    {"aotx_mx4_linear_workspace_bytes", (PyCFunction)(void (*)(void))call_mx4_linear_workspace_bytes, METH_FASTCALL,
+     "address, then aotx_mx4_linear_workspace_bytes's arguments"},
     {"aotx_mx4_moe_order", (PyCFunction)(void (*)(void))call_mx4_moe_order, METH_FASTCALL, "address, then aotx_mx4_moe_order's arguments"},
     {"aotx_mx4_matmul_grouped", (PyCFunction)(void (*)(void))call_mx4_matmul_grouped, METH_FASTCALL, "address, then aotx_mx4_matmul_grouped's arguments"},
     {NULL, NULL, 0, NULL},

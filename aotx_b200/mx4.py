@@ -55,7 +55,9 @@ class Mx4Tensor:
         """Both arrays in one allocation."""
         if k <= 0 or k % 32 != 0 or rows < 0:
             raise ValueError("k is a multiple of 32")
-        return cls._make(rows, k, device)
+        t = cls._make(rows, k, device)
+        t.device = t._bytes.device
+        return t
 
     @classmethod
     def _make(cls, rows, k, device):
@@ -66,8 +68,8 @@ class Mx4Tensor:
         t.rows, t.k = rows, k
         # (a row of codes is a multiple of 16 bytes, so the scales behind them lie on such a boundary too)
         t._behind = codes = rows * (k // 2)
-        t._bytes = held = torch.empty(codes + (k + 127) // 128 * rows * 4, dtype=torch.uint8, device=device)
-        t.device = held.device
+        t._bytes = torch.empty(codes + (k + 127) // 128 * rows * 4, dtype=torch.uint8, device=device)
+        t.device = device
         return t
 
     @property
@@ -112,6 +114,9 @@ def _dtype_code(dtype):
 class Mx4Calls:
     """The part of Q8Context that works on MX4 tensors."""
 
+    def _mx4_linear_bytes_call(self, *args):
+        return self.lib.aotx_mx4_linear_workspace_bytes(*args)
+
     def _mx4_elsewhere(self, t):
         return ValueError("a tensor on %s, a context for %s" % (t.device, self.device))
 
@@ -142,19 +147,26 @@ class Mx4Calls:
             raise ValueError("the values of a row lie side by side and rows do not overlap")
         return rows, k, max(apart, k)
 
-    def _mx4_result(self, y, rows, width, y_dtype, epilogue):
+    def _mx4_result(self, y, rows, n, y_dtype, epilogue):
+        """y of `rows` rows for n rows of weights, the caller's or a new one, and the code of its type."""
         if epilogue not in EPILOGUES:
             raise ValueError("unknown epilogue")
+        width = self._mx4_width(n, epilogue) if epilogue == EPILOGUE_SWIGLU else n
         if y is None:
             if epilogue == EPILOGUE_ADD:
                 raise ValueError("EPILOGUE_ADD adds into a y that the caller gives")
             torch = _module or _torch()
-            return torch.empty(rows, width, dtype=y_dtype or torch.float32, device=self.device)
+            if y_dtype is None:
+                y_dtype = torch.float32
+            code = _codes.get(y_dtype)
+            if code is None:
+                code = _dtype_code(y_dtype)
+            return torch.empty(rows, width, dtype=y_dtype, device=self.device), code
         if y.shape != (rows, width) or not y.is_contiguous() or (y_dtype is not None and y.dtype != y_dtype):
             raise ValueError("y is [%d][%d] without gaps" % (rows, width))
         if y.device != self.device:
             raise self._mx4_elsewhere(y)
-        return y
+        return y, _dtype_code(y.dtype)
 
     def _mx4_width(self, n, epilogue):
         if epilogue == EPILOGUE_SWIGLU:
@@ -230,12 +242,12 @@ class Mx4Calls:
     def mx4_matmul(self, w, x, m_dev=None, y=None, y_dtype=None, epilogue=EPILOGUE_STORE):
         """y[m][n] = x . w^T for two MX4 tensors; `m_dev`, `y` and `epilogue` as in `matmul_fused`."""
         self._mx4_pair(w, x.k, x)
-        y = self._mx4_result(y, x.rows, self._mx4_width(w.rows, epilogue), y_dtype, epilogue)
+        y, y_code = self._mx4_result(y, x.rows, w.rows, y_dtype, epilogue)
         w_codes, w_scales = w._addresses()
         x_codes, x_scales = x._addresses()
         result = self._mx4_matmul_call(self._address, self._stream(), w_codes, w_scales, w.rows, w.k, x_codes, x_scales, x.rows,
                                        None if m_dev is None else self._mx4_words("m_dev", m_dev, 1), y.data_ptr(),
-                                       _dtype_code(y.dtype), epilogue)
+                                       y_code, epilogue)
         if result != 0:
             self._check(result)
         return y
@@ -243,12 +255,14 @@ class Mx4Calls:
     def mx4_linear(self, w, x, m_dev=None, y=None, y_dtype=None, epilogue=EPILOGUE_STORE, workspace=None):
         """`mx4_matmul` of w with `mx4_quantize(x)`, up to the order of the float sums; few rows are quantised by the kernel
         that multiplies them."""
-        code = _dtype_code(x.dtype)
+        code = _codes.get(x.dtype)
+        if code is None:
+            code = _dtype_code(x.dtype)
         m, k, stride = self._mx4_rows_in(x)
         self._mx4_pair(w, k)
-        y = self._mx4_result(y, m, self._mx4_width(w.rows, epilogue), y_dtype, epilogue)
+        y, y_code = self._mx4_result(y, m, w.rows, y_dtype, epilogue)
         if workspace is None:
-            size = self.lib.aotx_mx4_linear_workspace_bytes(self._address, w.rows, k, m)
+            size = self._mx4_linear_bytes_call(self._address, w.rows, k, m)
             if size:
                 torch = _torch()
                 workspace = torch.empty(size, dtype=torch.uint8, device=self.device)
@@ -261,7 +275,7 @@ class Mx4Calls:
         w_codes, w_scales = w._addresses()
         result = self._mx4_linear_call(self._address, self._stream(), w_codes, w_scales, w.rows, k, x.data_ptr(), code, stride,
                                        m, None if m_dev is None else self._mx4_words("m_dev", m_dev, 1), y.data_ptr(),
-                                       _dtype_code(y.dtype), epilogue, _pointer(workspace), size)
+                                       y_code, epilogue, _pointer(workspace), size)
         if result != 0:
             self._check(result)
         return y
@@ -298,18 +312,17 @@ class Mx4Calls:
         if epilogue == EPILOGUE_ADD:
             raise ValueError("grouped products store or apply the gated unit")
         n = w.rows // experts
-        width = self._mx4_width(n, epilogue)
         if y is not None and y.dim() != 2:
-            raise ValueError("y is [rows][%d]" % width)
+            raise ValueError("y is [rows][%d]" % self._mx4_width(n, epilogue))
         rows = x.rows if y is None or y_rows is None else y.shape[0]
         if rows >= 1 << 32:
             raise ValueError("%d rows of y" % rows)
-        y = self._mx4_result(y, rows, width, y_dtype, epilogue)
+        y, y_code = self._mx4_result(y, rows, n, y_dtype, epilogue)
         w_codes, w_scales = w._addresses()
         x_codes, x_scales = x._addresses()
         result = self._mx4_grouped_call(self._address, self._stream(), w_codes, w_scales, experts, n, w.k, x_codes, x_scales,
                                         x.rows, self._mx4_words("offsets", offsets, experts + 1),
-                                        self._mx4_words("y_rows", y_rows, x.rows), rows, y.data_ptr(), _dtype_code(y.dtype),
+                                        self._mx4_words("y_rows", y_rows, x.rows), rows, y.data_ptr(), y_code,
                                         epilogue)
         if result != 0:
             self._check(result)

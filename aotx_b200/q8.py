@@ -135,6 +135,7 @@ class Q8Context(Mx4Calls):
         self._mx4_dequant_call = native_call(self.lib, "aotx_mx4_dequant")
         self._mx4_matmul_call = native_call(self.lib, "aotx_mx4_matmul")
         self._mx4_linear_call = native_call(self.lib, "aotx_mx4_linear")
+        self._mx4_linear_bytes_call = native_call(self.lib, "aotx_mx4_linear_workspace_bytes")
         self._mx4_order_call = native_call(self.lib, "aotx_mx4_moe_order")
         self._mx4_grouped_call = native_call(self.lib, "aotx_mx4_matmul_grouped")
         # The current stream as a number.  (Through the Stream object it took 2.4 us of the 8.2 us

@@ -1,9 +1,11 @@
 """What the Python layer of the MX4 tensors hands to the library, on CPU tensors: the types between the steps of a routed layer."""
 import copy
+import ctypes as C
 
 import pytest
 import torch
 
+from aotx_b200 import library
 from aotx_b200.mx4 import Mx4Calls, Mx4Tensor
 
 F32, F16, BF16 = 0, 1, 2
@@ -100,6 +102,19 @@ def test_released_storage_is_passed_on_as_a_null_pointer():
     x.codes.untyped_storage().resize_(0)
     c.mx4_matmul(w, x)
     assert passed(c)[1][0] == 0
+
+
+def test_the_size_of_a_workspace_as_ctypes_gives_it():
+    lib = library.load_library()
+    call = library.native_call(lib, "aotx_mx4_linear_workspace_bytes")
+    assert call.func.__name__ == "aotx_mx4_linear_workspace_bytes"
+    ctx = C.cast(C.create_string_buffer(4096), C.c_void_p).value        # zeros: no SM, so nothing is quantised by the product
+    for n, k, m in ((8, 64, 40), (1, 96, 1 << 24), (8, 33, 40), (0, 64, 40), (8, 64, 0), (1 << 20, 1 << 24, 1 << 20)):
+        assert call(ctx, n, k, m) == lib.aotx_mx4_linear_workspace_bytes(ctx, n, k, m)
+    assert call(ctx, 8, 64, 40) >= 40 * 32 + 40 * 4 and call(None, 8, 64, 40) == 0
+    for wrong in ((ctx, 8, 64), (ctx, 8, 64, 40, 0), (ctx, 8.0, 64, 40), (ctx, None, 64, 40)):
+        with pytest.raises(TypeError):
+            call(*wrong)
 
 
 class OnMeta(Recorded):
