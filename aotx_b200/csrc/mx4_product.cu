@@ -94,8 +94,8 @@ constexpr uint32_t kMxClusterSteps = 4;
 constexpr uint32_t kMxClusterSteps2 = 7;
 constexpr uint32_t kMxClusterSteps2Wide = 14;
 // And rows of x per tile, at most.  Narrower tiles come first where there are clusters for all: less to exchange (512 x 2048 by 128 rows
-// in one part 7.3 us, in two 5.5, in four 4.8; 6144 x 4096 by 100 rows in one part by clusters 9.4, in three, a block each, 8.8; 8192 x 2048
-// by 128 rows 9.5 and 6.7; but 6144 x 8192 by 100 rows 13.0 and 14.0).
+// in one part 7.3 us, in two 5.5, in four 4.7; 6144 x 4096 by 100 rows in one part by clusters 9.4, in two, a block each, 8.7; 8192 x 2048
+// by 128 rows 6.8 and 6.6; but 6144 x 8192 by 100 rows 12.8 and 13.9).
 constexpr uint32_t kMxClusterTok = 64;
 // What the kernel quantises of x itself: few rows, and few stages of them.  Every block turns the stages that it needs by itself; a
 // launch of its own costs a microsecond more than the product alone.  4096 x 4096 (4 stages a block), 1 row, 6.4 us against 7.3 apart, 8
@@ -141,7 +141,7 @@ struct MxArgs {
     uint32_t x_aligned;
     unsigned long long ldx;
     uint32_t slots;                // 0: x is in MX4 and goes through the ring
-    uint32_t cluster;              // blocks that share a tile; 0: the steps of all tiles are dealt in equal runs
+    uint32_t cluster;              // blocks that share a tile; 0: each has whole tiles, and runs of those left over or a whole one more
     uint32_t share;                // columns of the tile that a block of the cluster adds up and stores
     float *partial;                // per block: [row of x][row of w], and its flags
     unsigned int *flags;
@@ -1361,7 +1361,7 @@ static uint32_t row_tiles_of(uint32_t n, MxForm form)
 struct MxPlan {
     MxForm form;
     uint32_t ntok;
-    uint32_t cluster;              // blocks that share a tile; 0: equal runs of steps
+    uint32_t cluster;              // blocks that share a tile; 0: whole tiles, those left over whole or in equal runs of steps
     uint32_t grid;
     uint32_t slots;                // stages of x that a block of mx4_linear keeps, 0: x comes in MX4
 };

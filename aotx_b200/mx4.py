@@ -7,6 +7,8 @@ same call or, `mx4_linear`, on their way into a product.
 
 Every method enqueues on the current CUDA stream of PyTorch for the context's device and returns without synchronising.  Like
 the rest of the context's methods they are for one thread at a time; tensors used on several streams are ordered by the caller.
+A product may read its weights while the operation ahead of it on the stream is still running: what writes them just before it is
+`mx4_quantize`, or launches do not overlap (`set_overlap`).
 """
 EPILOGUE_STORE, EPILOGUE_ADD, EPILOGUE_SWIGLU = EPILOGUES = 0, 1, 2
 # The library's limits.  (It takes 32-bit numbers, and what is larger would be cut on the way: it is refused before.)
